@@ -1,6 +1,7 @@
 // gg_api.hip — the C ABI of libgigagan_amd.so (declared in include/gigagan_amd.h).
 // Argument validation, tile / split-K selection and kernel launches; no allocation, no synchronisation.
 #include "gg_device.h"
+#include "gg_host.h"
 #include "gg_gemm.h"
 #include "gg_gemm2.h"
 #include "gg_conv3.h"
@@ -33,7 +34,7 @@
 
 static thread_local char g_err[512] = "";
 
-static int gg_fail(int code, const char* fmt, ...) {
+int gg_fail(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof(g_err), fmt, ap);
@@ -41,7 +42,7 @@ static int gg_fail(int code, const char* fmt, ...) {
     return code;
 }
 
-static int gg_check_launch() {
+int gg_check_launch() {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) {
         snprintf(g_err, sizeof(g_err), "hip launch error %d: %s", (int)e, hipGetErrorString(e));

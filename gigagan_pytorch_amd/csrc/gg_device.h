@@ -81,6 +81,12 @@ GG_DEVICE f32x4 gg_mfma_16x16x32_bf16(u16x8 a, u16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gg_bf16x8_native, a), __builtin_bit_cast(gg_bf16x8_native, b), c, 0, 0, 0);
 }
 
+// the same contraction on IEEE half operands (v_mfma_f32_32x32x16_f16; raw 16-bit words, the lane mapping of the bf16 form)
+typedef __attribute__((ext_vector_type(8))) _Float16 gg_f16x8_native;
+GG_DEVICE f32x16 gg_mfma_32x32x16_f16(u16x8 a, u16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(gg_f16x8_native, a), __builtin_bit_cast(gg_f16x8_native, b), c, 0, 0, 0);
+}
+
 // ds_read_b64_tr_b16: every lane supplies the LDS address of 4 contiguous bf16 (8-byte aligned); inside each group
 // of 16 lanes, lane i receives element (i & 3) of the quads addressed by lanes 4*j + (i >> 2), j = 0..3 (measured on
 // gfx950 with tests/probes/tr_probe.hip). With lane s pointing at row (s >> 2), columns 4*(s & 3).. of a
@@ -218,6 +224,19 @@ GG_DEVICE float gg_row16_sum(float v) {
 #undef GG_DPP_ADD
     return v;
 }
+// sum / maximum of a lane's value and lane ^ 32's (v_permlane32_swap_b32: one vector instruction; gg_shfl_xor(v, 32) is an LDS round
+// trip). Both lanes get the low half's value first, so both get the same bits.
+GG_DEVICE float gg_sum_xor32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned a = r[0], b = r[1];          // (a bit cast of a vector's element itself reads element 0)
+    return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+GG_DEVICE float gg_max_xor32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned a = r[0], b = r[1];
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+GG_DEVICE void gg_sincospi(float x, float* s, float* c) { sincospif(x, s, c); }
 GG_DEVICE void gg_atomic_add(float* p, float v) { atomicAdd(p, v); }
 // "last workgroup to arrive" ticket: release this workgroup's global writes, take a ticket; the taker of the last ticket sees every
 // other workgroup's writes (acquire) and puts the counter back to zero when it is done
@@ -231,6 +250,7 @@ GG_DEVICE void gg_ticket_reset(unsigned* p) { atomicExch(p, 0u); }
 GG_DEVICE float gg_expf(float x) { return __expf(x); }
 GG_DEVICE float gg_exp2f(float x) { return __builtin_amdgcn_exp2f(x); }     // bare v_exp_f32 (no range fix-ups: x <= 128 here)
 GG_DEVICE bool gg_wave_any(bool pred) { return __builtin_amdgcn_ballot_w64(pred) != 0; }    // wave-uniform result
+GG_DEVICE unsigned long long gg_ballot(bool pred) { return __builtin_amdgcn_ballot_w64(pred); }
 GG_DEVICE float gg_rsqrtf(float x) { return rsqrtf(x); }
 GG_DEVICE float gg_rcpf(float x) { return __builtin_amdgcn_rcpf(x); }      // v_rcp_f32 (1 ulp): `1.f / x` compiles to a ~10-instruction IEEE division
 
@@ -241,6 +261,10 @@ GG_DEVICE float gg_rcpf(float x) { return __builtin_amdgcn_rcpf(x); }      // v_
 // a * b + c with ONE rounding, spelled out: where several unrolled copies of a reduction must give bit-identical results (the same
 // sample in another batch slot), `a * b + c` leaves the contraction into an fma to the compiler, which may decide differently per copy
 GG_HOST_DEVICE float gg_fmaf(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+
+// IEEE half as raw 16-bit words (round-to-nearest-even, as torch's .to(torch.float16))
+GG_HOST_DEVICE float gg_h2f(unsigned short h) { return (float)__builtin_bit_cast(_Float16, h); }
+GG_HOST_DEVICE unsigned short gg_f2h(float f) { return __builtin_bit_cast(unsigned short, (_Float16)f); }
 
 GG_HOST_DEVICE float gg_bf2f(bf16_t h) {
     union { unsigned int u; float f; } x;

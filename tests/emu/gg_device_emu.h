@@ -45,6 +45,7 @@ void gg_emu_launch(dim3 grid, dim3 block, const std::function<void()>& body);
 void gg_emu_syncthreads();
 f32x16 gg_emu_mfma_32x32x16_bf16(u16x8 a, u16x8 b, f32x16 c);
 f32x4 gg_emu_mfma_16x16x32_bf16(u16x8 a, u16x8 b, f32x4 c);
+f32x16 gg_emu_mfma_32x32x16_f16(u16x8 a, u16x8 b, f32x16 c);
 float gg_emu_shfl(float v, int src_lane);
 u16x4 gg_emu_lds_read_tr16(const bf16_t* p);
 
@@ -106,6 +107,7 @@ static inline f32x16 gg_mfma_32x32x16_bf16(u16x8 a, u16x8 b, f32x16 c) {
     return gg_emu_mfma_32x32x16_bf16(a, b, c);
 }
 static inline f32x4 gg_mfma_16x16x32_bf16(u16x8 a, u16x8 b, f32x4 c) { return gg_emu_mfma_16x16x32_bf16(a, b, c); }
+static inline f32x16 gg_mfma_32x32x16_f16(u16x8 a, u16x8 b, f32x16 c) { return gg_emu_mfma_32x32x16_f16(a, b, c); }
 static inline u16x4 gg_lds_read_tr16(const bf16_t* p) { return gg_emu_lds_read_tr16(p); }
 static inline float gg_shfl_xor(float v, int mask) {
     int lane = (int)(threadIdx.x & 63u);
@@ -125,6 +127,12 @@ static inline float gg_wave_sum_all(float v) {     // wave collective; the devic
     { int lane = (int)(threadIdx.x & 63u); v += gg_emu_shfl(v, (lane & ~15) | (15 - (lane & 15))); }
     return (gg_emu_shfl(v, 0) + gg_emu_shfl(v, 16)) + (gg_emu_shfl(v, 32) + gg_emu_shfl(v, 48));
 }
+static inline float gg_sum_xor32(float v) {        // wave collective; the low half's value first, as on the device
+    const float o = gg_shfl_xor(v, 32);
+    return (threadIdx.x & 32u) ? o + v : v + o;
+}
+static inline float gg_max_xor32(float v) { return fmaxf(v, gg_shfl_xor(v, 32)); }
+static inline void gg_sincospi(float x, float* s, float* c) { *s = (float)sin(M_PI * (double)x); *c = (float)cos(M_PI * (double)x); }
 static inline void gg_atomic_add(float* p, float v) { *p += v; }
 static inline unsigned gg_ticket_take(unsigned* p) { return (*p)++; }      // workgroups run one after another on the host
 static inline void gg_ticket_reset(unsigned* p) { *p = 0; }
@@ -135,6 +143,11 @@ static inline bool gg_wave_any(bool pred) {     // wave collective: every fiber 
     float f = pred ? 1.f : 0.f;
     for (int o = 1; o < 64; o <<= 1) f = fmaxf(f, gg_shfl_xor(f, o));
     return f > 0.f;
+}
+static inline unsigned long long gg_ballot(bool pred) {     // wave collective
+    unsigned long long m = 0;
+    for (int i = 0; i < 64; ++i) m |= (unsigned long long)(gg_emu_shfl(pred ? 1.f : 0.f, i) != 0.f) << i;
+    return m;
 }
 static inline float gg_rsqrtf(float x) { return 1.0f / sqrtf(x); }
 static inline float gg_rcpf(float x) { return 1.0f / x; }

@@ -99,7 +99,8 @@ static inline float bf2f_(unsigned short h) {
 // Lane mappings of v_mfma_f32_32x32x16_bf16 as documented in the CDNA4 guide:
 //   A: lane l -> row i = l&31, k = 8*(l>>5)+e ; B: lane l -> col j = l&31, k = 8*(l>>5)+e
 //   D: lane l, reg r -> row i = (r&3) + 8*(r>>2) + 4*(l>>5), col j = l&31
-f32x16 gg_emu_mfma_32x32x16_bf16(u16x8 a, u16x8 b, f32x16 c) {
+template <class Cvt>
+static f32x16 mfma_32x32x16(u16x8 a, u16x8 b, f32x16 c, Cvt cvt) {
     WaveState& w = g_waves[g_cur / 64];
     int lane = g_cur & 63;
     w.a[lane] = a;
@@ -111,14 +112,18 @@ f32x16 gg_emu_mfma_32x32x16_bf16(u16x8 a, u16x8 b, f32x16 c) {
         int i = (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5);
         float s = c[r];
         for (int k = 0; k < 16; ++k) {
-            float av = bf2f_(w.a[(k >> 3) * 32 + i][k & 7]);
-            float bv = bf2f_(w.b[(k >> 3) * 32 + j][k & 7]);
+            float av = cvt(w.a[(k >> 3) * 32 + i][k & 7]);
+            float bv = cvt(w.b[(k >> 3) * 32 + j][k & 7]);
             s += av * bv;
         }
         out[r] = s;
     }
     wave_sync();
     return out;
+}
+f32x16 gg_emu_mfma_32x32x16_bf16(u16x8 a, u16x8 b, f32x16 c) { return mfma_32x32x16(a, b, c, bf2f_); }
+f32x16 gg_emu_mfma_32x32x16_f16(u16x8 a, u16x8 b, f32x16 c) {
+    return mfma_32x32x16(a, b, c, [](unsigned short h) { return (float)__builtin_bit_cast(_Float16, h); });
 }
 
 // v_mfma_f32_16x16x32_bf16 (gg_device.h: lane l holds A[i = l & 15][k = 8 (l >> 4) + e] / B[k][j = l & 15]; D[i = 4 (l >> 4) + r][j = l & 15])
