@@ -56,6 +56,30 @@ class PlanEntry(C.Structure):        # mirrors gg_plan_entry
     _fields_ = [(f, C.c_int32) for f in FIELDS]
 
 
+class RotaryDesc(C.Structure):       # mirrors gg_rotary_desc
+    _fields_ = [
+        ('q', C.c_void_p), ('k', C.c_void_p), ('yq', C.c_void_p), ('yk', C.c_void_p),
+        ('q_strides', C.c_int64 * 3), ('k_strides', C.c_int64 * 3),
+        ('positions', C.c_void_p), ('p_strides', C.c_int64 * 3),
+        ('freqs', C.c_void_p), ('axes', C.c_void_p),
+        ('pos_type', C.c_int32), ('dtype', C.c_int32),
+        ('B', C.c_int32), ('n', C.c_int32), ('hq', C.c_int32), ('hk', C.c_int32), ('d', C.c_int32), ('pairs', C.c_int32),
+        ('n_axes', C.c_int32), ('interleaved', C.c_int32), ('inverse', C.c_int32), ('reserved', C.c_int32),
+    ]
+
+
+class WindowDesc(C.Structure):       # mirrors gg_window_desc
+    _fields_ = [
+        ('q', C.c_void_p), ('k', C.c_void_p), ('v', C.c_void_p), ('o', C.c_void_p), ('lse', C.c_void_p),
+        ('d_o', C.c_void_p), ('dq', C.c_void_p), ('dk', C.c_void_p), ('dv', C.c_void_p), ('dvec', C.c_void_p),
+        ('q_strides', C.c_int64 * 3), ('k_strides', C.c_int64 * 3), ('v_strides', C.c_int64 * 3), ('g_strides', C.c_int64 * 3),
+        ('lengths', C.c_void_p), ('key_mask', C.c_void_p), ('mask_stride', C.c_int64),
+        ('B', C.c_int32), ('n', C.c_int32), ('m', C.c_int32), ('h', C.c_int32), ('hk', C.c_int32), ('d', C.c_int32),
+        ('left', C.c_int32), ('right', C.c_int32), ('sinks', C.c_int32), ('dtype', C.c_int32), ('scale', C.c_float),
+        ('reserved', C.c_int32),
+    ]
+
+
 PLAN_TABLE = Path(os.environ.get('GG_PLAN_TABLE') or _HERE / 'plans' / 'gfx950.json')      # (GG_PLAN_TABLE: A/B runs against another tuning cache)
 
 
@@ -82,7 +106,7 @@ class Library:
         L.gg_gemm_plan.argtypes = [C.POINTER(GemmDesc), C.POINTER(C.c_int32), C.POINTER(C.c_int32)]
         self._declare_elementwise()
         self.is_emulator = bool(L.gg_is_emulator())
-        if L.gg_version() != 12:
+        if L.gg_version() != 13:
             raise RuntimeError(f'gigagan_pytorch_amd: ABI version mismatch in {path}')
         L.gg_gemm_plan_table.restype = C.c_int
         L.gg_gemm_plan_table.argtypes = [C.POINTER(PlanEntry), C.c_int32]

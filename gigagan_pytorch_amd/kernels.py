@@ -1,6 +1,7 @@
 """Raw (non-autograd) launches of the C-ABI kernels on torch tensors. Layout glue only — no arithmetic."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 
@@ -52,7 +53,7 @@ class LaunchProfiler:
     active - contraction, coefficient, modulation, mixing, resampling ... - so that an op's time is the time of everything it
     launches. Implemented as a proxy in front of the ctypes library object; eager execution only."""
     _NOT_LAUNCHES = ('gg_gemm_plan', 'gg_gemm_workspace_bytes', 'gg_last_error', 'gg_version', 'gg_is_emulator',
-                     'gg_bias_act_bwd_partials', 'gg_rmsnorm_blocks', 'gg_gemm_plan_table', 'gg_comm_', 'gg_graph_')
+                     'gg_bias_act_bwd_partials', 'gg_rmsnorm_blocks', 'gg_layernorm_blocks', 'gg_window_workspace_bytes', 'gg_gemm_plan_table', 'gg_comm_', 'gg_graph_')
 
     def __init__(self):
         self.records = []       # (entry point, start event, end event)
@@ -1376,6 +1377,227 @@ def rmsnorm_bwd2(x, g, v, gamma, want_dgamma: bool):
     rc = L.lib.gg_rmsnorm_bwd2(ptr(x), ptr(g), ptr(v), ptr(gamma), ptr(gx), ptr(gg), ptr(part), rows, Cc, RMS_EPS, L.stream(x))
     L.check(rc, 'gg_rmsnorm_bwd2')
     return gx, gg, (part.sum(0) if part is not None else None)
+
+
+# --------------------------------------------------------------------------------------------------
+# transformer operators (gg_transformer.hip): layer norm, rotary positions, attention with a sliding window and sinks
+# --------------------------------------------------------------------------------------------------
+_ROW_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _same_device(what: str, first: torch.Tensor, *rest):
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise ValueError(f'{what}: tensors on {first.device} and {t.device}')
+
+
+def _on_device(L, t: torch.Tensor):
+    """the launch's device made current where it is not (a launch goes to the current device, whatever device its stream is of)"""
+    if L.is_emulator or t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _row_type(what: str, t: torch.Tensor) -> int:
+    if t.dtype not in _ROW_TYPES:
+        raise TypeError(f'{what}: bfloat16, float16 or float32 expected, got {t.dtype}')
+    return _ROW_TYPES[t.dtype]
+
+
+def _rows2(x: torch.Tensor):
+    """(..., C) -> a (rows, C) view with unit feature stride and one row pitch, or a copy where the layout has none"""
+    r = x.reshape(-1, x.shape[-1])
+    if r.shape[1] > 1 and r.stride(1) != 1:
+        r = r.contiguous()
+    return r
+
+
+LAYERNORM_MAX_C = 16384
+
+
+def layernorm_fwd(x: torch.Tensor, w: torch.Tensor, b, eps: float, stats: bool):
+    """x (..., C) bf16 / fp16 / fp32, w and b (C,) fp32 -> (y like x, contiguous; mean, rstd (rows,) fp32 or None)."""
+    L = _C.lib()
+    L.require(x, w, b)
+    dt = _row_type('layernorm_fwd', x)
+    Cc = x.shape[-1]
+    assert all(t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.shape == (Cc,)) for t in (w, b))
+    _same_device('layernorm_fwd', x, w, b)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rows = y.numel() // Cc
+    mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else (None, None)
+    if rows:
+        x2 = _rows2(x)
+        with _on_device(L, x):
+            rc = L.lib.gg_layernorm_fwd(ptr(x2), x2.stride(0), ptr(w), ptr(b), ptr(y), ptr(mean), ptr(rstd), rows, Cc, eps, dt, L.stream(x))
+        L.check(rc, 'gg_layernorm_fwd')
+    return y, mean, rstd
+
+
+def layernorm_bwd(x: torch.Tensor, dy: torch.Tensor, w: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, want_db: bool):
+    """-> (dx like x, contiguous; dw (C,) fp32; db (C,) fp32 or None)."""
+    L = _C.lib()
+    L.require(x, dy, w, mean, rstd)
+    dt = _row_type('layernorm_bwd', x)
+    assert dy.dtype == x.dtype and dy.shape == x.shape
+    _same_device('layernorm_bwd', x, dy, w, mean, rstd)
+    Cc = x.shape[-1]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rows = dx.numel() // Cc
+    if not rows:
+        z = torch.zeros((2, Cc), dtype=torch.float32, device=x.device)
+        return dx, z[0], (z[1] if want_db else None)
+    x2, g2 = _rows2(x), _rows2(dy)
+    dw = torch.empty(Cc, dtype=torch.float32, device=x.device)
+    db = torch.empty_like(dw) if want_db else None
+    part = torch.empty((L.lib.gg_layernorm_blocks(rows, Cc), 2, Cc), dtype=torch.float32, device=x.device)
+    with _on_device(L, x):
+        rc = L.lib.gg_layernorm_bwd(ptr(x2), x2.stride(0), ptr(g2), g2.stride(0), ptr(w), ptr(mean), ptr(rstd), ptr(dx), ptr(part), ptr(dw),
+                                    ptr(db), rows, Cc, dt, L.stream(x))
+    L.check(rc, 'gg_layernorm_bwd')
+    return dx, dw, db
+
+
+class RotarySpec:
+    """what a rotary embedding keeps between calls: which axis turns which feature pairs, and how fast.
+
+    sections     feature pairs per axis, e.g. (16, 16) for the rows and columns of a map with 64-feature heads, (16, 24, 24) for
+                 time, height and width; 2 * sum(sections) features of a head turn, the rest are left as they are.
+    theta        pair i of an axis with c pairs turns by theta ** (-i / c) radians per position ...
+    shared       ... or, with one frequency ladder for all axes, the i-th pair of ALL pairs by theta ** (-i / sum(sections)).
+    interleaved  pairs are features (2i, 2i + 1) instead of (i, i + sum(sections))."""
+
+    def __init__(self, sections, theta: float = 10000.0, shared: bool = False, interleaved: bool = False):
+        self.sections = tuple(int(c) for c in sections)
+        if not self.sections or any(c < 0 for c in self.sections) or not 1 <= sum(self.sections) <= 128 or len(self.sections) > 255:
+            raise ValueError(f'RotarySpec: 1 to 128 feature pairs over the axes expected, got sections {tuple(sections)}')
+        if not (theta > 0 and math.isfinite(theta)):
+            raise ValueError(f'RotarySpec: theta must be positive, got {theta}')
+        self.theta, self.shared, self.interleaved = float(theta), bool(shared), bool(interleaved)
+        self.pairs = sum(self.sections)
+        if shared:
+            freqs = [self.theta ** (-i / self.pairs) for i in range(self.pairs)]
+        else:
+            freqs = [self.theta ** (-i / c) for c in self.sections for i in range(c)]
+        self._freqs = (C.c_double * self.pairs)(*freqs)
+        self._axes = (C.c_uint8 * self.pairs)(*[a for a, c in enumerate(self.sections) for _ in range(c)])
+
+    @property
+    def freqs(self):
+        """radians per position of every feature pair"""
+        return list(self._freqs)
+
+    @property
+    def axes(self):
+        """the axis that turns each feature pair"""
+        return list(self._axes)
+
+    def __deepcopy__(self, memo):
+        return RotarySpec(self.sections, self.theta, self.shared, self.interleaved)
+
+    def __reduce__(self):
+        return RotarySpec, (self.sections, self.theta, self.shared, self.interleaved)
+
+
+def _heads4(t: torch.Tensor) -> torch.Tensor:
+    """(B, h, n, d) with unit feature stride, copied where it has another"""
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+
+
+def rotary(q: torch.Tensor, k, positions: torch.Tensor, spec: RotarySpec, inverse: bool = False):
+    """q (B, h, n, d), k (B, hk, n, d) or None, any strides; positions (n, axes) or (B, n, axes) -> the turned q and k as
+    (B, heads, n, d) views of dense (B, n, heads, d) storage (k's place None without k)."""
+    L = _C.lib()
+    L.require(q, k, positions)
+    dt = _row_type('rotary', q)
+    B, h, n, d = q.shape
+    hk = 0 if k is None else k.shape[1]
+    outs = [None if t is None else torch.empty((B, n, t.shape[1], d), dtype=t.dtype, device=t.device).transpose(1, 2) for t in (q, k)]
+    if not (B and n):
+        return tuple(outs)
+    q = _heads4(q)
+    k = None if k is None else _heads4(k)
+    ps = positions.stride() if positions.dim() == 3 else (0, *positions.stride())
+    D = _C.RotaryDesc(q=ptr(q), k=ptr(k), yq=ptr(outs[0]), yk=ptr(outs[1]), q_strides=(C.c_int64 * 3)(*q.stride()[:3]),
+                      k_strides=(C.c_int64 * 3)(*(k.stride()[:3] if k is not None else (0, 0, 0))), positions=ptr(positions),
+                      p_strides=(C.c_int64 * 3)(*ps), freqs=C.addressof(spec._freqs), axes=C.addressof(spec._axes),
+                      pos_type=_POS_TYPES[positions.dtype], dtype=dt, B=B, n=n, hq=h, hk=hk, d=d, pairs=spec.pairs,
+                      n_axes=len(spec.sections), interleaved=int(spec.interleaved), inverse=int(inverse))
+    with _on_device(L, q):
+        rc = L.lib.gg_rotary(C.byref(D), L.stream(q))
+    L.check(rc, 'gg_rotary')
+    return tuple(outs)
+
+
+WINDOW_HEAD_DIMS = (32, 64, 128)
+
+
+def _strides3(t: torch.Tensor):
+    return (C.c_int64 * 3)(*(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])))
+
+
+def _attend4(t: torch.Tensor) -> torch.Tensor:
+    """(B, h, n, d) as the window kernels read it (unit feature stride, strides of whole 16-byte vectors, aligned); else a copy"""
+    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask):
+    B, h, n, d = q.shape
+    return _C.WindowDesc(q=ptr(q), k=ptr(k), v=ptr(v), o=ptr(o), lse=ptr(lse), q_strides=_strides3(q), k_strides=_strides3(k),
+                         v_strides=_strides3(v), lengths=ptr(lengths), key_mask=ptr(key_mask),
+                         mask_stride=0 if key_mask is None or B == 1 else key_mask.stride(0), B=B, n=n, m=k.shape[2], h=h, hk=k.shape[1], d=d,
+                         left=left, right=right, sinks=sinks, dtype=_ROW_TYPES[q.dtype], scale=scale)
+
+
+def window_fwd(q, k, v, scale: float, left: int, right: int, sinks: int, lengths, key_mask, want_lse: bool):
+    """q (B, h, n, d), k, v (B, hk, m, d) bf16 / fp16; lengths (B,) int32, key_mask (B, m) bool, both optional; left / right -1 = no
+    bound -> (o as a (B, h, n, d) view of dense (B, n, h, d) storage, lse (B * hk, n * h / hk) fp32 in the log2 domain or None)."""
+    L = _C.lib()
+    L.require(q, k, v, lengths, key_mask)
+    B, h, n, d = q.shape
+    o = torch.empty((B, n, h, d), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B * k.shape[1], n * (h // k.shape[1])), dtype=torch.float32, device=q.device) if want_lse else None
+    if not o.numel():
+        return o.transpose(1, 2), lse
+    if not k.shape[2]:
+        return o.zero_().transpose(1, 2), (lse.fill_(math.inf) if want_lse else None)
+    q, k, v = _attend4(q), _attend4(k), _attend4(v)
+    D = _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask)
+    with _on_device(L, q):
+        nbytes = L.lib.gg_window_workspace_bytes(C.byref(D), 0)
+        ws = _workspace(nbytes, q) if nbytes else None
+        rc = L.lib.gg_window_fwd(C.byref(D), ptr(ws), nbytes, L.stream(q))
+    L.check(rc, 'gg_window_fwd')
+    return o.transpose(1, 2), lse
+
+
+def window_bwd(q, k, v, o, lse, d_o, scale: float, left: int, right: int, sinks: int, lengths, key_mask):
+    """-> dq (B, h, n, d), dk, dv (B, hk, m, d) in the operands' type, as views of dense token-major storage; `o`, `lse` as window_fwd
+    returned them, d_o (B, h, n, d) with any strides."""
+    L = _C.lib()
+    L.require(q, k, v, o, lse, d_o, lengths, key_mask)
+    assert d_o.dtype == q.dtype and d_o.shape == q.shape
+    B, h, n, d = q.shape
+    hk, m = k.shape[1], k.shape[2]
+    dq = torch.empty((B, n, h, d), dtype=q.dtype, device=q.device)
+    dk, dv = torch.empty((2, B, m, hk, d), dtype=q.dtype, device=q.device)
+    views = dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2)
+    if not (dq.numel() and dk.numel()):
+        for t in (dq, dk, dv):
+            t.zero_()
+        return views
+    q, k, v, d_o = _attend4(q), _attend4(k), _attend4(v), _attend4(d_o)
+    D = _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask)
+    dvec = torch.empty_like(lse)
+    D.d_o, D.g_strides, D.dq, D.dk, D.dv, D.dvec = ptr(d_o), _strides3(d_o), ptr(dq), ptr(dk), ptr(dv), ptr(dvec)
+    with _on_device(L, q):
+        nbytes = L.lib.gg_window_workspace_bytes(C.byref(D), 1)
+        ws = _workspace(nbytes, q) if nbytes else None
+        rc = L.lib.gg_window_bwd(C.byref(D), ptr(ws), nbytes, L.stream(q))
+    L.check(rc, 'gg_window_bwd')
+    return views
 
 
 # --------------------------------------------------------------------------------------------------

@@ -25,6 +25,8 @@ from torch.autograd import Function
 
 from . import kernels as K
 
+RotarySpec = K.RotarySpec
+
 ACT_DTYPE = torch.bfloat16
 LRELU_SLOPE = 0.2
 second_order = False   # set (by the trainer) while a graph that will be differentiated twice is being built
@@ -742,6 +744,49 @@ class RmsNormBwdFn(Function):
         return gx, gg, dgamma, None, (v if ctx.needs_input_grad[4] else None)     # dx = ... + carry: d/d(carry) is v itself
 
 
+class LayerNormFn(Function):
+    """layer norm over the last axis in one pass (gg_layernorm.h); backward: dx and the workgroups' sums of dw, db in one pass over x
+    and dy, their total in a second launch. First order."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        w32, b32 = (None if t is None else t.detach().float().contiguous() for t in (weight, bias))
+        y, mean, rstd = K.layernorm_fwd(x, w32, b32, eps, any(ctx.needs_input_grad))
+        ctx.has_bias = bias is not None
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        if mean is not None:
+            ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dx, dw, db = K.layernorm_bwd(x, dy.to(x.dtype), weight.float().contiguous(), mean, rstd, ctx.has_bias)
+        return dx, dw.to(weight.dtype), (db.to(ctx.bias_dtype) if ctx.has_bias else None), None
+
+
+class RotaryFn(Function):
+    """rotary positions on q and, in the same launch, k (gg_rotary.h). The gradient of a turn is the turn by the opposite angle, so the
+    backward is this function with `inverse` flipped: differentiable any number of times (gradient penalty)."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, spec, inverse):
+        ctx.spec, ctx.inverse = spec, inverse
+        ctx.save_for_backward(positions)
+        ctx.dtypes = q.dtype, (None if k is None else k.dtype)
+        yq, yk = K.rotary(q, k, positions, spec, inverse)
+        return yq if k is None else (yq, yk)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        positions, = ctx.saved_tensors
+        gq, gk = (None if g is None else g.to(dt) for g, dt in zip((*grads, None)[:2], ctx.dtypes))
+        out = RotaryFn.apply(gq, gk, positions, ctx.spec, not ctx.inverse)
+        dq, dk = (out, None) if gk is None else out
+        return dq, dk, None, None, None
+
+
 class FlashAttnFn(Function):
     """fused self-attention over [B][n][heads*64] projections with the learned null key / value (gg_attention.h):
     forward saves only o and the per-query log-sum-exp; backward = two kernels (dq; dk/dv) that recompute P. When the
@@ -839,6 +884,27 @@ class FlashAttnGenFn(Function):
         if k0 is not None:
             dk0, dv0 = dk0.to(k0.dtype), dv0.to(v0.dtype)
         return dq, dk, dv, dk0, dv0, None, None, None
+
+
+class WindowAttnFn(Function):
+    """attention with a sliding window and sinks (gg_window.h): forward saves o and the rows' log-sum-exp, backward is two kernels (dq;
+    dk and dv, summed over the query heads of a shared key head) that recompute P. First order."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, key_mask, scale, left, right, sinks):
+        ctx.cfg = (scale, left, right, sinks)
+        train = any(ctx.needs_input_grad[:3])
+        o, lse = K.window_fwd(q, k, v, *ctx.cfg, lengths, key_mask, train)
+        if train:
+            ctx.save_for_backward(q, k, v, lengths, key_mask, o, lse)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o):
+        q, k, v, lengths, key_mask, o, lse = ctx.saved_tensors
+        dq, dk, dv = K.window_bwd(q, k, v, o, lse, d_o.to(q.dtype), *ctx.cfg, lengths, key_mask)
+        return dq, dk, dv, None, None, None, None, None, None
 
 
 def _rows_view(t):
@@ -1891,6 +1957,47 @@ class HipOps:
         out = GemmFn.apply(attn, v2, True, False, (n, dh, mp), None, None, 1.0, False)  # (BH, n, dh)
         return _fully_masked_rows(out.reshape(B, h, n, dh), v, key_mask)
 
+    def window_attention(self, q, k, v, *, scale, window=(None, None), sinks=0, key_mask=None, lengths=None):
+        """attention with a sliding window and a few first keys (sinks) that stay visible.
+
+        q (B, h, n, d), k and v (B, hk, m, d), h a multiple of hk (grouped heads), d 32, 64 or 128, bf16 or fp16, any strides. The queries
+        are the LAST n of a sequence: query i of item b sits at position p = lengths[b] - n + i (lengths (B,) int32 or int64 on the
+        device, at most m; m without) and sees key j when j < lengths[b], p - left <= j or j < sinks, j <= p + right, and key_mask[b, j]
+        ((B, m) bool, optional). window = (left, right), None = no bound; (None, 0) is causal attention; n = 1 is a decoding step on a
+        cache. A query that sees no key, and one at a negative position, gets zeros and no gradient. What lies in k and v where no
+        query sees it (stale slots, NaN padding) does not reach the result.
+
+        Returns (B, h, n, d), a view of (B, n, h, d) storage. First-order gradients for q, k and v."""
+        for name, t in (('q', q), ('k', k), ('v', v)):
+            if t.dim() != 4:
+                raise ValueError(f'window_attention: {name} must be (B, heads, tokens, features), got {tuple(t.shape)}')
+            if t.dtype not in (torch.bfloat16, torch.float16) or t.dtype != q.dtype:
+                raise TypeError(f'window_attention: q, k and v of one type, bfloat16 or float16, expected; {name} is {t.dtype}')
+        B, h, n, d = q.shape
+        hk, m = k.shape[1], k.shape[2]
+        if k.shape != v.shape or k.shape[0] != B or k.shape[3] != d or hk == 0 or h == 0 or h % hk:
+            raise ValueError(f'window_attention: shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit')
+        if d not in K.WINDOW_HEAD_DIMS:
+            raise ValueError(f'window_attention: heads of {K.WINDOW_HEAD_DIMS} features expected, got {d}')
+        scale = float(scale)
+        if not (0.0 < scale <= 1e30):
+            raise ValueError(f'window_attention: scale must be positive and finite, got {scale}')
+        left, right = (-1 if t is None else int(t) for t in window)
+        if any(t is not None and int(t) < 0 for t in window) or sinks < 0:
+            raise ValueError(f'window_attention: window sides and sinks must not be negative, got {tuple(window)} and {sinks}')
+        left, right, sinks = min(left, 1 << 29), min(right, 1 << 29), min(int(sinks), m)
+        if lengths is not None:
+            if tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64):
+                raise ValueError(f'window_attention: lengths must be int32 or int64 of shape ({B},)')
+            lengths = (lengths.clamp(0, m) if lengths.dtype == torch.int64 else lengths).to(torch.int32).contiguous()
+        if key_mask is not None:
+            if tuple(key_mask.shape) != (B, m) or key_mask.dtype != torch.bool:
+                raise ValueError(f'window_attention: key_mask must be bool of shape ({B}, {m})')
+            if m > 1 and key_mask.stride(1) != 1:
+                key_mask = key_mask.contiguous()
+        K._same_device('window_attention', q, k, v, lengths, key_mask)
+        return WindowAttnFn.apply(q, k, v, lengths, key_mask, scale, left, right, sinks)
+
     def self_attention(self, q, k, v, null_kv, *, heads, scale, l2):
         """SelfAttention.forward after the projections (gp.py:562-592); q, k, v logical (b, heads*d, x, y)."""
         b, c, x, y = q.shape
@@ -1935,6 +2042,49 @@ class HipOps:
         else:
             assert act is None
         return y
+
+    def layer_norm(self, x, weight, bias=None, eps=1e-5):
+        """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (..., C): bf16, fp16 or fp32 rows, the result in x's
+        type and contiguous; weight and bias (C,) in any floating type, their gradients summed in fp32. 0 < C <= 16384. Rows with one
+        pitch are read where they lie; other layouts are copied first. First-order gradients."""
+        C = x.shape[-1] if x.dim() else 0
+        if not 0 < C <= K.LAYERNORM_MAX_C:
+            raise ValueError(f'layer_norm: last axis of 1 to {K.LAYERNORM_MAX_C} features expected, got shape {tuple(x.shape)}')
+        if x.dtype not in K._ROW_TYPES:
+            raise TypeError(f'layer_norm: bfloat16, float16 or float32 expected, got {x.dtype}')
+        for name, t in (('weight', weight), ('bias', bias)):
+            if t is None and name == 'bias':
+                continue
+            if t is None or tuple(t.shape) != (C,) or not t.is_floating_point():
+                raise ValueError(f'layer_norm: {name} must be a floating tensor of shape ({C},)')
+        return LayerNormFn.apply(x, weight, bias, float(eps))
+
+    def rotary(self, q, positions, spec, k=None):
+        """rotary positions with several axes: feature pair i of every head turns by positions[..., axis(i)] * freq(i).
+
+        q (B, h, n, d), optional k (B, hk, n, d) of q's type (fewer heads allowed): bf16, fp16 or fp32, any strides. positions: int32,
+        int64 or fp32, (n, axes) for the whole batch or (B, n, axes); `spec` a RotarySpec (sections of feature pairs per axis,
+        theta, pairing). Angles are taken in fp64, so far positions keep their precision. Returns the turned q, or (q, k), as (B, heads, n, d)
+        views of (B, n, heads, d) storage - the layout the attention entry points read without a copy. Differentiable any number of times;
+        positions get no gradient."""
+        if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:])):
+            raise ValueError(f'rotary: q (B, h, n, d) and k (B, hk, n, d) expected, got {tuple(q.shape)}'
+                             + ('' if k is None else f' and {tuple(k.shape)}'))
+        if q.dtype not in K._ROW_TYPES or (k is not None and k.dtype != q.dtype):
+            raise TypeError(f'rotary: q and k of one type, bfloat16, float16 or float32, expected; got {q.dtype}'
+                            + ('' if k is None else f' and {k.dtype}'))
+        if not isinstance(spec, K.RotarySpec):
+            raise TypeError(f'rotary: a RotarySpec expected, got {type(spec).__name__}')
+        B, h, n, d = q.shape
+        if d < 2 * spec.pairs or h == 0 or (k is not None and k.shape[1] == 0):
+            raise ValueError(f'rotary: heads of at least {2 * spec.pairs} features expected, got {tuple(q.shape)}')
+        if positions.dtype not in K._POS_TYPES:
+            raise TypeError(f'rotary: int32, int64 or float32 positions expected, got {positions.dtype}')
+        A = len(spec.sections)
+        if tuple(positions.shape) not in ((n, A), (B, n, A)):
+            raise ValueError(f'rotary: positions of shape ({n}, {A}) or ({B}, {n}, {A}) expected, got {tuple(positions.shape)}')
+        K._same_device('rotary', q, k, positions)
+        return RotaryFn.apply(q, k, positions.detach(), spec, False)
 
     # -- unet pieces (unet_upsampler.py) -----------------------------------------------------------------
     def maxpool_highfreq(self, x):

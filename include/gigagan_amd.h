@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define GG_ABI_VERSION 12
+#define GG_ABI_VERSION 13
 
 int gg_version(void);
 const char* gg_last_error(void);
@@ -483,6 +483,65 @@ typedef struct gg_aconv_desc {
 } gg_aconv_desc;
 int gg_aconv_plan(const gg_aconv_desc* d, int32_t* tm, int32_t* nwn, int32_t* nwk, int32_t* lds_bytes, int32_t* grid);
 int gg_aconv_fwd(const gg_aconv_desc* d, void* stream);
+
+/* ---- transformer operators (csrc/gg_transformer.hip): the text encoder's blocks (gp.py:659-867) and the image attention blocks
+ * (gp.py:538-655) with a layer norm, with positions, and with a bounded view. dtype of the rows: 0 = bf16, 1 = IEEE half, 2 = fp32;
+ * statistics and sums fp32. */
+
+/* layer norm over the last axis: y = (x - mean) rstd w + b, rstd = 1 / sqrt(var + eps) (biased variance). x [rows] of C elements, row
+ * pitch ldx elements (0 = every row the same); y dense [rows][C]; w, b (b optional) fp32 [C]; mean, rstd fp32 [rows] (both or neither).
+ * 0 < C <= GG_LAYERNORM_MAX_C, any alignment. y may be x where ldx == C. */
+#define GG_LAYERNORM_MAX_C 16384
+int gg_layernorm_fwd(const void* x, int64_t ldx, const float* w, const float* b, void* y, float* mean, float* rstd, int64_t rows,
+                     int32_t C, float eps, int32_t dtype, void* stream);
+/* its gradient: dx dense [rows][C] in the rows' type, dw fp32 [C], db fp32 [C] (optional); part = fp32 workspace
+ * [gg_layernorm_blocks(rows, C)][2][C], the row sums of each workgroup, added in a fixed order by a second launch. */
+int32_t gg_layernorm_blocks(int64_t rows, int32_t C);
+int gg_layernorm_bwd(const void* x, int64_t ldx, const void* dy, int64_t ldy, const float* w, const float* mean, const float* rstd,
+                     void* dx, float* part, float* dw, float* db, int64_t rows, int32_t C, int32_t dtype, void* stream);
+
+/* rotary positions: feature pair i of every head of q (and k, optional: hk = 0) turns by positions[b][t][axes[i]] * freqs[i] radians
+ * (inverse: by the opposite angle - the gradient). Pairs are (i, i + pairs), interleaved: (2i, 2i + 1); features from 2 * pairs on are
+ * copied. q, k [B][heads][n][d] with element strides {batch, head, token} and unit feature stride; yq, yk dense [B][n][heads][d], not
+ * overlapping their inputs. positions: strides {batch, token, axis}, int32 / int64 / fp32. freqs and axes are HOST arrays of `pairs`
+ * entries, read during the call. 1 <= pairs <= 128, 2 * pairs <= d <= GG_ROTARY_MAX_D. */
+#define GG_ROTARY_MAX_D 65536
+typedef struct gg_rotary_desc {
+    const void* q; const void* k; void* yq; void* yk;
+    int64_t q_strides[3]; int64_t k_strides[3];
+    const void* positions; int64_t p_strides[3];
+    const double* freqs; const uint8_t* axes;
+    int32_t pos_type;       /* 0 int32, 1 int64, 2 fp32 */
+    int32_t dtype;
+    int32_t B, n, hq, hk, d, pairs, n_axes;
+    int32_t interleaved, inverse;
+    int32_t reserved;
+} gg_rotary_desc;
+int gg_rotary(const gg_rotary_desc* d, void* stream);
+
+/* attention with a sliding window and sinks (csrc/gg_window.h). q [B][h][n][d], k, v [B][hk][m][d], h a multiple of hk (grouped heads), d
+ * 32, 64 or 128, bf16 or half, element strides {batch, head, token} in multiples of 8 with unit feature stride, 16-byte aligned. Query i
+ * of item b sits at position p = len_b - n + i, len_b = lengths[b] (device int32, clamped to 0 .. m) or m, and sees key j when
+ * j < len_b, j <= p + right, (j >= p - left or j < sinks) and key_mask[b][j] (bytes, batch stride mask_stride; optional); left / right
+ * < 0 = no bound. A query that sees no key, or at p < 0, gets zeros and no gradient.
+ *   forward:  o dense [B][n][h][d], lse fp32 [B*hk][n*h/hk] (optional; log2 domain, +inf for a row that sees nothing)
+ *   backward: reads q, k, v, o, lse and d_o (strides g_strides), writes dq dense [B][n][h][d], dk, dv dense [B][m][hk][d] (every element)
+ *             and dvec fp32 [B*hk][n*h/hk] (scratch)
+ * Both take a workspace of gg_window_workspace_bytes(d, backward) bytes (0: none), 16-byte aligned, free again when the call's work on
+ * `stream` is done. Results do not depend on what runs beside: no atomics. */
+typedef struct gg_window_desc {
+    const void* q; const void* k; const void* v; void* o; float* lse;
+    const void* d_o; void* dq; void* dk; void* dv; float* dvec;
+    int64_t q_strides[3], k_strides[3], v_strides[3], g_strides[3];
+    const int32_t* lengths;
+    const void* key_mask; int64_t mask_stride;
+    int32_t B, n, m, h, hk, d, left, right, sinks, dtype;
+    float scale;
+    int32_t reserved;
+} gg_window_desc;
+size_t gg_window_workspace_bytes(const gg_window_desc* d, int32_t backward);
+int gg_window_fwd(const gg_window_desc* d, void* workspace, size_t workspace_bytes, void* stream);
+int gg_window_bwd(const gg_window_desc* d, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- hipGraph repair. The training step is replayed as a captured hipGraph (the reference has no counterpart: it launches eagerly,
  * gp.py:2227-2580). The HIP runtime PyTorch 2.10+rocm7.0 carries (7.0.51831) re-executes a captured hipMemsetAsync with a corrupted
