@@ -52,17 +52,22 @@ GG_KERNEL GG_LAUNCH_BOUNDS(TPR > 256 ? TPR : 256) void gg_layernorm_fwd_kernel(G
     const long long row = row0 < p.rows ? row0 : p.rows - 1;          // (every lane takes part in the sums)
     const E* xr = (const E*)p.x + row * p.ldx;
     GgRaw8<T> raw[NV];
+#pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (t + i * TPR) * 8;
         raw[i] = gg_raw8_load<T>(xr + (c < p.C ? c : 0), p.C - c);
     }
     float s = 0.f;
+#pragma unroll
     for (int i = 0; i < NV; ++i)
+#pragma unroll
         for (int e = 0; e < 8; ++e) s += gg_raw8_get<T>(raw[i], e);
     const float mean = gg_ln_row_sum<TPR>(s, sRed[0]) / (float)p.C;
     float s2 = 0.f;
+#pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (t + i * TPR) * 8;
+#pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float d = gg_raw8_get<T>(raw[i], e) - mean;
             s2 += c + e < p.C ? d * d : 0.f;
@@ -75,6 +80,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS(TPR > 256 ? TPR : 256) void gg_layernorm_fwd_kernel(G
         p.rstd[row] = rstd;
     }
     E* yr = (E*)p.y + row * p.C;
+#pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (t + i * TPR) * 8, n = p.C - c;
         if (n <= 0) break;
@@ -82,6 +88,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS(TPR > 256 ? TPR : 256) void gg_layernorm_fwd_kernel(G
         GgRaw8<GG_ELT_F32> b = {};
         if (p.b) b = gg_raw8_load<GG_ELT_F32>(p.b + c, n);
         float v[8];
+#pragma unroll
         for (int e = 0; e < 8; ++e)
             v[e] = gg_fmaf((gg_raw8_get<T>(raw[i], e) - mean) * rstd, gg_raw8_get<GG_ELT_F32>(w, e), gg_raw8_get<GG_ELT_F32>(b, e));
         gg_raw8_set<T>(raw[i], v);
@@ -93,14 +100,15 @@ template <int T, int TPR, int NV>
 GG_KERNEL GG_LAUNCH_BOUNDS(TPR > 256 ? TPR : 256) void gg_layernorm_bwd_kernel(GgLnParams p) {
     typedef typename GgElt<T>::type E;
     constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;
-    constexpr int WIDE = TPR < 64 ? 64 : TPR;                         // threads that end up holding distinct rows' sums
     GG_SHARED float sRed[2][2][16];                                   // (two sets: a row's sums may be read while the next row's are written)
     GG_SHARED float sAcc[RPB > 1 ? 3 * (TPR < 64 ? TPR : 64) * NV * 8 : 1];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     float w[NV][8], dw[NV][8], db[NV][8];
+#pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (t + i * TPR) * 8;
         const GgRaw8<GG_ELT_F32> wr = gg_raw8_load<GG_ELT_F32>(p.w + (c < p.C ? c : 0), p.C - c);
+#pragma unroll
         for (int e = 0; e < 8; ++e) {
             w[i][e] = gg_raw8_get<GG_ELT_F32>(wr, e);
             dw[i][e] = db[i][e] = 0.f;
@@ -114,6 +122,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS(TPR > 256 ? TPR : 256) void gg_layernorm_bwd_kernel(G
         const E* xr = (const E*)p.x + row * p.ldx;
         const E* gr = (const E*)p.dy + row * p.ldy;
         GgRaw8<T> x[NV], g[NV];
+#pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + i * TPR) * 8, cc = c < p.C ? c : 0;
             x[i] = gg_raw8_load<T>(xr + cc, p.C - c);
@@ -121,7 +130,9 @@ GG_KERNEL GG_LAUNCH_BOUNDS(TPR > 256 ? TPR : 256) void gg_layernorm_bwd_kernel(G
         }
         const float mean = p.mean[row], rstd = p.rstd[row];
         float s1 = 0.f, s2 = 0.f;
+#pragma unroll
         for (int i = 0; i < NV; ++i)
+#pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float gw = gg_raw8_get<T>(g[i], e) * w[i][e];
                 s1 += gw;
@@ -131,10 +142,12 @@ GG_KERNEL GG_LAUNCH_BOUNDS(TPR > 256 ? TPR : 256) void gg_layernorm_bwd_kernel(G
         s2 = gg_ln_row_sum<TPR>(s2, sRed[odd][1]) * inv;
         if (!in) continue;      // (the last rows' tail: the lanes come back together at the sums below)
         E* dr = (E*)p.y + row * p.C;
+#pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + i * TPR) * 8, n = p.C - c;
             if (n <= 0) break;
             float v[8];
+#pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float gv = gg_raw8_get<T>(g[i], e), xh = (gg_raw8_get<T>(x[i], e) - mean) * rstd;
                 v[e] = rstd * (gv * w[i][e] - s1 - xh * s2);
@@ -148,7 +161,9 @@ GG_KERNEL GG_LAUNCH_BOUNDS(TPR > 256 ? TPR : 256) void gg_layernorm_bwd_kernel(G
     }
     // the workgroup's rows added up: lanes of one wave that share columns first, then the waves in order
     if constexpr (TPR < 64) {
+#pragma unroll
         for (int i = 0; i < NV; ++i)
+#pragma unroll
             for (int e = 0; e < 8; ++e)
                 for (int o = TPR; o < 64; o <<= 1) {
                     dw[i][e] += gg_shfl_xor(dw[i][e], o);
@@ -162,17 +177,19 @@ GG_KERNEL GG_LAUNCH_BOUNDS(TPR > 256 ? TPR : 256) void gg_layernorm_bwd_kernel(G
             float (*acc)[8] = which ? db : dw;
             gg_sync();
             if (wave && lane < (TPR < 64 ? TPR : 64))
+#pragma unroll
                 for (int i = 0; i < NV; ++i)
                     for (int e = 0; e < 8; ++e) sAcc[(wave - 1) * COLS + (i * 8 + e) * (TPR < 64 ? TPR : 64) + lane] = acc[i][e];
             gg_sync();
             if (wave == 0 && lane < (TPR < 64 ? TPR : 64))
+#pragma unroll
                 for (int i = 0; i < NV; ++i)
                     for (int e = 0; e < 8; ++e)
                         for (int k = 0; k < 3; ++k) acc[i][e] += sAcc[k * COLS + (i * 8 + e) * (TPR < 64 ? TPR : 64) + lane];
         }
         if (threadIdx.x >= (TPR < 64 ? TPR : 64)) return;
     }
-    (void)WIDE;
+#pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (t + i * TPR) * 8, n = p.C - c;
         if (n <= 0) break;
@@ -185,18 +202,24 @@ GG_KERNEL GG_LAUNCH_BOUNDS(TPR > 256 ? TPR : 256) void gg_layernorm_bwd_kernel(G
     }
 }
 
-// column sums of the [blocks][2 C] partial rows: 32 columns x 8 row strides per workgroup, the strides added in order at the end
-GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_layernorm_finish_kernel(const float* part, float* dw, float* db, int blocks, int C) {
-    GG_SHARED float sSum[8][32];
+// column sums of the [blocks][2 C] partial rows: 32 columns x 32 row strides per workgroup (eight loads in flight a thread, then the
+// strides in order)
+GG_KERNEL GG_LAUNCH_BOUNDS(1024) void gg_layernorm_finish_kernel(const float* part, float* dw, float* db, int blocks, int C) {
+    GG_SHARED float sSum[32][33];
     const int col = blockIdx.x * 32 + (threadIdx.x & 31), r0 = threadIdx.x >> 5;
     float s = 0.f;
-    if (col < 2 * C)
-        for (int r = r0; r < blocks; r += 8) s += part[(long long)r * 2 * C + col];
+    if (col < 2 * C) {
+#pragma unroll 8
+        for (int r = r0; r < blocks; r += 32) s += part[(long long)r * 2 * C + col];
+    }
     sSum[r0][threadIdx.x & 31] = s;
     gg_sync();
-    if (r0 == 0 && col < 2 * C) {
-        for (int i = 1; i < 8; ++i) s += sSum[i][threadIdx.x & 31];
-        if (col < C) dw[col] = s;
-        else if (db) db[col - C] = s;
+    // strides of column r0 side by side in one half-wave
+    s = sSum[threadIdx.x & 31][r0];
+    for (int o = 1; o < 32; o <<= 1) s += gg_shfl_xor(s, o);
+    const int out = blockIdx.x * 32 + r0;
+    if ((threadIdx.x & 31) == 0 && out < 2 * C) {
+        if (out < C) dw[out] = s;
+        else if (db) db[out - C] = s;
     }
 }

@@ -76,7 +76,7 @@ extern "C" int gg_layernorm_bwd(const void* x, int64_t ldx, const void* dy, int6
 #undef GG_LN_GO
     rc = gg_check_launch();
     if (rc) return rc;
-    GG_LAUNCH(gg_layernorm_finish_kernel, dim3((unsigned)((2 * C + 31) / 32)), dim3(256), (hipStream_t)stream, (const float*)part, dw, db, blocks, (int)C);
+    GG_LAUNCH(gg_layernorm_finish_kernel, dim3((unsigned)((2 * C + 31) / 32)), dim3(1024), (hipStream_t)stream, (const float*)part, dw, db, blocks, (int)C);
     return gg_check_launch();
 }
 
@@ -111,6 +111,8 @@ extern "C" int gg_rotary(const gg_rotary_desc* d, void* stream) {
     const int per = (d->pairs + 7) / 8 + (d->d - 2 * d->pairs + 7) / 8;
     long long tb = 1024 / ((long long)(d->hq + d->hk) * per);
     if (tb > GG_ROT_LDS_PAIRS / d->pairs) tb = GG_ROT_LDS_PAIRS / d->pairs;
+    const long long fill = (long long)d->B * d->n / 1024;           // (few tokens: rather spread over the chip)
+    if (tb > fill) tb = fill;
     p.tb = (int)(tb < 1 ? 1 : tb);
     const long long grid = (long long)d->B * ((d->n + p.tb - 1) / p.tb);
     if (grid > 0x7fffffffll) return gg_fail(-2, "gg_rotary: too many tokens");

@@ -57,6 +57,7 @@ GG_DEVICE f32x16 ggw_mfma(u16x8 a, u16x8 b, f32x16 c) {
 template <int T>
 GG_DEVICE u16x8 ggw_pack8(const f32x16& v, int c) {
     u16x8 f;
+#pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = gg_elt<T>(v[8 * c + e]);
     return f;
 }
@@ -65,13 +66,16 @@ template <int T>
 GG_DEVICE bool ggw_bad8(u16x8 x) {
     constexpr unsigned short E = T == GG_ELT_BF16 ? 0x7f80 : 0x7c00;
     bool bad = false;
+#pragma unroll
     for (int e = 0; e < 8; ++e) bad = bad || (x[e] & E) == E;
     return bad;
 }
 template <int N>
 GG_DEVICE bool ggw_not_finite(const f32x16* v) {
     float s = 0.f;
+#pragma unroll
     for (int i = 0; i < N; ++i)
+#pragma unroll
         for (int r = 0; r < 16; ++r) s = gg_fmaf(v[i][r], 0.f, s);
     return s != s;
 }
@@ -134,6 +138,7 @@ GG_DEVICE bool ggw_in_range(const GgwRange& r, int sinks, int j) { return j <= r
 template <int D> struct GgwRegs { u16x8 v[D / 32]; };
 template <int D>
 GG_DEVICE void ggw_store_tile(const GgwRegs<D>& r, char* tile) {
+#pragma unroll
     for (int i = 0; i < D / 32; ++i) {
         const int v = threadIdx.x + 256 * i, row = v / (D / 8), c8 = v % (D / 8);
         *(u16x8*)(tile + row * GgwTile<D>::PITCH + c8 * 16) = r.v[i];
@@ -142,6 +147,7 @@ GG_DEVICE void ggw_store_tile(const GgwRegs<D>& r, char* tile) {
 // the second walk: vectors with a NaN or an infinity are taken out and marked, bad[row][vector]
 template <int T, int D>
 GG_DEVICE void ggw_take_bad(GgwRegs<D>& r, unsigned char* bad, bool add) {
+#pragma unroll
     for (int i = 0; i < D / 32; ++i) {
         const bool b = ggw_bad8<T>(r.v[i]);
         if (b) r.v[i] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
@@ -152,6 +158,7 @@ GG_DEVICE void ggw_take_bad(GgwRegs<D>& r, unsigned char* bad, bool add) {
 template <int D>
 GG_DEVICE bool ggw_any_bad(const unsigned char* bad, int row) {
     unsigned any = 0;
+#pragma unroll
     for (int c = 0; c < D / 8; c += 4) any |= *(const unsigned*)(bad + row * (D / 8) + c);
     return any != 0;
 }
@@ -163,8 +170,10 @@ GG_DEVICE void ggw_add_bad(f32x16* ot, const unsigned char* bad, int tk, int j0,
         if (!ggw_any_bad<D>(bad, jr)) continue;             // (workgroup- or wave-uniform; a marked key lies inside the range)
         const int j = j0 + jr;
         float s = 0.f;
+#pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
             const u16x8 kv = *(const u16x8*)(kb + (long long)j * kn + kk * 16 + 8 * hi);
+#pragma unroll
             for (int e = 0; e < 8; ++e) s = gg_fmaf(gg_elt_f<T>(qf[kk][e]), gg_elt_f<T>(kv[e]), s);
         }
         s = gg_sum_xor32(s);
@@ -173,6 +182,7 @@ GG_DEVICE void ggw_add_bad(f32x16* ot, const unsigned char* bad, int tk, int j0,
         for (int c = 0; c < D / 8; ++c)
             if (bad[jr * (D / 8) + c]) {
                 const u16x4 v4 = *(const u16x4*)(vb + (long long)j * vn + c * 8 + 4 * hi);
+#pragma unroll
                 for (int e = 0; e < 4; ++e) ot[c / 4][4 * (c % 4) + e] += pj > 0.f ? pj * gg_elt_f<T>(v4[e]) : 0.f;
             }
     }
@@ -181,6 +191,7 @@ GG_DEVICE void ggw_add_bad(f32x16* ot, const unsigned char* bad, int tk, int j0,
 template <int D>
 GG_DEVICE GgwRegs<D> ggw_load_keys(const unsigned short* base, long long stride, int j0, const GgwRange& rg, int sinks, const unsigned char* keep) {
     GgwRegs<D> r;
+#pragma unroll
     for (int i = 0; i < D / 32; ++i) {
         const int v = threadIdx.x + 256 * i, j = j0 + v / (D / 8), c8 = v % (D / 8);
         r.v[i] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
@@ -242,6 +253,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_fwd_kernel(GgWinParams p) {
     u16x8 qf[KK];
     {
         const unsigned short* qr = p.q + b * p.qb + (long long)(kvh * p.g + row.head) * p.qh + (long long)row.token * p.qn + 8 * hi;
+#pragma unroll
         for (int kk = 0; kk < KK; ++kk) qf[kk] = *(const u16x8*)(qr + kk * 16);
     }
     const float a2 = p.scale * GGW_LOG2E;
@@ -266,7 +278,9 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_fwd_kernel(GgWinParams p) {
 walk:
     m = -1.0e30f;
     l = 0.f;
+#pragma unroll
     for (int db = 0; db < DB; ++db)
+#pragma unroll
         for (int r = 0; r < 16; ++r) ot[db][r] = 0.f;
     if (ta < tb) {
         load(ta);
@@ -283,15 +297,20 @@ walk:
         const int j0 = ggw_tile_at(rg, i) * 64;
         if (j0 <= whij && (j0 + 63 >= wlo - p.left || j0 < p.sinks) && wr0 < rows) {
             f32x16 st[2];
+#pragma unroll
             for (int jb = 0; jb < 2; ++jb) {
+#pragma unroll
                 for (int r = 0; r < 16; ++r) st[jb][r] = 0.f;
+#pragma unroll
                 for (int kk = 0; kk < KK; ++kk) st[jb] = ggw_mfma<T>(ggw_frag<D>(sK[buf], jb * 32, kk, lane), qf[kk], st[jb]);
             }
             if (!(whole && !keep && j0 + 63 <= wlij && (j0 >= whi - p.left || j0 + 63 < p.sinks))) {
                 unsigned long long bits = ~0ull;
                 if (keep) bits = gg_ballot(sKeep[buf][lane] != 0);
                 bits >>= 4 * hi;
+#pragma unroll
                 for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const int jr = jb * 32 + (r & 3) + 8 * (r >> 2), j = j0 + jr + 4 * hi;
                         const bool see = j <= hij && (j >= lo || j < p.sinks) && ((bits >> jr) & 1);
@@ -299,26 +318,35 @@ walk:
                     }
             }
             float mx = -__builtin_inff();
+#pragma unroll
             for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
                 for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[jb][r]);
             mx = gg_max_xor32(mx) * a2;
             if (gg_wave_any(mx > m + GGW_TAU)) {
                 const float mn = fmaxf(m, mx), corr = gg_exp2f(m - mn);
                 l *= corr;
                 m = mn;
+#pragma unroll
                 for (int db = 0; db < DB; ++db)
+#pragma unroll
                     for (int r = 0; r < 16; ++r) ot[db][r] *= corr;
             }
             float sum = 0.f;
+#pragma unroll
             for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     st[jb][r] = gg_exp2f(gg_fmaf(st[jb][r], a2, -m));
                     sum += st[jb][r];
                 }
             l += sum;
+#pragma unroll
             for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const u16x8 pf = ggw_pack8<T>(st[jb], c);
+#pragma unroll
                     for (int db = 0; db < DB; ++db) ot[db] = ggw_mfma<T>(ggw_frag_tr<D>(sV[buf], db * 32, jb * 32 + 16 * c, lane), pf, ot[db]);
                 }
             if (again)
@@ -344,7 +372,9 @@ walk:
     if (SPLIT) {
         const long long sp = (long long)split * p.B * p.hk * rows + at;
         float* po = p.part_o + sp * D;
+#pragma unroll
         for (int db = 0; db < DB; ++db)
+#pragma unroll
             for (int gq = 0; gq < 4; ++gq)
                 *(f32x4*)(po + db * 32 + 8 * gq + 4 * hi) = f32x4{ot[db][4 * gq], ot[db][4 * gq + 1], ot[db][4 * gq + 2], ot[db][4 * gq + 3]};
         if (hi == 0) { p.part_ml[2 * sp] = m; p.part_ml[2 * sp + 1] = l; }
@@ -352,9 +382,12 @@ walk:
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     unsigned short* orow = p.o + (((long long)b * p.n + row.token) * p.h + kvh * p.g + row.head) * D;
+#pragma unroll
     for (int db = 0; db < DB; ++db)
+#pragma unroll
         for (int gq = 0; gq < 4; ++gq) {
             u16x4 o4;
+#pragma unroll
             for (int e = 0; e < 4; ++e) o4[e] = gg_elt<T>(ot[db][4 * gq + e] * inv);
             *(u16x4*)(orow + db * 32 + 8 * gq + 4 * hi) = o4;
         }
@@ -393,6 +426,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_few_kernel(GgWinParams p) {
     u16x8 qf[KK];
     {
         const unsigned short* qr = p.q + b * p.qb + (long long)(kvh * p.g + row.head) * p.qh + (long long)row.token * p.qn + 8 * hi;
+#pragma unroll
         for (int kk = 0; kk < KK; ++kk) qf[kk] = *(const u16x8*)(qr + kk * 16);
     }
     const float a2 = p.scale * GGW_LOG2E;
@@ -405,7 +439,9 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_few_kernel(GgWinParams p) {
         const int j0 = ggw_tile_at(rg, i) * 32, j = j0 + (lane & 31);
         const bool ok = j <= rg.khi;                                            // (0 <= khi < len: the clamped row exists)
         const unsigned short* kr = kb + (long long)(ok ? j : rg.khi) * p.kn + 8 * hi;
+#pragma unroll
         for (int kk = 0; kk < KK; ++kk) kf[kk] = *(const u16x8*)(kr + kk * 16);
+#pragma unroll
         for (int s = 0; s < D / 16; ++s) {
             const int v = lane + 64 * s, jv = j0 + v / (D / 8), c8 = v % (D / 8);
             vr[s] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
@@ -417,12 +453,15 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_few_kernel(GgWinParams p) {
 walk:
     m = -1.0e30f;
     l = 0.f;
+#pragma unroll
     for (int db = 0; db < DB; ++db)
+#pragma unroll
         for (int r = 0; r < 16; ++r) ot[db][r] = 0.f;
     if (ta + wave < tb) load(ta + wave);
     for (int i = ta + wave; i < tb; i += 4) {
         const int j0 = ggw_tile_at(rg, i) * 32;
         gg_wave_sync();
+#pragma unroll
         for (int s = 0; s < D / 16; ++s) {
             const int v = lane + 64 * s;
             if (again) {
@@ -434,35 +473,44 @@ walk:
         }
         gg_wave_sync();
         f32x16 st;
+#pragma unroll
         for (int r = 0; r < 16; ++r) st[r] = 0.f;
+#pragma unroll
         for (int kk = 0; kk < KK; ++kk) st = ggw_mfma<T>(kf[kk], qf[kk], st);
         unsigned bits = 0xffffffffu;
         if (keep) bits = (unsigned)gg_ballot(kept);
         bits >>= 4 * hi;
         if (i + 4 < tb) load(i + 4);
+#pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int jr = (r & 3) + 8 * (r >> 2), j = j0 + jr + 4 * hi;
             const bool see = j <= hij && (j >= lo || j < p.sinks) && ((bits >> jr) & 1);
             st[r] = see ? st[r] : -__builtin_inff();
         }
         float mx = -__builtin_inff();
+#pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[r]);
         mx = gg_max_xor32(mx) * a2;
         if (gg_wave_any(mx > m + GGW_TAU)) {
             const float mn = fmaxf(m, mx), corr = gg_exp2f(m - mn);
             l *= corr;
             m = mn;
+#pragma unroll
             for (int db = 0; db < DB; ++db)
+#pragma unroll
                 for (int r = 0; r < 16; ++r) ot[db][r] *= corr;
         }
         float sum = 0.f;
+#pragma unroll
         for (int r = 0; r < 16; ++r) {
             st[r] = gg_exp2f(gg_fmaf(st[r], a2, -m));
             sum += st[r];
         }
         l += sum;
+#pragma unroll
         for (int c = 0; c < 2; ++c) {
             const u16x8 pf = ggw_pack8<T>(st, c);
+#pragma unroll
             for (int db = 0; db < DB; ++db) ot[db] = ggw_mfma<T>(ggw_frag_tr<D>(sV[wave], db * 32, 16 * c, lane), pf, ot[db]);
         }
         if (again)
@@ -484,7 +532,9 @@ walk:
     const float f = gg_exp2f(m - top);
     for (int w = 0; w < 4; ++w) {
         if (wave == w)
+#pragma unroll
             for (int db = 0; db < DB; ++db)
+#pragma unroll
                 for (int gq = 0; gq < 4; ++gq) {
                     float* at = &sO[q][db * 32 + 8 * gq + 4 * hi];
                     f32x4 x = {ot[db][4 * gq] * f, ot[db][4 * gq + 1] * f, ot[db][4 * gq + 2] * f, ot[db][4 * gq + 3] * f};
@@ -510,6 +560,7 @@ walk:
             const float inv = lt == 0.f ? 0.f : 1.f / lt;
             const int token = (int)((unsigned)r / (unsigned)p.g), head = r - token * p.g;
             u16x4 o4;
+#pragma unroll
             for (int e = 0; e < 4; ++e) o4[e] = gg_elt<T>(x[e] * inv);
             *(u16x4*)(p.o + (((long long)b * p.n + token) * p.h + kvh * p.g + head) * D + d) = o4;
             if (d == 0 && p.lse) p.lse[at] = lt == 0.f ? __builtin_inff() : mt + log2f(lt);
@@ -526,9 +577,11 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_join_kernel(GgWinParams p) {
     const int d = (int)(i % (D / 4)) * 4;
     if (at >= all) return;
     float top = -1.0e30f;
+#pragma unroll 8
     for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[2 * (s * all + at)]);
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
+#pragma unroll 8
     for (int s = 0; s < p.splits; ++s) {
         const float f = gg_exp2f(p.part_ml[2 * (s * all + at)] - top);
         l += f * p.part_ml[2 * (s * all + at) + 1];
@@ -538,6 +591,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_join_kernel(GgWinParams p) {
     const int bkv = (int)(at / rows), r = (int)(at - (long long)bkv * rows);
     const int b = bkv / p.hk, kvh = bkv - b * p.hk, token = r / p.g, head = r - token * p.g;
     u16x4 o4;
+#pragma unroll
     for (int e = 0; e < 4; ++e) o4[e] = gg_elt<T>(x[e] * inv);
     *(u16x4*)(p.o + (((long long)b * p.n + token) * p.h + kvh * p.g + head) * D + d) = o4;
     if (d == 0 && p.lse) p.lse[at] = l == 0.f ? __builtin_inff() : top + log2f(l);
@@ -582,10 +636,12 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_dq_kernel(GgWinParams p) {
     {
         const unsigned short* qr = p.q + b * p.qb + hq * p.qh + (long long)row.token * p.qn + 8 * hi;
         const unsigned short* gr = p.d_o + b * p.gb + hq * p.gh + (long long)row.token * p.gn + 8 * hi;
+#pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
             qf[kk] = *(const u16x8*)(qr + kk * 16);
             gf[kk] = *(const u16x8*)(gr + kk * 16);
             const u16x8 of = *(const u16x8*)(p.o + orow + 8 * hi + kk * 16);
+#pragma unroll
             for (int e = 0; e < 8; ++e) dsum += gg_elt_f<T>(gf[kk][e]) * gg_elt_f<T>(of[e]);
         }
     }
@@ -614,7 +670,9 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_dq_kernel(GgWinParams p) {
         if (keep && threadIdx.x < 64) sKeep[buf][threadIdx.x] = rkeep;
     };
 walk:
+#pragma unroll
     for (int db = 0; db < DB; ++db)
+#pragma unroll
         for (int r = 0; r < 16; ++r) dqt[db][r] = 0.f;
     if (rg.nt > 0) {
         load(0);
@@ -634,22 +692,29 @@ walk:
             unsigned long long bits = ~0ull;
             if (keep) bits = gg_ballot(sKeep[buf][lane] != 0);
             bits >>= 4 * hi;
+#pragma unroll
             for (int jb = 0; jb < 2; ++jb) {
                 f32x16 st, dp;
+#pragma unroll
                 for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = -dsum; }
+#pragma unroll
                 for (int kk = 0; kk < KK; ++kk) {
                     st = ggw_mfma<T>(ggw_frag<D>(sK[buf], jb * 32, kk, lane), qf[kk], st);
                     dp = ggw_mfma<T>(ggw_frag<D>(sV[buf], jb * 32, kk, lane), gf[kk], dp);
                 }
+#pragma unroll
                 for (int r = 0; r < 16; ++r) st[r] = gg_exp2f(gg_fmaf(st[r], a2, -lse)) * dp[r];
                 if (masked)
+#pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const int jr = jb * 32 + (r & 3) + 8 * (r >> 2), j = j0 + jr + 4 * hi;
                         const bool see = j <= hij && (j >= lo || j < p.sinks) && ((bits >> jr) & 1);
                         st[r] = see ? st[r] : 0.f;
                     }
+#pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const u16x8 sf = ggw_pack8<T>(st, c);
+#pragma unroll
                     for (int db = 0; db < DB; ++db) dqt[db] = ggw_mfma<T>(ggw_frag_tr<D>(sK[buf], db * 32, jb * 32 + 16 * c, lane), sf, dqt[db]);
                 }
             }
@@ -672,9 +737,12 @@ walk:
         }
     }
     if (rr >= rows) return;
+#pragma unroll
     for (int db = 0; db < DB; ++db)
+#pragma unroll
         for (int gq = 0; gq < 4; ++gq) {
             u16x4 o4;
+#pragma unroll
             for (int e = 0; e < 4; ++e) o4[e] = gg_elt<T>(dqt[db][4 * gq + e] * p.scale + nan);
             *(u16x4*)(p.dq + orow + db * 32 + 8 * gq + 4 * hi) = o4;
         }
@@ -735,6 +803,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_dkv_kernel(GgWinParams p) {
     {
         const unsigned short* kr = p.k + b * p.kb + kvh * p.kh + (long long)kjc * p.kn + 8 * hi;
         const unsigned short* vr = p.v + b * p.vb + kvh * p.vh + (long long)kjc * p.vn + 8 * hi;
+#pragma unroll
         for (int kk = 0; kk < KK; ++kk) { kf[kk] = *(const u16x8*)(kr + kk * 16); vf[kk] = *(const u16x8*)(vr + kk * 16); }
     }
     const float a2 = p.scale * GGW_LOG2E;
@@ -747,6 +816,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_dkv_kernel(GgWinParams p) {
     float r_lse = 0.f, r_d = 0.f;
     int r_pos = 0;
     auto load = [&](int i0) {
+#pragma unroll
         for (int s = 0; s < D / 32; ++s) {
             const int v = threadIdx.x + 256 * s, c8 = v % (D / 8);
             int r = i0 + v / (D / 8);
@@ -768,7 +838,9 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_dkv_kernel(GgWinParams p) {
     bool again = false;             // the second walk: a key that a row with a NaN or an infinity sees gets NaN, the others go without that row
     float nan = 0.f;
 walk:
+#pragma unroll
     for (int i = 0; i < 2 * DB; ++i)
+#pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     if (threadIdx.x == 0) sAgain = 0;
     if (ra <= rb) load((int)ra);
@@ -783,6 +855,7 @@ walk:
         if (threadIdx.x < 64) { sLse[threadIdx.x] = r_lse; sD[threadIdx.x] = r_d; sPos[threadIdx.x] = r_pos; }
         gg_sync();
         if (i0 + 64 <= (int)rb) load(i0 + 64);
+#pragma unroll
         for (int ib = 0; ib < 2; ++ib) {
             // the 32 rows' positions: all there, and the wave's 32 keys all seen by all of them?
             const int r1 = i0 + ib * 32 + 31;
@@ -791,20 +864,25 @@ walk:
             if (kj0 > phi + p.right || (wlast < plo - p.left && kj0 >= p.sinks) || kj0 >= len) continue;
             const bool full = whole && r1 <= (int)rb && wlast <= plo + p.right && (kj0 >= phi - p.left || wlast < p.sinks);
             f32x16 st, dp;
+#pragma unroll
             for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
                 st = ggw_mfma<T>(ggw_frag<D>(sQ, ib * 32, kk, lane), kf[kk], st);
                 dp = ggw_mfma<T>(ggw_frag<D>(sG, ib * 32, kk, lane), vf[kk], dp);
             }
+#pragma unroll
             for (int gq = 0; gq < 4; ++gq) {
                 const int at = ib * 32 + 8 * gq + 4 * hi;
                 const f32x4 ls = *(const f32x4*)&sLse[at], dd = *(const f32x4*)&sD[at];
+#pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 4 * gq + e;
                     st[r] = gg_exp2f(gg_fmaf(st[r], a2, -ls[e]));
                     dp[r] = st[r] * (dp[r] - dd[e]);
                 }
                 if (!full)
+#pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int r = 4 * gq + e, pos = sPos[at + e];
                         const bool see = kept && kj <= pos + p.right && (kj >= pos - p.left || kj < p.sinks);
@@ -812,8 +890,10 @@ walk:
                         dp[r] = see ? dp[r] : 0.f;
                     }
             }
+#pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const u16x8 pf = ggw_pack8<T>(st, c), sf = ggw_pack8<T>(dp, c);
+#pragma unroll
                 for (int db = 0; db < DB; ++db) {
                     dvt[db] = ggw_mfma<T>(ggw_frag_tr<D>(sG, db * 32, ib * 32 + 16 * c, lane), pf, dvt[db]);
                     dkt[db] = ggw_mfma<T>(ggw_frag_tr<D>(sQ, db * 32, ib * 32 + 16 * c, lane), sf, dkt[db]);
@@ -839,7 +919,9 @@ walk:
     }
     if (chunked) {
         float* po = p.part_o + ((((long long)bkv * p.sink_tiles + tile) * p.sink_chunks + chunk) * 2 * 128 + wave * 32 + (lane & 31)) * D;
+#pragma unroll
         for (int db = 0; db < DB; ++db)
+#pragma unroll
             for (int gq = 0; gq < 4; ++gq) {
                 const int d = db * 32 + 8 * gq + 4 * hi;
                 *(f32x4*)(po + d) = f32x4{dkt[db][4 * gq] + nan, dkt[db][4 * gq + 1] + nan, dkt[db][4 * gq + 2] + nan, dkt[db][4 * gq + 3] + nan};
@@ -849,9 +931,12 @@ walk:
     }
     if (kj >= p.m) return;
     const long long krow = (((long long)b * p.m + kj) * p.hk + kvh) * D;
+#pragma unroll
     for (int db = 0; db < DB; ++db)
+#pragma unroll
         for (int gq = 0; gq < 4; ++gq) {
             u16x4 k4, v4;
+#pragma unroll
             for (int e = 0; e < 4; ++e) {
                 k4[e] = gg_elt<T>(dkt[db][4 * gq + e] * p.scale + nan);
                 v4[e] = gg_elt<T>(dvt[db][4 * gq + e] + nan);
@@ -879,6 +964,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_sink_kernel(GgWinParams p) {
     const int b = bkv / p.hk, kvh = bkv - b * p.hk;
     const long long at = (((long long)b * p.m + j) * p.hk + kvh) * D + d;
     u16x4 k4, v4;
+#pragma unroll
     for (int e = 0; e < 4; ++e) { k4[e] = gg_elt<T>(sk[e] * p.scale); v4[e] = gg_elt<T>(sv[e]); }
     *(u16x4*)(p.dk + at) = k4;
     *(u16x4*)(p.dv + at) = v4;
