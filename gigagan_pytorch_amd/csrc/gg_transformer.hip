@@ -127,6 +127,7 @@ extern "C" int gg_rotary(const gg_rotary_desc* d, void* stream) {
 // what a call launches: a function of the sizes alone, so that the workspace query and the call agree
 struct GgWinPlan {
     bool few;                   // rows fit one 32-row tile: gg_win_few_kernel
+    int waves;                  // else: waves of 32 rows a workgroup
     int row_tiles, splits;      // forward
     int key_tiles, sink_tiles, sink_chunks;     // dk / dv
     size_t fwd_bytes, bwd_bytes;
@@ -139,7 +140,8 @@ static GgWinPlan gg_win_plan(const gg_window_desc* d) {
     const long long g = d->h / d->hk, rows = (long long)d->n * g, heads = (long long)d->B * d->hk;
     const long long left = gg_win_bound(d->left), right = gg_win_bound(d->right), sinks = d->sinks < d->m ? d->sinks : d->m;
     w.few = rows <= 32;
-    const int tr = w.few ? 32 : 128, tk = w.few ? 32 : 64;
+    w.waves = d->d == 128 && heads * ((rows + 255) / 256) >= 256 ? 8 : 4;
+    const int tr = w.few ? 32 : 32 * w.waves, tk = w.few ? 32 : 64;
     w.row_tiles = (int)((rows + tr - 1) / tr);
     // keys that one row tile visits at most, in tiles
     long long span = left + right + (rows < tr ? rows : tr) / g + 1 + sinks;
@@ -150,7 +152,7 @@ static GgWinPlan gg_win_plan(const gg_window_desc* d) {
     long long s = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks;
     if (s > tiles / least) s = tiles / least;
     if (s > 64) s = 64;
-    w.splits = (int)(s < 1 ? 1 : s);
+    w.splits = (int)(s < 1 || w.waves == 8 ? 1 : s);
     w.fwd_bytes = w.splits > 1 ? (size_t)w.splits * heads * rows * (d->d + 2) * sizeof(float) : 0;
     w.key_tiles = (d->m + 127) / 128;
     w.sink_tiles = (int)((sinks + 127) / 128);
@@ -178,9 +180,15 @@ static int gg_win_check(const char* who, const gg_window_desc* d, GgWinParams& p
     for (const void* x : ptrs)
         if ((unsigned long long)x & 15) return gg_fail(-4, "%s: operands must be 16-byte aligned", who);
     const int64_t* strides[] = {d->q_strides, d->k_strides, d->v_strides, d->d_o ? d->g_strides : d->q_strides};
-    for (const int64_t* s : strides)
+    for (int w = 0; w < 4; ++w) {
+        const int64_t* s = strides[w];
         for (int i = 0; i < 3; ++i)
             if (s[i] < 0 || (s[i] & 7)) return gg_fail(-4, "%s: strides must be multiples of 8 elements", who);
+        // a tile of 64 rows is addressed by 32-bit offsets from its first token
+        const bool query = w == 0 || w == 3;
+        if (s[2] >= GG_WINDOW_MAX_STRIDE || (query && s[1] >= 64ll * GG_WINDOW_MAX_STRIDE / g))
+            return gg_fail(-4, "%s: token strides must be below 2^24 elements and head strides of queries below 2^30 a group", who);
+    }
     memset(&p, 0, sizeof(p));
     p.q = (const unsigned short*)d->q; p.k = (const unsigned short*)d->k; p.v = (const unsigned short*)d->v;
     p.d_o = (const unsigned short*)d->d_o;
@@ -228,8 +236,9 @@ extern "C" int gg_window_fwd(const gg_window_desc* d, void* workspace, size_t wo
     hipStream_t s = (hipStream_t)stream;
 #define GG_WIN_GO(T, D)                                                                                                       \
     if (w.few) GG_LAUNCH((gg_win_few_kernel<T, D>), dim3((unsigned)grid), dim3(256), s, p);                                     \
-    else if (w.splits > 1) GG_LAUNCH((gg_win_fwd_kernel<T, D, true>), dim3((unsigned)grid), dim3(256), s, p);                   \
-    else GG_LAUNCH((gg_win_fwd_kernel<T, D, false>), dim3((unsigned)grid), dim3(256), s, p);                                    \
+    else if (w.splits > 1) GG_LAUNCH((gg_win_fwd_kernel<T, D, 4, true>), dim3((unsigned)grid), dim3(256), s, p);                \
+    else if (w.waves == 8) GG_LAUNCH((gg_win_fwd_kernel<T, D, 8, false>), dim3((unsigned)grid), dim3(512), s, p);               \
+    else GG_LAUNCH((gg_win_fwd_kernel<T, D, 4, false>), dim3((unsigned)grid), dim3(256), s, p);                                 \
     rc = gg_check_launch();                                                                                                   \
     if (rc || w.splits == 1) return rc;                                                                                       \
     GG_LAUNCH((gg_win_join_kernel<T, D>), dim3((unsigned)((all * (D / 4) + 255) / 256)), dim3(256), s, p);
@@ -247,14 +256,15 @@ extern "C" int gg_window_bwd(const gg_window_desc* d, void* workspace, size_t wo
     if (w.bwd_bytes && (!workspace || workspace_bytes < w.bwd_bytes || ((unsigned long long)workspace & 15)))
         return gg_fail(-5, "gg_window_bwd: needs %zu workspace bytes, 16-byte aligned", w.bwd_bytes);
     const long long rows = (long long)p.n * p.g, heads = (long long)p.B * p.hk;
-    const long long dq_grid = heads * ((rows + 127) / 128);
+    const long long dq_tiles = (rows + 32 * w.waves - 1) / (32 * w.waves), dq_grid = heads * dq_tiles;
     const long long kv_grid = heads * ((long long)w.sink_tiles * w.sink_chunks + w.key_tiles - w.sink_tiles);
     if (dq_grid > 0x7fffffffll || kv_grid > 0x7fffffffll) return gg_fail(-2, "gg_window_bwd: too many rows");
     hipStream_t s = (hipStream_t)stream;
     p.part_o = (float*)workspace;
 #define GG_WIN_GO(T, D)                                                                                                       \
-    p.row_tiles = (int)((rows + 127) / 128);                                                                                  \
-    GG_LAUNCH((gg_win_dq_kernel<T, D>), dim3((unsigned)dq_grid), dim3(256), s, p);                                              \
+    p.row_tiles = (int)dq_tiles;                                                                                              \
+    if (w.waves == 8) GG_LAUNCH((gg_win_dq_kernel<T, D, 8>), dim3((unsigned)dq_grid), dim3(512), s, p);                         \
+    else GG_LAUNCH((gg_win_dq_kernel<T, D, 4>), dim3((unsigned)dq_grid), dim3(256), s, p);                                      \
     rc = gg_check_launch();                                                                                                   \
     if (rc) return rc;                                                                                                        \
     p.row_tiles = w.key_tiles; p.sink_tiles = w.sink_tiles; p.sink_chunks = w.sink_chunks;                                    \

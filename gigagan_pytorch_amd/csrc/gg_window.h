@@ -16,13 +16,14 @@
 // Key tiles outside the window are not visited; the tiles a wave sees entirely take no mask arithmetic.
 //
 // NaN and infinities. Where a row does not see a key its probability is an exact zero, but zero times a NaN in the shared tile is NaN.
-// Keys that no row of the workgroup sees are staged as zeros. For the rest every kernel looks at its own result once, at the end: if
-// something in it is not finite, the tiles are walked a second time with every non-finite vector taken out of the tile and accounted
-// for by itself, key by key, for the rows that see it. Finite inputs never take the second walk.
+// Keys behind the sequence's end are staged as zeros. For the rest every kernel looks at its own result once, at the end: if something in
+// it is not finite, the tiles are walked a second time with every non-finite vector taken out of the tile and accounted for by itself,
+// key by key, for the rows that see it. Finite inputs never take the second walk.
 #pragma once
 #include "gg_element.h"
 
 #define GGW_NONE 0x20000000          // "no bound" of a window side, and (negated, doubled) the position of a row that is not there
+#define GGW_SPAN 0xf0000000u         // buffer length behind a row tile's first token; an offset of this size reads zeros
 #define GGW_LOG2E 1.4426950408889634f
 #define GGW_TAU 8.0f                 // the running maximum moves when a score exceeds it by 2^8: fewer rescales of the output, P <= 2^8
 
@@ -79,19 +80,32 @@ GG_DEVICE bool ggw_not_finite(const f32x16* v) {
         for (int r = 0; r < 16; ++r) s = gg_fmaf(v[i][r], 0.f, s);
     return s != s;
 }
-template <int D> struct GgwTile { static constexpr int PITCH = 2 * D + 32; static constexpr int BYTES = 64 * PITCH; };
+// A tile is 64 rows of D features as the LDS-DMA deposits them: wave instruction after wave instruction of 64 x 16 bytes, rows back to
+// back. No padding is possible, so the 16-byte vectors of a row are permuted instead: vector c lies at position c ^ ggw_swz(row) (the
+// DMA's source addresses are permuted, its LDS addresses cannot be). Eight consecutive rows then hit eight different vectors (row reads,
+// ds_read_b128) and four consecutive rows four different PAIRS of vectors (transpose reads, 32 bytes of each row).
+template <int D> struct GgwTile { static constexpr int BYTES = 64 * D * 2; };
+template <int D>
+GG_DEVICE int ggw_swz(int row) {
+    if constexpr (D == 32) return (row >> 2) & 3;           // (64-byte rows: four of them span the banks)
+    else return ((row & 3) << 1) ^ ((row >> 2) & 1);
+}
 
 // A operand, rows as they lie: lane l -> row row0 + (l & 31), features kk*16 + 8(l >> 5) + 0..7
 template <int D>
 GG_DEVICE u16x8 ggw_frag(const char* tile, int row0, int kk, int lane) {
-    return *(const u16x8*)(tile + (row0 + (lane & 31)) * GgwTile<D>::PITCH + (kk * 16 + 8 * (lane >> 5)) * 2);
+    const int row = lane & 31;                              // (row0 is a multiple of 32: it does not change the permutation)
+    return *(const u16x8*)(tile + row0 * D * 2 + ((row * D * 2 + (((lane >> 5) ^ ggw_swz<D>(row)) << 4)) ^ (kk << 5)));
 }
 // A operand of the tile's transpose: lane l -> feature d0 + (l & 31), slots (hi, e) <-> rows rb + 4hi + (e & 3) + 8(e >> 2)
 template <int D>
 GG_DEVICE u16x8 ggw_frag_tr(const char* tile, int d0, int rb, int lane) {
     const int i = lane & 15, gq = lane >> 4;
-    const char* p = tile + (rb + 4 * (gq >> 1) + (i >> 2)) * GgwTile<D>::PITCH + (d0 + (gq & 1) * 16 + 4 * (i & 3)) * 2;
-    const u16x4 a = gg_lds_read_tr16((const bf16_t*)p), b = gg_lds_read_tr16((const bf16_t*)(p + 8 * GgwTile<D>::PITCH));
+    const int row = 4 * (gq >> 1) + (i >> 2), c = 2 * (gq & 1) + ((i & 3) >> 1);
+    // (rb is a multiple of 16; rows 8 further on have the same permutation, except in 64-byte rows)
+    const char* p = tile + rb * D * 2 + ((row * D * 2 + ((c ^ ggw_swz<D>(row)) << 4) + 8 * (i & 1)) ^ (d0 << 1));
+    const char* p8 = D == 32 ? tile + (rb + 8 + row) * D * 2 + ((c ^ ggw_swz<D>(row + 8)) << 4) + 8 * (i & 1) : p + 16 * D;
+    const u16x4 a = gg_lds_read_tr16((const bf16_t*)p), b = gg_lds_read_tr16((const bf16_t*)p8);
     return u16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
@@ -130,29 +144,44 @@ GG_DEVICE GgwRange ggw_range(const GgWinParams& p, int len, int t0, int t1) {
     return r;
 }
 GG_DEVICE int ggw_tile_at(const GgwRange& r, int i) { return i < r.st ? i : r.w0 + i - r.st; }
-// a key that some row of the range sees (key mask apart): others are staged as zeros, so that what lies there (stale cache slots,
-// NaN padding) never meets a zero probability in a product
+// a key that some row of the range sees (key mask apart)
 GG_DEVICE bool ggw_in_range(const GgwRange& r, int sinks, int j) { return j <= r.khi && (j >= r.klo || j < sinks); }
 
-// a 64-row tile on its way from memory to LDS: 256 threads, 16 bytes each per step
-template <int D> struct GgwRegs { u16x8 v[D / 32]; };
-template <int D>
-GG_DEVICE void ggw_store_tile(const GgwRegs<D>& r, char* tile) {
+// One 64-row tile from memory to LDS by DMA: NW waves, D / (8 NW) instructions each. `base` points at the tile's first row, `rows` of it
+// exist (the rest is deposited as zeros by the buffer's bounds check). voff[] = ggw_dma_offsets.
+template <int D, int NW> struct GgwDma { static constexpr int N = D / (8 * NW) < 1 ? 1 : D / (8 * NW); };
+template <int D, int NW>
+GG_DEVICE void ggw_dma_offsets(unsigned* voff, long long stride) {
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-        const int v = threadIdx.x + 256 * i, row = v / (D / 8), c8 = v % (D / 8);
-        *(u16x8*)(tile + row * GgwTile<D>::PITCH + c8 * 16) = r.v[i];
+    for (int i = 0; i < GgwDma<D, NW>::N; ++i) {
+        const int v = threadIdx.x + 64 * NW * i, row = v / (D / 8), c = v % (D / 8);
+        voff[i] = (unsigned)(row * stride * 2) + ((c ^ ggw_swz<D>(row)) << 4);
     }
 }
-// the second walk: vectors with a NaN or an infinity are taken out and marked, bad[row][vector]
-template <int T, int D>
-GG_DEVICE void ggw_take_bad(GgwRegs<D>& r, unsigned char* bad, bool add) {
+template <int D, int NW>
+GG_DEVICE void ggw_dma(const unsigned short* base, int rows, long long stride, const unsigned* voff, char* tile, int wave) {
+    if (GgwDma<D, NW>::N * 8 * NW > D && wave >= D / 8) return;             // (D 32, eight waves: four of them have nothing to fetch)
+    const unsigned long long bytes = rows <= 0 ? 0 : ((unsigned long long)(rows < 64 ? rows - 1 : 63) * stride + D) * 2;
+    const GgBufS buf = gg_make_bufs(base, bytes);
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-        const bool b = ggw_bad8<T>(r.v[i]);
-        if (b) r.v[i] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-        const int at = threadIdx.x + 256 * i;               // = row * (D / 8) + vector
-        bad[at] = (unsigned char)((add ? bad[at] : 0) | b);
+    for (int i = 0; i < GgwDma<D, NW>::N; ++i) gg_bufs_load_lds16(buf, voff[i], 0, tile + (wave + NW * i) * 1024);
+}
+
+// The second walk's tile, through registers: rows that `want` names, the others zeros; vectors with a NaN or an infinity are taken out
+// and marked, bad[row][vector] (add: on top of what is marked there; bad null: all stay).
+template <int T, int D, int NW, class Row>
+GG_DEVICE void ggw_stage_clean(char* tile, unsigned char* bad, bool add, Row row_at) {
+    for (int v = threadIdx.x; v < 64 * (D / 8); v += 64 * NW) {
+        const int row = v / (D / 8), c = v % (D / 8);
+        const unsigned short* src = row_at(row);            // null: nobody sees it
+        u16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (src) x = *(const u16x8*)(src + c * 8);
+        if (bad) {
+            const bool b = ggw_bad8<T>(x);
+            if (b) x = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+            bad[v] = (unsigned char)((add ? bad[v] : 0) | b);
+        }
+        *(u16x8*)(tile + row * D * 2 + ((c ^ ggw_swz<D>(row)) << 4)) = x;
     }
 }
 template <int D>
@@ -177,7 +206,7 @@ GG_DEVICE void ggw_add_bad(f32x16* ot, const unsigned char* bad, int tk, int j0,
             for (int e = 0; e < 8; ++e) s = gg_fmaf(gg_elt_f<T>(qf[kk][e]), gg_elt_f<T>(kv[e]), s);
         }
         s = gg_sum_xor32(s);
-        const float pj = see(j, jr) ? gg_exp2f(gg_fmaf(s, a2, -m)) : 0.f;
+        const float pj = see(j) ? gg_exp2f(gg_fmaf(s, a2, -m)) : 0.f;
 #pragma unroll
         for (int c = 0; c < D / 8; ++c)
             if (bad[jr * (D / 8) + c]) {
@@ -186,18 +215,6 @@ GG_DEVICE void ggw_add_bad(f32x16* ot, const unsigned char* bad, int tk, int j0,
                 for (int e = 0; e < 4; ++e) ot[c / 4][4 * (c % 4) + e] += pj > 0.f ? pj * gg_elt_f<T>(v4[e]) : 0.f;
             }
     }
-}
-// keys j0 .. j0 + 63 of one (batch, key head)
-template <int D>
-GG_DEVICE GgwRegs<D> ggw_load_keys(const unsigned short* base, long long stride, int j0, const GgwRange& rg, int sinks, const unsigned char* keep) {
-    GgwRegs<D> r;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-        const int v = threadIdx.x + 256 * i, j = j0 + v / (D / 8), c8 = v % (D / 8);
-        r.v[i] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-        if (ggw_in_range(rg, sinks, j) && (!keep || keep[j])) r.v[i] = *(const u16x8*)(base + (long long)j * stride + c8 * 8);
-    }
-    return r;
 }
 
 // this lane's row of the tile that starts at row r0, and the wave's 32 rows
@@ -216,16 +233,47 @@ GG_DEVICE GgwRow ggw_row(const GgWinParams& p, int r, int len) {
     return w;
 }
 
+// the rows of one wave, lane by lane, and what its 32 rows see between them
+struct GgwWave {
+    GgwRow row;
+    int r0, r;              // the wave's first row, this lane's
+    int lo, hi;             // this lane: window keys lo .. hi (hi = -1: nothing)
+    int lo_any, hi_any;     // (wave-uniform) window keys that some / all of the wave's rows see
+    int lo_all, hi_all;
+    bool there;             // some row exists
+};
+GG_DEVICE GgwWave ggw_wave(const GgWinParams& p, int r0, int len, bool masked) {
+    GgwWave w;
+    const int rows = p.n * p.g, lane = threadIdx.x & 63, shift = len - p.n;
+    w.r0 = r0;
+    w.r = r0 + (lane & 31);
+    w.row = ggw_row(p, w.r, len);
+    w.there = r0 < rows;
+    const int last = r0 + 31 < rows ? r0 + 31 : rows - 1;
+    const int plo = r0 / p.g + shift, phi = last / p.g + shift;
+    w.lo = w.row.pos - p.left;
+    w.hi = w.row.in ? (w.row.pos + p.right < len - 1 ? w.row.pos + p.right : len - 1) : -1;
+    w.lo_any = plo - p.left;
+    w.hi_any = w.there ? (phi + p.right < len - 1 ? phi + p.right : len - 1) : -1;
+    w.lo_all = phi - p.left;
+    // rows that are missing or padding see nothing, and a key mask may take any key away: no tile is whole then
+    w.hi_all = r0 + 31 < rows && plo >= 0 && !masked ? (plo + p.right < len - 1 ? plo + p.right : len - 1) : -1;
+    return w;
+}
+GG_DEVICE bool ggw_some(const GgwWave& w, int sinks, int j0, int j1) { return j0 <= w.hi_any && (j1 >= w.lo_any || j0 < sinks); }
+GG_DEVICE bool ggw_whole(const GgwWave& w, int sinks, int j0, int j1) { return j1 <= w.hi_all && (j0 >= w.lo_all || j1 < sinks); }
+GG_DEVICE bool ggw_sees(const GgwWave& w, int sinks, int j) { return j <= w.hi && (j >= w.lo || j < sinks); }
+
 // ---- forward -------------------------------------------------------------------------------------------------------
-// workgroup: 4 waves x 32 rows, key tiles of 64 staged once for all four, double buffered (one barrier a tile).
+// workgroup: NW waves x 32 rows, key tiles of 64 fetched once for all of them by LDS-DMA, double buffered: one barrier a tile, behind
+// which the next tile's transfers start and run under this tile's arithmetic.
 // SPLIT: the tiles are dealt out to p.splits workgroups, which leave (m, l, O) for gg_win_join_kernel.
-template <int T, int D, bool SPLIT>
-GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_fwd_kernel(GgWinParams p) {
+template <int T, int D, int NW, bool SPLIT>
+GG_KERNEL GG_LAUNCH_BOUNDS2(64 * NW, 2) void gg_win_fwd_kernel(GgWinParams p) {
     constexpr int KK = D / 16, DB = D / 32;
-    GG_SHARED __attribute__((aligned(16))) char sK[2][GgwTile<D>::BYTES];
-    GG_SHARED __attribute__((aligned(16))) char sV[2][GgwTile<D>::BYTES];
-    GG_SHARED unsigned char sKeep[2][64];
-    GG_SHARED __attribute__((aligned(16))) unsigned char sBad[2][64 * (D / 8)];
+    GG_SHARED __attribute__((aligned(1024))) char sK[2][GgwTile<D>::BYTES];
+    GG_SHARED __attribute__((aligned(1024))) char sV[2][GgwTile<D>::BYTES];
+    GG_SHARED __attribute__((aligned(16))) unsigned char sBad[64 * (D / 8)];
     GG_SHARED int sAgain;
 
     const int lane = threadIdx.x & 63, wave = gg_uniform(threadIdx.x >> 6), hi = lane >> 5;
@@ -236,45 +284,32 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_fwd_kernel(GgWinParams p) {
     const int b = bkv / p.hk, kvh = bkv - b * p.hk;
     const int rows = p.n * p.g;
     const int len = ggw_len(p, b);
-    const int r0 = tile * 128, rl = r0 + 127 < rows - 1 ? r0 + 127 : rows - 1;
+    const int r0 = tile * (32 * NW), rl = r0 + 32 * NW - 1 < rows - 1 ? r0 + 32 * NW - 1 : rows - 1;
     const GgwRange rg = ggw_range<64>(p, len, r0 / p.g, rl / p.g);
     const int ta = SPLIT ? (int)((long long)rg.nt * split / p.splits) : 0, tb = SPLIT ? (int)((long long)rg.nt * (split + 1) / p.splits) : rg.nt;
 
-    const int wr0 = r0 + wave * 32;
-    const GgwRow row = ggw_row(p, wr0 + (lane & 31), len);
-    const bool whole = wr0 + 31 < rows && wr0 / p.g + len - p.n >= 0;          // (wave-uniform) 32 rows, none of them padding
-    const int wlo = wr0 / p.g + len - p.n, whi = (wr0 + 31 < rows ? wr0 + 31 : rows - 1) / p.g + len - p.n;
-    const int lo = row.pos - p.left, hij = row.in ? (row.pos + p.right < len - 1 ? row.pos + p.right : len - 1) : -1;
-    const int whij = whi + p.right < len - 1 ? whi + p.right : len - 1, wlij = wlo + p.right < len - 1 ? wlo + p.right : len - 1;
-
+    const unsigned char* keep = p.keep ? p.keep + b * p.keep_b : nullptr;
+    const GgwWave w = ggw_wave(p, r0 + wave * 32, len, keep != nullptr);
     const unsigned short* kb = p.k + b * p.kb + kvh * p.kh;
     const unsigned short* vb = p.v + b * p.vb + kvh * p.vh;
-    const unsigned char* keep = p.keep ? p.keep + b * p.keep_b : nullptr;
     u16x8 qf[KK];
     {
-        const unsigned short* qr = p.q + b * p.qb + (long long)(kvh * p.g + row.head) * p.qh + (long long)row.token * p.qn + 8 * hi;
+        const unsigned short* qr = p.q + b * p.qb + (long long)(kvh * p.g + w.row.head) * p.qh + (long long)w.row.token * p.qn + 8 * hi;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) qf[kk] = *(const u16x8*)(qr + kk * 16);
     }
+    unsigned ko[GgwDma<D, NW>::N], vo[GgwDma<D, NW>::N];
+    ggw_dma_offsets<D, NW>(ko, p.kn);
+    ggw_dma_offsets<D, NW>(vo, p.vn);
+    auto fetch = [&](int i, int buf) {
+        const int j0 = ggw_tile_at(rg, i) * 64;
+        ggw_dma<D, NW>(kb + (long long)j0 * p.kn, len - j0, p.kn, ko, sK[buf], wave);
+        ggw_dma<D, NW>(vb + (long long)j0 * p.vn, len - j0, p.vn, vo, sV[buf], wave);
+    };
     const float a2 = p.scale * GGW_LOG2E;
     float m, l;
     f32x16 ot[DB];
-
-    GgwRegs<D> rk, rv;
-    unsigned char rkeep = 1;
-    auto load = [&](int i) {
-        const int j0 = ggw_tile_at(rg, i) * 64;
-        rk = ggw_load_keys<D>(kb, p.kn, j0, rg, p.sinks, keep);
-        rv = ggw_load_keys<D>(vb, p.vn, j0, rg, p.sinks, keep);
-        if (keep && threadIdx.x < 64) rkeep = j0 + (int)threadIdx.x < len ? keep[j0 + threadIdx.x] : 0;
-    };
     bool again = false;             // the second walk (workgroup-uniform)
-    auto store = [&](int buf) {
-        if (again) ggw_take_bad<T, D>(rv, sBad[buf], false);
-        ggw_store_tile<D>(rk, sK[buf]);
-        ggw_store_tile<D>(rv, sV[buf]);
-        if (keep && threadIdx.x < 64) sKeep[buf][threadIdx.x] = rkeep;
-    };
 walk:
     m = -1.0e30f;
     l = 0.f;
@@ -282,81 +317,80 @@ walk:
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) ot[db][r] = 0.f;
-    if (ta < tb) {
-        load(ta);
-        store(0);
-        if (ta + 1 < tb) load(ta + 1);
-    }
     if (threadIdx.x == 0) sAgain = 0;
-    gg_sync();
+    if (!again && ta < tb) fetch(ta, 0);
     for (int i = ta, buf = 0; i < tb; ++i, buf ^= 1) {
-        if (i + 1 < tb) {
-            store(buf ^ 1);         // (free since the barrier that ended the last tile)
-            if (i + 2 < tb) load(i + 2);
-        }
         const int j0 = ggw_tile_at(rg, i) * 64;
-        if (j0 <= whij && (j0 + 63 >= wlo - p.left || j0 < p.sinks) && wr0 < rows) {
-            f32x16 st[2];
+        if (!again) {
+            gg_wait_vm<0>();
+            gg_barrier_lds();       // this tile is there for everyone, and everyone is through with the last one: its buffer is free
+            if (i + 1 < tb) fetch(i + 1, buf ^ 1);
+        } else {
+            gg_sync();
+            auto in = [&](int j) { return ggw_in_range(rg, p.sinks, j) && (!keep || keep[j]); };
+            ggw_stage_clean<T, D, NW>(sK[buf], nullptr, false, [&](int row) { return in(j0 + row) ? kb + (long long)(j0 + row) * p.kn : nullptr; });
+            ggw_stage_clean<T, D, NW>(sV[buf], sBad, false, [&](int row) { return in(j0 + row) ? vb + (long long)(j0 + row) * p.vn : nullptr; });
+            gg_sync();
+        }
+        if (!ggw_some(w, p.sinks, j0, j0 + 63)) continue;
+        f32x16 st[2];
 #pragma unroll
-            for (int jb = 0; jb < 2; ++jb) {
+        for (int jb = 0; jb < 2; ++jb) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) st[jb][r] = 0.f;
+            for (int r = 0; r < 16; ++r) st[jb][r] = 0.f;
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk) st[jb] = ggw_mfma<T>(ggw_frag<D>(sK[buf], jb * 32, kk, lane), qf[kk], st[jb]);
-            }
-            if (!(whole && !keep && j0 + 63 <= wlij && (j0 >= whi - p.left || j0 + 63 < p.sinks))) {
-                unsigned long long bits = ~0ull;
-                if (keep) bits = gg_ballot(sKeep[buf][lane] != 0);
-                bits >>= 4 * hi;
-#pragma unroll
-                for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int jr = jb * 32 + (r & 3) + 8 * (r >> 2), j = j0 + jr + 4 * hi;
-                        const bool see = j <= hij && (j >= lo || j < p.sinks) && ((bits >> jr) & 1);
-                        st[jb][r] = see ? st[jb][r] : -__builtin_inff();
-                    }
-            }
-            float mx = -__builtin_inff();
-#pragma unroll
-            for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[jb][r]);
-            mx = gg_max_xor32(mx) * a2;
-            if (gg_wave_any(mx > m + GGW_TAU)) {
-                const float mn = fmaxf(m, mx), corr = gg_exp2f(m - mn);
-                l *= corr;
-                m = mn;
-#pragma unroll
-                for (int db = 0; db < DB; ++db)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) ot[db][r] *= corr;
-            }
-            float sum = 0.f;
+            for (int kk = 0; kk < KK; ++kk) st[jb] = ggw_mfma<T>(ggw_frag<D>(sK[buf], jb * 32, kk, lane), qf[kk], st[jb]);
+        }
+        if (!ggw_whole(w, p.sinks, j0, j0 + 63)) {
+            unsigned long long bits = ~0ull;
+            if (keep) bits = gg_ballot(j0 + lane < len && keep[j0 + lane]);
+            bits >>= 4 * hi;
 #pragma unroll
             for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    st[jb][r] = gg_exp2f(gg_fmaf(st[jb][r], a2, -m));
-                    sum += st[jb][r];
+                    const int jr = jb * 32 + (r & 3) + 8 * (r >> 2);
+                    const bool see = ggw_sees(w, p.sinks, j0 + jr + 4 * hi) && ((bits >> jr) & 1);
+                    st[jb][r] = see ? st[jb][r] : -__builtin_inff();
                 }
-            l += sum;
-#pragma unroll
-            for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const u16x8 pf = ggw_pack8<T>(st[jb], c);
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) ot[db] = ggw_mfma<T>(ggw_frag_tr<D>(sV[buf], db * 32, jb * 32 + 16 * c, lane), pf, ot[db]);
-                }
-            if (again)
-                ggw_add_bad<T, D>(ot, sBad[buf], 64, j0, kb, p.kn, vb, p.vn, qf, a2, m, hi, [&](int j, int jr) {
-                    return j <= hij && (j >= lo || j < p.sinks) && (!keep || sKeep[buf][jr]);
-                });
         }
-        gg_sync();
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[jb][r]);
+        mx = gg_max_xor32(mx) * a2;
+        if (gg_wave_any(mx > m + GGW_TAU)) {
+            const float mn = fmaxf(m, mx), corr = gg_exp2f(m - mn);
+            l *= corr;
+            m = mn;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) ot[db][r] *= corr;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                st[jb][r] = gg_exp2f(gg_fmaf(st[jb][r], a2, -m));
+                sum += st[jb][r];
+            }
+        l += sum;
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const u16x8 pf = ggw_pack8<T>(st[jb], c);
+#pragma unroll
+                for (int db = 0; db < DB; ++db) ot[db] = ggw_mfma<T>(ggw_frag_tr<D>(sV[buf], db * 32, jb * 32 + 16 * c, lane), pf, ot[db]);
+            }
+        if (again)
+            ggw_add_bad<T, D>(ot, sBad, 64, j0, kb, p.kn, vb, p.vn, qf, a2, m, hi, [&](int j) { return ggw_sees(w, p.sinks, j) && (!keep || keep[j]); });
     }
     if (!again) {
+        gg_sync();
         if (ggw_not_finite<DB>(ot)) sAgain = 1;
         gg_sync();
         if (sAgain) {
@@ -366,9 +400,8 @@ walk:
         }
     }
     l = gg_sum_xor32(l);
-    const int r = wr0 + (lane & 31);
-    if (r >= rows) return;
-    const long long at = (long long)bkv * rows + r;
+    if (w.r >= rows) return;
+    const long long at = (long long)bkv * rows + w.r;
     if (SPLIT) {
         const long long sp = (long long)split * p.B * p.hk * rows + at;
         float* po = p.part_o + sp * D;
@@ -381,7 +414,7 @@ walk:
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    unsigned short* orow = p.o + (((long long)b * p.n + row.token) * p.h + kvh * p.g + row.head) * D;
+    unsigned short* orow = p.o + (((long long)b * p.n + w.row.token) * p.h + kvh * p.g + w.row.head) * D;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -401,8 +434,8 @@ walk:
 // gg_win_join_kernel.
 template <int T, int D>
 GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_few_kernel(GgWinParams p) {
-    constexpr int KK = D / 16, DB = D / 32, PITCH = GgwTile<D>::PITCH;
-    GG_SHARED __attribute__((aligned(16))) char sV[4][32 * PITCH];
+    constexpr int KK = D / 16, DB = D / 32;
+    GG_SHARED __attribute__((aligned(16))) char sV[4][32 * D * 2];
     GG_SHARED __attribute__((aligned(16))) unsigned char sBad[4][32 * (D / 8)];
     GG_SHARED float sM[4][32], sL[4][32];
     GG_SHARED __attribute__((aligned(16))) float sO[32][D + 4];
@@ -469,7 +502,8 @@ walk:
                 if (bad) vr[s] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
                 sBad[wave][v] = bad;
             }
-            *(u16x8*)(sV[wave] + (v / (D / 8)) * PITCH + (v % (D / 8)) * 16) = vr[s];
+            const int vrow = v / (D / 8);
+            *(u16x8*)(sV[wave] + vrow * D * 2 + (((v % (D / 8)) ^ ggw_swz<D>(vrow)) << 4)) = vr[s];
         }
         gg_wave_sync();
         f32x16 st;
@@ -514,10 +548,7 @@ walk:
             for (int db = 0; db < DB; ++db) ot[db] = ggw_mfma<T>(ggw_frag_tr<D>(sV[wave], db * 32, 16 * c, lane), pf, ot[db]);
         }
         if (again)
-            ggw_add_bad<T, D>(ot, sBad[wave], 32, j0, kb, p.kn, vb, p.vn, qf, a2, m, hi, [&](int j, int jr) {
-                (void)jr;
-                return j <= hij && (j >= lo || j < p.sinks) && (!keep || keep[j]);
-            });
+            ggw_add_bad<T, D>(ot, sBad[wave], 32, j0, kb, p.kn, vb, p.vn, qf, a2, m, hi, [&](int j) { return j <= hij && (j >= lo || j < p.sinks) && (!keep || keep[j]); });
     }
     if (!again && gg_wave_any(ggw_not_finite<DB>(ot))) {
         again = true;
@@ -598,14 +629,13 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_join_kernel(GgWinParams p) {
 }
 
 // ---- backward, part 1: dq and D ---------------------------------------------------------------------------------------
-// the forward's mapping: 4 waves x 32 rows, key tiles of 64; K is read as rows (scores) and transposed (dq), V as rows (dP)
-template <int T, int D>
-GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_dq_kernel(GgWinParams p) {
+// the forward's mapping and transfers; K is read as rows (scores) and transposed (dq), V as rows (dP)
+template <int T, int D, int NW>
+GG_KERNEL GG_LAUNCH_BOUNDS2(64 * NW, 2) void gg_win_dq_kernel(GgWinParams p) {
     constexpr int KK = D / 16, DB = D / 32;
-    GG_SHARED __attribute__((aligned(16))) char sK[2][GgwTile<D>::BYTES];
-    GG_SHARED __attribute__((aligned(16))) char sV[2][GgwTile<D>::BYTES];
-    GG_SHARED unsigned char sKeep[2][64];
-    GG_SHARED __attribute__((aligned(16))) unsigned char sBad[2][64 * (D / 8)];
+    GG_SHARED __attribute__((aligned(1024))) char sK[2][GgwTile<D>::BYTES];
+    GG_SHARED __attribute__((aligned(1024))) char sV[2][GgwTile<D>::BYTES];
+    GG_SHARED __attribute__((aligned(16))) unsigned char sBad[64 * (D / 8)];
     GG_SHARED int sAgain;
 
     const int lane = threadIdx.x & 63, wave = gg_uniform(threadIdx.x >> 6), hi = lane >> 5;
@@ -614,28 +644,20 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_dq_kernel(GgWinParams p) {
     const int b = bkv / p.hk, kvh = bkv - b * p.hk;
     const int rows = p.n * p.g;
     const int len = ggw_len(p, b);
-    const int r0 = tile * 128, rl = r0 + 127 < rows - 1 ? r0 + 127 : rows - 1;
+    const int r0 = tile * (32 * NW), rl = r0 + 32 * NW - 1 < rows - 1 ? r0 + 32 * NW - 1 : rows - 1;
     const GgwRange rg = ggw_range<64>(p, len, r0 / p.g, rl / p.g);
-
-    const int wr0 = r0 + wave * 32;
-    const GgwRow row = ggw_row(p, wr0 + (lane & 31), len);
-    const bool whole = wr0 + 31 < rows && wr0 / p.g + len - p.n >= 0;
-    const int wlo = wr0 / p.g + len - p.n, whi = (wr0 + 31 < rows ? wr0 + 31 : rows - 1) / p.g + len - p.n;
-    const int lo = row.pos - p.left, hij = row.in ? (row.pos + p.right < len - 1 ? row.pos + p.right : len - 1) : -1;
-    const int whij = whi + p.right < len - 1 ? whi + p.right : len - 1, wlij = wlo + p.right < len - 1 ? wlo + p.right : len - 1;
-
+    const unsigned char* keep = p.keep ? p.keep + b * p.keep_b : nullptr;
+    const GgwWave w = ggw_wave(p, r0 + wave * 32, len, keep != nullptr);
     const unsigned short* kb = p.k + b * p.kb + kvh * p.kh;
     const unsigned short* vb = p.v + b * p.vb + kvh * p.vh;
-    const unsigned char* keep = p.keep ? p.keep + b * p.keep_b : nullptr;
-    const int hq = kvh * p.g + row.head;
-    const long long orow = (((long long)b * p.n + row.token) * p.h + hq) * D;
-    const int rr = wr0 + (lane & 31);
-    const long long at = (long long)bkv * rows + (rr < rows ? rr : rows - 1);
+    const int hq = kvh * p.g + w.row.head;
+    const long long orow = (((long long)b * p.n + w.row.token) * p.h + hq) * D;
+    const long long at = (long long)bkv * rows + (w.r < rows ? w.r : rows - 1);
     u16x8 qf[KK], gf[KK];
     float dsum = 0.f;
     {
-        const unsigned short* qr = p.q + b * p.qb + hq * p.qh + (long long)row.token * p.qn + 8 * hi;
-        const unsigned short* gr = p.d_o + b * p.gb + hq * p.gh + (long long)row.token * p.gn + 8 * hi;
+        const unsigned short* qr = p.q + b * p.qb + hq * p.qh + (long long)w.row.token * p.qn + 8 * hi;
+        const unsigned short* gr = p.d_o + b * p.gb + hq * p.gh + (long long)w.row.token * p.gn + 8 * hi;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
             qf[kk] = *(const u16x8*)(qr + kk * 16);
@@ -647,87 +669,79 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_dq_kernel(GgWinParams p) {
     }
     dsum = gg_sum_xor32(dsum);
     const float lse = p.lse[at], a2 = p.scale * GGW_LOG2E;
-    if (hi == 0 && rr < rows) p.dvec[at] = dsum;
-    f32x16 dqt[DB];
-
-    GgwRegs<D> rk, rv;
-    unsigned char rkeep = 1;
-    auto load = [&](int i) {
+    if (hi == 0 && w.r < rows) p.dvec[at] = dsum;
+    unsigned ko[GgwDma<D, NW>::N], vo[GgwDma<D, NW>::N];
+    ggw_dma_offsets<D, NW>(ko, p.kn);
+    ggw_dma_offsets<D, NW>(vo, p.vn);
+    auto fetch = [&](int i, int buf) {
         const int j0 = ggw_tile_at(rg, i) * 64;
-        rk = ggw_load_keys<D>(kb, p.kn, j0, rg, p.sinks, keep);
-        rv = ggw_load_keys<D>(vb, p.vn, j0, rg, p.sinks, keep);
-        if (keep && threadIdx.x < 64) rkeep = j0 + (int)threadIdx.x < len ? keep[j0 + threadIdx.x] : 0;
+        ggw_dma<D, NW>(kb + (long long)j0 * p.kn, len - j0, p.kn, ko, sK[buf], wave);
+        ggw_dma<D, NW>(vb + (long long)j0 * p.vn, len - j0, p.vn, vo, sV[buf], wave);
     };
+    f32x16 dqt[DB];
     bool again = false;             // the second walk: a row that sees a key with a NaN or an infinity gets NaN, the others go without that key
     float nan = 0.f;
-    auto store = [&](int buf) {
-        if (again) {
-            ggw_take_bad<T, D>(rk, sBad[buf], false);
-            ggw_take_bad<T, D>(rv, sBad[buf], true);
-        }
-        ggw_store_tile<D>(rk, sK[buf]);
-        ggw_store_tile<D>(rv, sV[buf]);
-        if (keep && threadIdx.x < 64) sKeep[buf][threadIdx.x] = rkeep;
-    };
 walk:
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dqt[db][r] = 0.f;
-    if (rg.nt > 0) {
-        load(0);
-        store(0);
-        if (rg.nt > 1) load(1);
-    }
     if (threadIdx.x == 0) sAgain = 0;
-    gg_sync();
+    if (!again && rg.nt > 0) {
+        gg_wait_vm<0>();            // (the rows above: the transfers' count starts at zero)
+        fetch(0, 0);
+    }
     for (int i = 0, buf = 0; i < rg.nt; ++i, buf ^= 1) {
-        if (i + 1 < rg.nt) {
-            store(buf ^ 1);
-            if (i + 2 < rg.nt) load(i + 2);
-        }
         const int j0 = ggw_tile_at(rg, i) * 64;
-        if (j0 <= whij && (j0 + 63 >= wlo - p.left || j0 < p.sinks) && wr0 < rows) {
-            const bool masked = !(whole && !keep && j0 + 63 <= wlij && (j0 >= whi - p.left || j0 + 63 < p.sinks));
-            unsigned long long bits = ~0ull;
-            if (keep) bits = gg_ballot(sKeep[buf][lane] != 0);
-            bits >>= 4 * hi;
+        if (!again) {
+            gg_wait_vm<0>();
+            gg_barrier_lds();
+            if (i + 1 < rg.nt) fetch(i + 1, buf ^ 1);
+        } else {
+            gg_sync();
+            auto in = [&](int j) { return ggw_in_range(rg, p.sinks, j) && (!keep || keep[j]); };
+            ggw_stage_clean<T, D, NW>(sK[buf], sBad, false, [&](int row) { return in(j0 + row) ? kb + (long long)(j0 + row) * p.kn : nullptr; });
+            ggw_stage_clean<T, D, NW>(sV[buf], sBad, true, [&](int row) { return in(j0 + row) ? vb + (long long)(j0 + row) * p.vn : nullptr; });
+            gg_sync();
+        }
+        if (!ggw_some(w, p.sinks, j0, j0 + 63)) continue;
+        const bool masked = !ggw_whole(w, p.sinks, j0, j0 + 63);
+        unsigned long long bits = ~0ull;
+        if (keep) bits = gg_ballot(j0 + lane < len && keep[j0 + lane]);
+        bits >>= 4 * hi;
 #pragma unroll
-            for (int jb = 0; jb < 2; ++jb) {
-                f32x16 st, dp;
+        for (int jb = 0; jb < 2; ++jb) {
+            f32x16 st, dp;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = -dsum; }
+            for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = -dsum; }
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk) {
-                    st = ggw_mfma<T>(ggw_frag<D>(sK[buf], jb * 32, kk, lane), qf[kk], st);
-                    dp = ggw_mfma<T>(ggw_frag<D>(sV[buf], jb * 32, kk, lane), gf[kk], dp);
-                }
+            for (int kk = 0; kk < KK; ++kk) {
+                st = ggw_mfma<T>(ggw_frag<D>(sK[buf], jb * 32, kk, lane), qf[kk], st);
+                dp = ggw_mfma<T>(ggw_frag<D>(sV[buf], jb * 32, kk, lane), gf[kk], dp);
+            }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) st[r] = gg_exp2f(gg_fmaf(st[r], a2, -lse)) * dp[r];
-                if (masked)
+            for (int r = 0; r < 16; ++r) st[r] = gg_exp2f(gg_fmaf(st[r], a2, -lse)) * dp[r];
+            if (masked) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int jr = jb * 32 + (r & 3) + 8 * (r >> 2), j = j0 + jr + 4 * hi;
-                        const bool see = j <= hij && (j >= lo || j < p.sinks) && ((bits >> jr) & 1);
-                        st[r] = see ? st[r] : 0.f;
-                    }
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const u16x8 sf = ggw_pack8<T>(st, c);
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) dqt[db] = ggw_mfma<T>(ggw_frag_tr<D>(sK[buf], db * 32, jb * 32 + 16 * c, lane), sf, dqt[db]);
+                for (int r = 0; r < 16; ++r) {
+                    const int jr = jb * 32 + (r & 3) + 8 * (r >> 2);
+                    const bool see = ggw_sees(w, p.sinks, j0 + jr + 4 * hi) && ((bits >> jr) & 1);
+                    st[r] = see ? st[r] : 0.f;
                 }
             }
-            if (again)
-                for (int jr = 0; jr < 64; ++jr)
-                    if (ggw_any_bad<D>(sBad[buf], jr)) {
-                        const int j = j0 + jr;
-                        if (j <= hij && (j >= lo || j < p.sinks) && (!keep || sKeep[buf][jr])) nan = __builtin_nanf("");
-                    }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const u16x8 sf = ggw_pack8<T>(st, c);
+#pragma unroll
+                for (int db = 0; db < DB; ++db) dqt[db] = ggw_mfma<T>(ggw_frag_tr<D>(sK[buf], db * 32, jb * 32 + 16 * c, lane), sf, dqt[db]);
+            }
         }
-        gg_sync();
+        if (again)
+            for (int jr = 0; jr < 64; ++jr)
+                if (ggw_any_bad<D>(sBad, jr) && ggw_sees(w, p.sinks, j0 + jr) && (!keep || keep[j0 + jr])) nan = __builtin_nanf("");
     }
     if (!again) {
+        gg_sync();
         if (ggw_not_finite<DB>(dqt)) sAgain = 1;
         gg_sync();
         if (sAgain) {
@@ -736,7 +750,7 @@ walk:
             goto walk;
         }
     }
-    if (rr >= rows) return;
+    if (w.r >= rows) return;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -749,17 +763,17 @@ walk:
 }
 
 // ---- backward, part 2: dk, dv -----------------------------------------------------------------------------------------
-// workgroup: 4 waves x 32 keys, row tiles of 64 (Q and dO, each read as rows and transposed). The key tiles that hold sinks are seen by
+// workgroup: 4 waves x 32 keys, row tiles of 64 (Q and dO by LDS-DMA, double buffered, each read as rows and transposed). The key tiles that hold sinks are seen by
 // every later row: their rows are cut into p.sink_chunks chunks, each a workgroup of its own that leaves fp32 sums for
 // gg_win_sink_kernel.  part_o: [B*hk][sink_tiles][chunks][2][128][D].
 template <int T, int D>
-GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_dkv_kernel(GgWinParams p) {
+GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
     constexpr int KK = D / 16, DB = D / 32;
-    GG_SHARED __attribute__((aligned(16))) char sQ[GgwTile<D>::BYTES];
-    GG_SHARED __attribute__((aligned(16))) char sG[GgwTile<D>::BYTES];
-    GG_SHARED __attribute__((aligned(16))) float sLse[64];
-    GG_SHARED __attribute__((aligned(16))) float sD[64];
-    GG_SHARED __attribute__((aligned(16))) int sPos[64];
+    GG_SHARED __attribute__((aligned(1024))) char sQ[2][GgwTile<D>::BYTES];
+    GG_SHARED __attribute__((aligned(1024))) char sG[2][GgwTile<D>::BYTES];
+    GG_SHARED __attribute__((aligned(16))) float sLse[2][64];
+    GG_SHARED __attribute__((aligned(16))) float sD[2][64];
+    GG_SHARED __attribute__((aligned(16))) int sPos[2][64];
     GG_SHARED __attribute__((aligned(16))) unsigned char sBad[64 * (D / 8)];
     GG_SHARED int sAgain;
 
@@ -812,28 +826,52 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_dkv_kernel(GgWinParams p) {
 
     const unsigned short* qb = p.q + b * p.qb + (long long)kvh * p.g * p.qh;
     const unsigned short* gb = p.d_o + b * p.gb + (long long)kvh * p.g * p.gh;
-    GgwRegs<D> rq, rg;
+    // this thread's vectors of a row tile: row index -> (token, head) kept up from tile to tile, addresses relative to the tile's first
+    // token (host: they fit 32 bits)
+    constexpr int NV = D / 32;
+    const int step_t = 64 / p.g, step_h = 64 - step_t * p.g;
+    int vt[NV], vh[NV];
+    int rt = 0, rh = 0;                     // the row whose statistics this thread fetches (threads 0 .. 63)
+    auto start = [&](int i0) {
+#pragma unroll
+        for (int s = 0; s < NV; ++s) {
+            const int r = i0 + (int)(threadIdx.x + 256 * s) / (D / 8);
+            vt[s] = (int)((unsigned)r / (unsigned)p.g);
+            vh[s] = r - vt[s] * p.g;
+        }
+        const int r = i0 + (int)(threadIdx.x & 63);
+        rt = (int)((unsigned)r / (unsigned)p.g);
+        rh = r - rt * p.g;
+    };
     float r_lse = 0.f, r_d = 0.f;
     int r_pos = 0;
-    auto load = [&](int i0) {
+    auto fetch = [&](int i0, int buf) {
+        const int t0 = (int)((unsigned)i0 / (unsigned)p.g);
+        const GgBufS bq = gg_make_bufs(qb + (long long)t0 * p.qn, GGW_SPAN), bg = gg_make_bufs(gb + (long long)t0 * p.gn, GGW_SPAN);
 #pragma unroll
-        for (int s = 0; s < D / 32; ++s) {
-            const int v = threadIdx.x + 256 * s, c8 = v % (D / 8);
-            int r = i0 + v / (D / 8);
-            r = r <= (int)rb ? r : (int)rb;
-            const int tok = (int)((unsigned)r / (unsigned)p.g), hd = r - tok * p.g;
-            rq.v[s] = rg.v[s] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-            if (p.lse[(long long)bkv * rows + r] < __builtin_inff()) {          // (a row that sees nothing: zeros, whatever lies there)
-                rq.v[s] = *(const u16x8*)(qb + hd * p.qh + (long long)tok * p.qn + c8 * 8);
-                rg.v[s] = *(const u16x8*)(gb + hd * p.gh + (long long)tok * p.gn + c8 * 8);
-            }
+        for (int s = 0; s < NV; ++s) {
+            const int v = threadIdx.x + 256 * s, row = v / (D / 8), c = (v % (D / 8)) ^ ggw_swz<D>(row);
+            // (rows behind the last one: an offset that the buffer's bounds check turns into zeros)
+            const bool in = i0 + row <= (int)rb;
+            const unsigned oq = in ? (unsigned)(((long long)(vt[s] - t0) * p.qn + (long long)vh[s] * p.qh) * 2) + (c << 4) : GGW_SPAN;
+            const unsigned og = in ? (unsigned)(((long long)(vt[s] - t0) * p.gn + (long long)vh[s] * p.gh) * 2) + (c << 4) : GGW_SPAN;
+            gg_bufs_load_lds16(bq, oq, 0, sQ[buf] + (wave + 4 * s) * 1024);
+            gg_bufs_load_lds16(bg, og, 0, sG[buf] + (wave + 4 * s) * 1024);
+            vt[s] += step_t;
+            vh[s] += step_h;
+            if (vh[s] >= p.g) { vh[s] -= p.g; ++vt[s]; }
         }
-        if (threadIdx.x < 64) {
-            const int r = i0 + (int)threadIdx.x, rc = r <= (int)rb ? r : (int)rb;
-            r_lse = r <= (int)rb ? p.lse[(long long)bkv * rows + rc] : __builtin_inff();
-            r_d = p.dvec[(long long)bkv * rows + rc];
-            r_pos = r <= (int)rb ? (int)((unsigned)r / (unsigned)p.g) + shift : -2 * GGW_NONE;
-        }
+    };
+    auto stats = [&](int i0) {              // lse = +inf: a row that is not there or sees nothing
+        const int r = i0 + (int)(threadIdx.x & 63);
+        const bool in = r <= (int)rb;
+        const long long at = (long long)bkv * rows + (in ? r : (int)rb);
+        r_lse = in ? p.lse[at] : __builtin_inff();
+        r_d = in ? p.dvec[at] : 0.f;
+        r_pos = in ? rt + shift : -2 * GGW_NONE;
+        rt += step_t;
+        rh += step_h;
+        if (rh >= p.g) { rh -= p.g; ++rt; }
     };
     bool again = false;             // the second walk: a key that a row with a NaN or an infinity sees gets NaN, the others go without that row
     float nan = 0.f;
@@ -843,18 +881,32 @@ walk:
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     if (threadIdx.x == 0) sAgain = 0;
-    if (ra <= rb) load((int)ra);
-    for (int i0 = (int)ra; i0 <= (int)rb; i0 += 64) {
-        gg_sync();
-        if (again) {
-            ggw_take_bad<T, D>(rq, sBad, false);
-            ggw_take_bad<T, D>(rg, sBad, true);
+    if (ra <= rb) {
+        start((int)ra);
+        stats((int)ra);
+        if (!again) fetch((int)ra, 0);
+    }
+    for (int i0 = (int)ra, buf = 0; i0 <= (int)rb; i0 += 64, buf ^= 1) {
+        if (threadIdx.x < 64) { sLse[buf][threadIdx.x] = r_lse; sD[buf][threadIdx.x] = r_d; sPos[buf][threadIdx.x] = r_pos; }
+        if (!again) {
+            gg_wait_vm<0>();
+            gg_barrier_lds();
+            if (i0 + 64 <= (int)rb) {
+                stats(i0 + 64);
+                fetch(i0 + 64, buf ^ 1);
+            }
+        } else {
+            gg_sync();
+            auto at = [&](const unsigned short* base, long long hs, long long ns, int row) -> const unsigned short* {
+                const int r = i0 + row, tok = (int)((unsigned)r / (unsigned)p.g);
+                if (r > (int)rb || !(sLse[buf][row] < __builtin_inff())) return nullptr;
+                return base + (long long)tok * ns + (long long)(r - tok * p.g) * hs;
+            };
+            ggw_stage_clean<T, D, 4>(sQ[buf], sBad, false, [&](int row) { return at(qb, p.qh, p.qn, row); });
+            ggw_stage_clean<T, D, 4>(sG[buf], sBad, true, [&](int row) { return at(gb, p.gh, p.gn, row); });
+            if (i0 + 64 <= (int)rb) stats(i0 + 64);
+            gg_sync();
         }
-        ggw_store_tile<D>(rq, sQ);
-        ggw_store_tile<D>(rg, sG);
-        if (threadIdx.x < 64) { sLse[threadIdx.x] = r_lse; sD[threadIdx.x] = r_d; sPos[threadIdx.x] = r_pos; }
-        gg_sync();
-        if (i0 + 64 <= (int)rb) load(i0 + 64);
 #pragma unroll
         for (int ib = 0; ib < 2; ++ib) {
             // the 32 rows' positions: all there, and the wave's 32 keys all seen by all of them?
@@ -868,13 +920,13 @@ walk:
             for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = 0.f; }
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
-                st = ggw_mfma<T>(ggw_frag<D>(sQ, ib * 32, kk, lane), kf[kk], st);
-                dp = ggw_mfma<T>(ggw_frag<D>(sG, ib * 32, kk, lane), vf[kk], dp);
+                st = ggw_mfma<T>(ggw_frag<D>(sQ[buf], ib * 32, kk, lane), kf[kk], st);
+                dp = ggw_mfma<T>(ggw_frag<D>(sG[buf], ib * 32, kk, lane), vf[kk], dp);
             }
 #pragma unroll
             for (int gq = 0; gq < 4; ++gq) {
                 const int at = ib * 32 + 8 * gq + 4 * hi;
-                const f32x4 ls = *(const f32x4*)&sLse[at], dd = *(const f32x4*)&sD[at];
+                const f32x4 ls = *(const f32x4*)&sLse[buf][at], dd = *(const f32x4*)&sD[buf][at];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 4 * gq + e;
@@ -884,7 +936,7 @@ walk:
                 if (!full)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int r = 4 * gq + e, pos = sPos[at + e];
+                        const int r = 4 * gq + e, pos = sPos[buf][at + e];
                         const bool see = kept && kj <= pos + p.right && (kj >= pos - p.left || kj < p.sinks);
                         st[r] = see ? st[r] : 0.f;
                         dp[r] = see ? dp[r] : 0.f;
@@ -895,14 +947,14 @@ walk:
                 const u16x8 pf = ggw_pack8<T>(st, c), sf = ggw_pack8<T>(dp, c);
 #pragma unroll
                 for (int db = 0; db < DB; ++db) {
-                    dvt[db] = ggw_mfma<T>(ggw_frag_tr<D>(sG, db * 32, ib * 32 + 16 * c, lane), pf, dvt[db]);
-                    dkt[db] = ggw_mfma<T>(ggw_frag_tr<D>(sQ, db * 32, ib * 32 + 16 * c, lane), sf, dkt[db]);
+                    dvt[db] = ggw_mfma<T>(ggw_frag_tr<D>(sG[buf], db * 32, ib * 32 + 16 * c, lane), pf, dvt[db]);
+                    dkt[db] = ggw_mfma<T>(ggw_frag_tr<D>(sQ[buf], db * 32, ib * 32 + 16 * c, lane), sf, dkt[db]);
                 }
             }
             if (again)
                 for (int ir = ib * 32; ir < ib * 32 + 32; ++ir)
                     if (ggw_any_bad<D>(sBad, ir)) {
-                        const int pos = sPos[ir];
+                        const int pos = sPos[buf][ir];
                         if (kept && kj <= pos + p.right && (kj >= pos - p.left || kj < p.sinks)) nan = __builtin_nanf("");
                     }
         }

@@ -1537,10 +1537,13 @@ def _strides3(t: torch.Tensor):
     return (C.c_int64 * 3)(*(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])))
 
 
-def _attend4(t: torch.Tensor) -> torch.Tensor:
-    """(B, h, n, d) as the window kernels read it (unit feature stride, strides of whole 16-byte vectors, aligned); else a copy"""
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+def _attend4(t: torch.Tensor, group: int = 0) -> torch.Tensor:
+    """(B, h, n, d) as the window kernels read it (unit feature stride, strides of whole 16-byte vectors below their limits, aligned), or
+    a copy that is; `group`: query heads a key head, for queries"""
+    s = [x if n > 1 else 0 for x, n in zip(t.stride(), t.shape)]
+    ok = (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not (s[0] | s[1] | s[2]) & 7 and s[2] < 1 << 24
+          and (not group or s[1] * group < 1 << 30))
+    return t if ok else t.transpose(1, 2).clone(memory_format=torch.contiguous_format).transpose(1, 2)
 
 
 def _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask):
@@ -1563,7 +1566,7 @@ def window_fwd(q, k, v, scale: float, left: int, right: int, sinks: int, lengths
         return o.transpose(1, 2), lse
     if not k.shape[2]:
         return o.zero_().transpose(1, 2), (lse.fill_(math.inf) if want_lse else None)
-    q, k, v = _attend4(q), _attend4(k), _attend4(v)
+    q, k, v = _attend4(q, h // k.shape[1]), _attend4(k), _attend4(v)
     D = _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask)
     with _on_device(L, q):
         nbytes = L.lib.gg_window_workspace_bytes(C.byref(D), 0)
@@ -1588,7 +1591,7 @@ def window_bwd(q, k, v, o, lse, d_o, scale: float, left: int, right: int, sinks:
         for t in (dq, dk, dv):
             t.zero_()
         return views
-    q, k, v, d_o = _attend4(q), _attend4(k), _attend4(v), _attend4(d_o)
+    q, k, v, d_o = _attend4(q, h // hk), _attend4(k), _attend4(v), _attend4(d_o, h // hk)
     D = _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask)
     dvec = torch.empty_like(lse)
     D.d_o, D.g_strides, D.dq, D.dk, D.dv, D.dvec = ptr(d_o), _strides3(d_o), ptr(dq), ptr(dk), ptr(dv), ptr(dvec)
