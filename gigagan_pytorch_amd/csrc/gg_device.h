@@ -19,6 +19,7 @@
 #define GG_DEVICE __device__ __forceinline__
 #define GG_HOST_DEVICE __host__ __device__ __forceinline__
 #define GG_KERNEL __global__
+#define GG_NOINLINE __device__ __attribute__((noinline))      // a rare path whose registers must not weigh on the kernel that calls it
 #define GG_SHARED __shared__
 #define GG_LAUNCH_BOUNDS(n) __launch_bounds__(n)
 #define GG_LAUNCH_BOUNDS2(n, waves_per_simd) __launch_bounds__(n, waves_per_simd)   // caps the register allocation for that occupancy
@@ -180,6 +181,11 @@ GG_DEVICE void gg_bufs_load_lds16(GgBufS r, unsigned voff, unsigned soff, void* 
 // hand-over of LDS data between the lanes of ONE wave (a wave-private staging area): the hardware executes a wave's LDS instructions
 // in order, so nothing is emitted - the builtin only pins the compiler's schedule; the emulator, whose lanes are independent fibers,
 // makes it a wave rendezvous
+// nothing is scheduled across this point: a software pipeline written out in the source keeps its order (left to itself the compiler
+// sinks every LDS read to its use to save registers, and each use then waits for the LDS)
+// a value the compiler must take as new here (it cannot hoist what is computed from it above this point)
+GG_DEVICE void gg_opaque(unsigned& v) { asm volatile("" : "+v"(v)); }
+GG_DEVICE void gg_sched_fence() { __builtin_amdgcn_sched_barrier(0); }
 GG_DEVICE void gg_wave_sync() { __builtin_amdgcn_wave_barrier(); }
 // a 16-byte store marked non-temporal (global_store_dwordx4 ... nt): a streamed output row does not displace the operand tiles that the
 // same workgroups keep re-reading from this XCD's L2 (gg_pgemm.h)

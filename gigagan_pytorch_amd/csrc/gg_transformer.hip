@@ -127,8 +127,7 @@ extern "C" int gg_rotary(const gg_rotary_desc* d, void* stream) {
 // what a call launches: a function of the sizes alone, so that the workspace query and the call agree
 struct GgWinPlan {
     bool few;                   // rows fit one 32-row tile: gg_win_few_kernel
-    int waves;                  // else: waves of 32 rows a workgroup
-    int row_tiles, splits;      // forward
+    int row_tiles, splits, join;        // forward
     int key_tiles, sink_tiles, sink_chunks;     // dk / dv
     size_t fwd_bytes, bwd_bytes;
 };
@@ -140,8 +139,7 @@ static GgWinPlan gg_win_plan(const gg_window_desc* d) {
     const long long g = d->h / d->hk, rows = (long long)d->n * g, heads = (long long)d->B * d->hk;
     const long long left = gg_win_bound(d->left), right = gg_win_bound(d->right), sinks = d->sinks < d->m ? d->sinks : d->m;
     w.few = rows <= 32;
-    w.waves = d->d == 128 && heads * ((rows + 255) / 256) >= 256 ? 8 : 4;
-    const int tr = w.few ? 32 : 32 * w.waves, tk = w.few ? 32 : 64;
+    const int tr = w.few ? 32 : 128, tk = w.few ? 32 : 64;
     w.row_tiles = (int)((rows + tr - 1) / tr);
     // keys that one row tile visits at most, in tiles
     long long span = left + right + (rows < tr ? rows : tr) / g + 1 + sinks;
@@ -152,7 +150,10 @@ static GgWinPlan gg_win_plan(const gg_window_desc* d) {
     long long s = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks;
     if (s > tiles / least) s = tiles / least;
     if (s > 64) s = 64;
-    w.splits = (int)(s < 1 || w.waves == 8 ? 1 : s);
+    w.splits = (int)(s < 1 ? 1 : s);
+    // thread groups a row in the join: each takes four splits or so
+    w.join = 1;
+    while (w.join * 4 < w.splits && w.join < 1024 / d->d) w.join *= 2;
     w.fwd_bytes = w.splits > 1 ? (size_t)w.splits * heads * rows * (d->d + 2) * sizeof(float) : 0;
     w.key_tiles = (d->m + 127) / 128;
     w.sink_tiles = (int)((sinks + 127) / 128);
@@ -194,10 +195,10 @@ static int gg_win_check(const char* who, const gg_window_desc* d, GgWinParams& p
     p.d_o = (const unsigned short*)d->d_o;
     p.o = (unsigned short*)d->o; p.dq = (unsigned short*)d->dq; p.dk = (unsigned short*)d->dk; p.dv = (unsigned short*)d->dv;
     p.lse = d->lse; p.dvec = d->dvec;
-    p.qb = d->q_strides[0]; p.qh = d->q_strides[1]; p.qn = d->q_strides[2];
-    p.kb = d->k_strides[0]; p.kh = d->k_strides[1]; p.kn = d->k_strides[2];
-    p.vb = d->v_strides[0]; p.vh = d->v_strides[1]; p.vn = d->v_strides[2];
-    p.gb = d->g_strides[0]; p.gh = d->g_strides[1]; p.gn = d->g_strides[2];
+    p.qb = d->q_strides[0]; p.qh = d->q_strides[1]; p.qn = (unsigned)d->q_strides[2];
+    p.kb = d->k_strides[0]; p.kh = d->k_strides[1]; p.kn = (unsigned)d->k_strides[2];
+    p.vb = d->v_strides[0]; p.vh = d->v_strides[1]; p.vn = (unsigned)d->v_strides[2];
+    p.gb = d->g_strides[0]; p.gh = d->g_strides[1]; p.gn = (unsigned)d->g_strides[2];
     p.lengths = d->lengths; p.keep = (const unsigned char*)d->key_mask; p.keep_b = d->mask_stride;
     p.B = d->B; p.n = d->n; p.m = d->m; p.h = d->h; p.hk = d->hk; p.g = (int)g;
     p.left = gg_win_bound(d->left); p.right = gg_win_bound(d->right); p.sinks = d->sinks < d->m ? d->sinks : d->m;
@@ -225,23 +226,22 @@ extern "C" int gg_window_fwd(const gg_window_desc* d, void* workspace, size_t wo
     const GgWinPlan w = gg_win_plan(d);
     if (w.fwd_bytes && (!workspace || workspace_bytes < w.fwd_bytes || ((unsigned long long)workspace & 15)))
         return gg_fail(-5, "gg_window_fwd: needs %zu workspace bytes, 16-byte aligned", w.fwd_bytes);
-    p.splits = w.splits; p.row_tiles = w.row_tiles;
+    p.splits = w.splits; p.join = w.join; p.row_tiles = w.row_tiles;
     const long long all = (long long)p.B * p.hk * p.n * p.g;
     if (w.splits > 1) {
         p.part_o = (float*)workspace;
         p.part_ml = p.part_o + (long long)w.splits * all * d->d;
     }
     const long long grid = (long long)p.B * p.hk * w.row_tiles * w.splits;
-    if (grid > 0x7fffffffll || all * (d->d / 4) / 256 >= 0x7fffffffll) return gg_fail(-2, "gg_window_fwd: too many rows");
+    if (grid > 0x7fffffffll || all * w.join / (1024 / d->d) >= 0x7fffffffll) return gg_fail(-2, "gg_window_fwd: too many rows");
     hipStream_t s = (hipStream_t)stream;
 #define GG_WIN_GO(T, D)                                                                                                       \
     if (w.few) GG_LAUNCH((gg_win_few_kernel<T, D>), dim3((unsigned)grid), dim3(256), s, p);                                     \
-    else if (w.splits > 1) GG_LAUNCH((gg_win_fwd_kernel<T, D, 4, true>), dim3((unsigned)grid), dim3(256), s, p);                \
-    else if (w.waves == 8) GG_LAUNCH((gg_win_fwd_kernel<T, D, 8, false>), dim3((unsigned)grid), dim3(512), s, p);               \
-    else GG_LAUNCH((gg_win_fwd_kernel<T, D, 4, false>), dim3((unsigned)grid), dim3(256), s, p);                                 \
+    else if (w.splits > 1) GG_LAUNCH((gg_win_fwd_kernel<T, D, true>), dim3((unsigned)grid), dim3(256), s, p);                   \
+    else GG_LAUNCH((gg_win_fwd_kernel<T, D, false>), dim3((unsigned)grid), dim3(256), s, p);                                    \
     rc = gg_check_launch();                                                                                                   \
     if (rc || w.splits == 1) return rc;                                                                                       \
-    GG_LAUNCH((gg_win_join_kernel<T, D>), dim3((unsigned)((all * (D / 4) + 255) / 256)), dim3(256), s, p);
+    GG_LAUNCH((gg_win_join_kernel<T, D>), dim3((unsigned)((all * w.join + 1024 / D - 1) / (1024 / D))), dim3(256), s, p);
     GG_WIN_SHAPES(GG_WIN_GO)
 #undef GG_WIN_GO
     return gg_check_launch();
@@ -256,15 +256,14 @@ extern "C" int gg_window_bwd(const gg_window_desc* d, void* workspace, size_t wo
     if (w.bwd_bytes && (!workspace || workspace_bytes < w.bwd_bytes || ((unsigned long long)workspace & 15)))
         return gg_fail(-5, "gg_window_bwd: needs %zu workspace bytes, 16-byte aligned", w.bwd_bytes);
     const long long rows = (long long)p.n * p.g, heads = (long long)p.B * p.hk;
-    const long long dq_tiles = (rows + 32 * w.waves - 1) / (32 * w.waves), dq_grid = heads * dq_tiles;
+    const long long dq_tiles = (rows + 127) / 128, dq_grid = heads * dq_tiles;
     const long long kv_grid = heads * ((long long)w.sink_tiles * w.sink_chunks + w.key_tiles - w.sink_tiles);
     if (dq_grid > 0x7fffffffll || kv_grid > 0x7fffffffll) return gg_fail(-2, "gg_window_bwd: too many rows");
     hipStream_t s = (hipStream_t)stream;
     p.part_o = (float*)workspace;
 #define GG_WIN_GO(T, D)                                                                                                       \
     p.row_tiles = (int)dq_tiles;                                                                                              \
-    if (w.waves == 8) GG_LAUNCH((gg_win_dq_kernel<T, D, 8>), dim3((unsigned)dq_grid), dim3(512), s, p);                         \
-    else GG_LAUNCH((gg_win_dq_kernel<T, D, 4>), dim3((unsigned)dq_grid), dim3(256), s, p);                                      \
+    GG_LAUNCH((gg_win_dq_kernel<T, D>), dim3((unsigned)dq_grid), dim3(256), s, p);                                              \
     rc = gg_check_launch();                                                                                                   \
     if (rc) return rc;                                                                                                        \
     p.row_tiles = w.key_tiles; p.sink_tiles = w.sink_tiles; p.sink_chunks = w.sink_chunks;                                    \

@@ -16,9 +16,9 @@
 // Key tiles outside the window are not visited; the tiles a wave sees entirely take no mask arithmetic.
 //
 // NaN and infinities. Where a row does not see a key its probability is an exact zero, but zero times a NaN in the shared tile is NaN.
-// Keys behind the sequence's end are staged as zeros. For the rest every kernel looks at its own result once, at the end: if something in
-// it is not finite, the tiles are walked a second time with every non-finite vector taken out of the tile and accounted for by itself,
-// key by key, for the rows that see it. Finite inputs never take the second walk.
+// Keys behind the sequence's end are staged as zeros. For the rest every wave looks at its own result once, at the end: rows (dk / dv:
+// keys) whose result is not finite are computed again one by one, from memory and from what they see alone (ggw_fix_*). Finite inputs
+// never come there.
 #pragma once
 #include "gg_element.h"
 
@@ -32,7 +32,8 @@ struct GgWinParams {
     unsigned short *o, *dq, *dk, *dv;       // dense: o, dq [B][n][h][D]; dk, dv [B][m][hk][D]
     float* lse;                             // [B*hk][n*g]: log2 of the row's sum of 2^(scale log2e s); +inf for a row that sees nothing
     float* dvec;                            // [B*hk][n*g]: D_i
-    long long qb, qh, qn, kb, kh, kn, vb, vh, vn, gb, gh, gn;      // element strides of q, k, v, dO
+    long long qb, qh, kb, kh, vb, vh, gb, gh;       // element strides of q, k, v, dO: batch, head ...
+    unsigned qn, kn, vn, gn;                        // ... and token (below 2^24)
     const int* lengths;                     // [B] or null (= m)
     const unsigned char* keep;              // [B][m], batch stride keep_b, or null
     long long keep_b;
@@ -41,7 +42,7 @@ struct GgWinParams {
     int B, n, m, h, hk, g;
     int left, right, sinks;
     float scale;
-    int splits;
+    int splits, join;                       // ... and the thread groups that join a row's splits
     int row_tiles;                          // row (dk / dv: key) tiles per (batch, key head)
     int sink_tiles, sink_chunks;            // dk / dv: key tiles that hold sinks, and the row chunks each of them is split into
 };
@@ -62,23 +63,16 @@ GG_DEVICE u16x8 ggw_pack8(const f32x16& v, int c) {
     for (int e = 0; e < 8; ++e) f[e] = gg_elt<T>(v[8 * c + e]);
     return f;
 }
-// eight 16-bit values of which one is NaN or infinite
-template <int T>
-GG_DEVICE bool ggw_bad8(u16x8 x) {
-    constexpr unsigned short E = T == GG_ELT_BF16 ? 0x7f80 : 0x7c00;
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) bad = bad || (x[e] & E) == E;
-    return bad;
-}
+// which of the wave's 32 rows (columns of the transposed results) hold something that is not finite, as bits
 template <int N>
-GG_DEVICE bool ggw_not_finite(const f32x16* v) {
+GG_DEVICE unsigned ggw_not_finite(const f32x16* v) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s = gg_fmaf(v[i][r], 0.f, s);
-    return s != s;
+    s = gg_sum_xor32(s);
+    return (unsigned)gg_ballot(s != s);
 }
 // A tile is 64 rows of D features as the LDS-DMA deposits them: wave instruction after wave instruction of 64 x 16 bytes, rows back to
 // back. No padding is possible, so the 16-byte vectors of a row are permuted instead: vector c lies at position c ^ ggw_swz(row) (the
@@ -95,22 +89,51 @@ GG_DEVICE int ggw_swz(int row) {
     else return ((row & 3) << 2) | q;
 }
 
-// A operand, rows as they lie: lane l -> row row0 + (l & 31), features kk*16 + 8(l >> 5) + 0..7
+// This lane's offsets inside a tile, for the two kinds of reads. The vector's index (features 16 kk.., d0..) enters by exclusive or, one
+// instruction at the read: kept opaque per tile, or the compiler hoists two dozen addresses out of the loop and runs out of registers.
+struct GgwLane { unsigned rows, cols; };
 template <int D>
-GG_DEVICE u16x8 ggw_frag(const char* tile, int row0, int kk, int lane) {
-    const int row = lane & 31;                              // (row0 is a multiple of 32: it does not change the permutation)
-    return *(const u16x8*)(tile + row0 * D * 2 + ((row * D * 2 + (((lane >> 5) ^ ggw_swz<D>(row)) << 4)) ^ (kk << 5)));
+GG_DEVICE GgwLane ggw_lane() {
+    const int lane = threadIdx.x & 63, row = lane & 31;
+    const int i = lane & 15, gq = lane >> 4, trow = 4 * (gq >> 1) + (i >> 2), c = 2 * (gq & 1) + ((i & 3) >> 1);
+    GgwLane o = {(unsigned)(row * D * 2 + (((lane >> 5) ^ ggw_swz<D>(row)) << 4)), (unsigned)(trow * D * 2 + ((c ^ ggw_swz<D>(trow)) << 4) + 8 * (i & 1))};
+    return o;
 }
-// A operand of the tile's transpose: lane l -> feature d0 + (l & 31), slots (hi, e) <-> rows rb + 4hi + (e & 3) + 8(e >> 2)
+GG_DEVICE GgwLane ggw_here(GgwLane o) {
+    gg_opaque(o.rows);
+    gg_opaque(o.cols);
+    return o;
+}
+// A operand, rows as they lie: lane l -> row row0 + (l & 31), features kk*16 + 8(l >> 5) + 0..7 (row0 a multiple of 32)
 template <int D>
-GG_DEVICE u16x8 ggw_frag_tr(const char* tile, int d0, int rb, int lane) {
-    const int i = lane & 15, gq = lane >> 4;
-    const int row = 4 * (gq >> 1) + (i >> 2), c = 2 * (gq & 1) + ((i & 3) >> 1);
-    // (rb is a multiple of 16 and does not change the permutation; eight rows further on it differs by 2)
-    const int at = (row * D * 2 + ((c ^ ggw_swz<D>(row)) << 4) + 8 * (i & 1)) ^ (d0 << 1);
+GG_DEVICE u16x8 ggw_frag(const char* tile, int row0, int kk, const GgwLane& o) {
+    return *(const u16x8*)(tile + row0 * D * 2 + (o.rows ^ (unsigned)(kk << 5)));
+}
+// A operand of the tile's transpose: lane l -> feature d0 + (l & 31), slots (hi, e) <-> rows rb + 4hi + (e & 3) + 8(e >> 2) (rb a multiple
+// of 16; eight rows further on the permutation differs by 2)
+template <int D>
+GG_DEVICE u16x8 ggw_frag_tr(const char* tile, int d0, int rb, const GgwLane& o) {
+    const unsigned at = o.cols ^ (unsigned)(d0 << 1);
     const u16x4 a = gg_lds_read_tr16((const bf16_t*)(tile + rb * D * 2 + at));
     const u16x4 b = gg_lds_read_tr16((const bf16_t*)(tile + (rb + 8) * D * 2 + (at ^ 32)));
     return u16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// N products whose A operands come from the LDS, GGW_AHEAD operands read ahead of their use and the order kept
+#define GGW_AHEAD 4
+template <int N, class Read, class Use>
+GG_DEVICE void ggw_pipe(Read read, Use use) {
+    constexpr int A = GGW_AHEAD < N ? GGW_AHEAD : N;
+    u16x8 f[A];
+#pragma unroll
+    for (int s = 0; s < A; ++s) f[s] = read(s);
+    gg_sched_fence();
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+        use(s, f[s % A]);
+        if (s + A < N) f[s % A] = read(s + A);
+        gg_sched_fence();
+    }
 }
 
 // consecutive items (tiles of one (batch, key head), which share keys) go to one XCD and its L2: the dispatcher deals workgroups out to
@@ -151,74 +174,22 @@ GG_DEVICE int ggw_tile_at(const GgwRange& r, int i) { return i < r.st ? i : r.w0
 // a key that some row of the range sees (key mask apart)
 GG_DEVICE bool ggw_in_range(const GgwRange& r, int sinks, int j) { return j <= r.khi && (j >= r.klo || j < sinks); }
 
-// One 64-row tile from memory to LDS by DMA: NW waves, D / (8 NW) instructions each. `base` points at the tile's first row, `rows` of it
-// exist (the rest is deposited as zeros by the buffer's bounds check). voff[] = ggw_dma_offsets.
-template <int D, int NW> struct GgwDma { static constexpr int N = D / (8 * NW) < 1 ? 1 : D / (8 * NW); };
-template <int D, int NW>
-GG_DEVICE void ggw_dma_offsets(unsigned* voff, long long stride) {
+// Keys j0 .. j0 + 63 from memory to LDS by DMA: four waves, D / 32 instructions each. Rows from `len` on are deposited as zeros by the
+// buffer's bounds check. voff[] = ggw_dma_offsets.
+template <int D>
+GG_DEVICE void ggw_dma_offsets(unsigned* voff, unsigned stride) {
 #pragma unroll
-    for (int i = 0; i < GgwDma<D, NW>::N; ++i) {
-        const int v = threadIdx.x + 64 * NW * i, row = v / (D / 8), c = v % (D / 8);
-        voff[i] = (unsigned)(row * stride * 2) + ((c ^ ggw_swz<D>(row)) << 4);
-    }
-}
-template <int D, int NW>
-GG_DEVICE void ggw_dma(const unsigned short* base, int rows, long long stride, const unsigned* voff, char* tile, int wave) {
-    if (GgwDma<D, NW>::N * 8 * NW > D && wave >= D / 8) return;             // (D 32, eight waves: four of them have nothing to fetch)
-    const unsigned long long bytes = rows <= 0 ? 0 : ((unsigned long long)(rows < 64 ? rows - 1 : 63) * stride + D) * 2;
-    const GgBufS buf = gg_make_bufs(base, bytes);
-#pragma unroll
-    for (int i = 0; i < GgwDma<D, NW>::N; ++i) gg_bufs_load_lds16(buf, voff[i], 0, tile + (wave + NW * i) * 1024);
-}
-
-// The second walk's tile, through registers: rows that `want` names, the others zeros; vectors with a NaN or an infinity are taken out
-// and marked, bad[row][vector] (add: on top of what is marked there; bad null: all stay).
-template <int T, int D, int NW, class Row>
-GG_DEVICE void ggw_stage_clean(char* tile, unsigned char* bad, bool add, Row row_at) {
-    for (int v = threadIdx.x; v < 64 * (D / 8); v += 64 * NW) {
-        const int row = v / (D / 8), c = v % (D / 8);
-        const unsigned short* src = row_at(row);            // null: nobody sees it
-        u16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (src) x = *(const u16x8*)(src + c * 8);
-        if (bad) {
-            const bool b = ggw_bad8<T>(x);
-            if (b) x = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-            bad[v] = (unsigned char)((add ? bad[v] : 0) | b);
-        }
-        *(u16x8*)(tile + row * D * 2 + ((c ^ ggw_swz<D>(row)) << 4)) = x;
+    for (int i = 0; i < D / 32; ++i) {
+        const int v = threadIdx.x + 256 * i, row = v / (D / 8), c = v % (D / 8);
+        voff[i] = row * stride * 2 + ((c ^ ggw_swz<D>(row)) << 4);
     }
 }
 template <int D>
-GG_DEVICE bool ggw_any_bad(const unsigned char* bad, int row) {
-    unsigned any = 0;
+GG_DEVICE void ggw_dma(const unsigned short* base, int j0, int len, unsigned stride, const unsigned* voff, char* tile, int wave) {
+    const int last = len - 1 - j0 < 63 ? len - 1 - j0 : 63;                 // the tile's last row that exists
+    const GgBufS buf = gg_make_bufs(base + (unsigned long long)(unsigned)j0 * stride, last < 0 ? 0u : (last * stride + D) * 2);
 #pragma unroll
-    for (int c = 0; c < D / 8; c += 4) any |= *(const unsigned*)(bad + row * (D / 8) + c);
-    return any != 0;
-}
-// forward: what the vectors that were taken out of a key tile give the rows that see their keys. K and V are read where they lie.
-template <int T, int D, class See>
-GG_DEVICE void ggw_add_bad(f32x16* ot, const unsigned char* bad, int tk, int j0, const unsigned short* kb, long long kn, const unsigned short* vb,
-                           long long vn, const u16x8* qf, float a2, float m, int hi, See see) {
-    for (int jr = 0; jr < tk; ++jr) {
-        if (!ggw_any_bad<D>(bad, jr)) continue;             // (workgroup- or wave-uniform; a marked key lies inside the range)
-        const int j = j0 + jr;
-        float s = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            const u16x8 kv = *(const u16x8*)(kb + (long long)j * kn + kk * 16 + 8 * hi);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s = gg_fmaf(gg_elt_f<T>(qf[kk][e]), gg_elt_f<T>(kv[e]), s);
-        }
-        s = gg_sum_xor32(s);
-        const float pj = see(j) ? gg_exp2f(gg_fmaf(s, a2, -m)) : 0.f;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c)
-            if (bad[jr * (D / 8) + c]) {
-                const u16x4 v4 = *(const u16x4*)(vb + (long long)j * vn + c * 8 + 4 * hi);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) ot[c / 4][4 * (c % 4) + e] += pj > 0.f ? pj * gg_elt_f<T>(v4[e]) : 0.f;
-            }
-    }
+    for (int i = 0; i < D / 32; ++i) gg_bufs_load_lds16(buf, voff[i], 0, tile + (wave + 4 * i) * 1024);
 }
 
 // this lane's row of the tile that starts at row r0, and the wave's 32 rows
@@ -269,140 +240,59 @@ GG_DEVICE bool ggw_whole(const GgwWave& w, int sinks, int j0, int j1) { return j
 GG_DEVICE bool ggw_sees(const GgwWave& w, int sinks, int j) { return j <= w.hi && (j >= w.lo || j < sinks); }
 
 // ---- forward -------------------------------------------------------------------------------------------------------
-// workgroup: NW waves x 32 rows, key tiles of 64 fetched once for all of them by LDS-DMA, double buffered: one barrier a tile, behind
-// which the next tile's transfers start and run under this tile's arithmetic.
-// SPLIT: the tiles are dealt out to p.splits workgroups, which leave (m, l, O) for gg_win_join_kernel.
-template <int T, int D, int NW, bool SPLIT>
-GG_KERNEL GG_LAUNCH_BOUNDS2(64 * NW, 2) void gg_win_fwd_kernel(GgWinParams p) {
-    constexpr int KK = D / 16, DB = D / 32;
-    GG_SHARED __attribute__((aligned(1024))) char sK[2][GgwTile<D>::BYTES];
-    GG_SHARED __attribute__((aligned(1024))) char sV[2][GgwTile<D>::BYTES];
-    GG_SHARED __attribute__((aligned(16))) unsigned char sBad[64 * (D / 8)];
-    GG_SHARED int sAgain;
 
-    const int lane = threadIdx.x & 63, wave = gg_uniform(threadIdx.x >> 6), hi = lane >> 5;
-    int item = ggw_item();
-    int split = 0;
-    if (SPLIT) { split = item % p.splits; item /= p.splits; }
-    const int bkv = item / p.row_tiles, tile = item - bkv * p.row_tiles;
-    const int b = bkv / p.hk, kvh = bkv - b * p.hk;
-    const int rows = p.n * p.g;
-    const int len = ggw_len(p, b);
-    const int r0 = tile * (32 * NW), rl = r0 + 32 * NW - 1 < rows - 1 ? r0 + 32 * NW - 1 : rows - 1;
-    const GgwRange rg = ggw_range<64>(p, len, r0 / p.g, rl / p.g);
-    const int ta = SPLIT ? (int)((long long)rg.nt * split / p.splits) : 0, tb = SPLIT ? (int)((long long)rg.nt * (split + 1) / p.splits) : rg.nt;
-
-    const unsigned char* keep = p.keep ? p.keep + b * p.keep_b : nullptr;
-    const GgwWave w = ggw_wave(p, r0 + wave * 32, len, keep != nullptr);
-    const unsigned short* kb = p.k + b * p.kb + kvh * p.kh;
-    const unsigned short* vb = p.v + b * p.vb + kvh * p.vh;
-    u16x8 qf[KK];
-    {
-        const unsigned short* qr = p.q + b * p.qb + (long long)(kvh * p.g + w.row.head) * p.qh + (long long)w.row.token * p.qn + 8 * hi;
+// scores that their row does not see become -inf; keep: this item's key mask or null
+GG_DEVICE void ggw_mask(f32x16* st, int blocks, const GgwWave& w, int sinks, int j0, int len, const unsigned char* keep) {
+    const int lane = threadIdx.x & 63, hi = lane >> 5;
+    unsigned long long bits = ~0ull;
+    if (keep) bits = gg_ballot(j0 + lane < len && keep[j0 + lane]);
+    bits >>= 4 * hi;
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) qf[kk] = *(const u16x8*)(qr + kk * 16);
-    }
-    unsigned ko[GgwDma<D, NW>::N], vo[GgwDma<D, NW>::N];
-    ggw_dma_offsets<D, NW>(ko, p.kn);
-    ggw_dma_offsets<D, NW>(vo, p.vn);
-    auto fetch = [&](int i, int buf) {
-        const int j0 = ggw_tile_at(rg, i) * 64;
-        ggw_dma<D, NW>(kb + (long long)j0 * p.kn, len - j0, p.kn, ko, sK[buf], wave);
-        ggw_dma<D, NW>(vb + (long long)j0 * p.vn, len - j0, p.vn, vo, sV[buf], wave);
-    };
-    const float a2 = p.scale * GGW_LOG2E;
-    float m, l;
-    f32x16 ot[DB];
-    bool again = false;             // the second walk (workgroup-uniform)
-walk:
-    m = -1.0e30f;
-    l = 0.f;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) ot[db][r] = 0.f;
-    if (threadIdx.x == 0) sAgain = 0;
-    if (!again && ta < tb) fetch(ta, 0);
-    for (int i = ta, buf = 0; i < tb; ++i, buf ^= 1) {
-        const int j0 = ggw_tile_at(rg, i) * 64;
-        if (!again) {
-            gg_wait_vm<0>();
-            gg_barrier_lds();       // this tile is there for everyone, and everyone is through with the last one: its buffer is free
-            if (i + 1 < tb) fetch(i + 1, buf ^ 1);
-        } else {
-            gg_sync();
-            auto in = [&](int j) { return ggw_in_range(rg, p.sinks, j) && (!keep || keep[j]); };
-            ggw_stage_clean<T, D, NW>(sK[buf], nullptr, false, [&](int row) { return in(j0 + row) ? kb + (long long)(j0 + row) * p.kn : nullptr; });
-            ggw_stage_clean<T, D, NW>(sV[buf], sBad, false, [&](int row) { return in(j0 + row) ? vb + (long long)(j0 + row) * p.vn : nullptr; });
-            gg_sync();
-        }
-        if (!ggw_some(w, p.sinks, j0, j0 + 63)) continue;
-        f32x16 st[2];
-#pragma unroll
-        for (int jb = 0; jb < 2; ++jb) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) st[jb][r] = 0.f;
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk) st[jb] = ggw_mfma<T>(ggw_frag<D>(sK[buf], jb * 32, kk, lane), qf[kk], st[jb]);
-        }
-        if (!ggw_whole(w, p.sinks, j0, j0 + 63)) {
-            unsigned long long bits = ~0ull;
-            if (keep) bits = gg_ballot(j0 + lane < len && keep[j0 + lane]);
-            bits >>= 4 * hi;
-#pragma unroll
-            for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int jr = jb * 32 + (r & 3) + 8 * (r >> 2);
-                    const bool see = ggw_sees(w, p.sinks, j0 + jr + 4 * hi) && ((bits >> jr) & 1);
-                    st[jb][r] = see ? st[jb][r] : -__builtin_inff();
-                }
-        }
-        float mx = -__builtin_inff();
-#pragma unroll
-        for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[jb][r]);
-        mx = gg_max_xor32(mx) * a2;
-        if (gg_wave_any(mx > m + GGW_TAU)) {
-            const float mn = fmaxf(m, mx), corr = gg_exp2f(m - mn);
-            l *= corr;
-            m = mn;
-#pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) ot[db][r] *= corr;
-        }
-        float sum = 0.f;
-#pragma unroll
-        for (int jb = 0; jb < 2; ++jb)
+    for (int jb = 0; jb < 2; ++jb)
+        if (jb < blocks) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                st[jb][r] = gg_exp2f(gg_fmaf(st[jb][r], a2, -m));
-                sum += st[jb][r];
+                const int jr = jb * 32 + (r & 3) + 8 * (r >> 2);
+                const bool see = ggw_sees(w, sinks, j0 + jr + 4 * hi) && ((bits >> jr) & 1);
+                st[jb][r] = see ? st[jb][r] : -__builtin_inff();
             }
-        l += sum;
-#pragma unroll
-        for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const u16x8 pf = ggw_pack8<T>(st[jb], c);
-#pragma unroll
-                for (int db = 0; db < DB; ++db) ot[db] = ggw_mfma<T>(ggw_frag_tr<D>(sV[buf], db * 32, jb * 32 + 16 * c, lane), pf, ot[db]);
-            }
-        if (again)
-            ggw_add_bad<T, D>(ot, sBad, 64, j0, kb, p.kn, vb, p.vn, qf, a2, m, hi, [&](int j) { return ggw_sees(w, p.sinks, j) && (!keep || keep[j]); });
-    }
-    if (!again) {
-        gg_sync();
-        if (ggw_not_finite<DB>(ot)) sAgain = 1;
-        gg_sync();
-        if (sAgain) {
-            again = true;
-            gg_sync();
-            goto walk;
         }
+}
+// one softmax step over N 32-key blocks of scores: running maximum m (log2 domain), this lane's part of the row's sum l, the probabilities
+// packed as the next product's operands. The maximum moves (and O with it) only when a score exceeds it by 2^GGW_TAU.
+template <int T, int DB, int N>
+GG_DEVICE void ggw_softmax(f32x16* st, u16x8* pf, f32x16* ot, float& m, float& l, float a2) {
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int jb = 0; jb < N; ++jb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[jb][r]);
+    mx = gg_max_xor32(mx) * a2;
+    if (gg_wave_any(mx > m + GGW_TAU)) {
+        const float mn = fmaxf(m, mx), corr = gg_exp2f(m - mn);
+        l *= corr;
+        m = mn;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ot[db][r] *= corr;
     }
+    float sum = 0.f;
+#pragma unroll
+    for (int jb = 0; jb < N; ++jb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            st[jb][r] = gg_exp2f(gg_fmaf(st[jb][r], a2, -m));
+            sum += st[jb][r];
+        }
+    l += sum;
+#pragma unroll
+    for (int jc = 0; jc < 2 * N; ++jc) pf[jc] = ggw_pack8<T>(st[jc >> 1], jc & 1);
+}
+// the wave's 32 rows: o and the log-sum-exp, or (SPLIT) what gg_win_join_kernel takes
+template <int T, int D, bool SPLIT>
+GG_DEVICE void ggw_write_rows(const GgWinParams& p, const GgwWave& w, int bkv, int split, const f32x16* ot, float m, float l) {
+    const int hi = (threadIdx.x & 63) >> 5, rows = p.n * p.g;
     l = gg_sum_xor32(l);
     if (w.r >= rows) return;
     const long long at = (long long)bkv * rows + w.r;
@@ -410,17 +300,18 @@ walk:
         const long long sp = (long long)split * p.B * p.hk * rows + at;
         float* po = p.part_o + sp * D;
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
+        for (int db = 0; db < D / 32; ++db)
 #pragma unroll
             for (int gq = 0; gq < 4; ++gq)
                 *(f32x4*)(po + db * 32 + 8 * gq + 4 * hi) = f32x4{ot[db][4 * gq], ot[db][4 * gq + 1], ot[db][4 * gq + 2], ot[db][4 * gq + 3]};
         if (hi == 0) { p.part_ml[2 * sp] = m; p.part_ml[2 * sp + 1] = l; }
         return;
     }
+    const int b = bkv / p.hk, kvh = bkv - b * p.hk;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     unsigned short* orow = p.o + (((long long)b * p.n + w.row.token) * p.h + kvh * p.g + w.row.head) * D;
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < D / 32; ++db)
 #pragma unroll
         for (int gq = 0; gq < 4; ++gq) {
             u16x4 o4;
@@ -430,6 +321,155 @@ walk:
         }
     if (hi == 0 && p.lse) p.lse[at] = l == 0.f ? __builtin_inff() : m + log2f(l);
 }
+template <int KK>
+GG_DEVICE void ggw_load_row(u16x8* f, const unsigned short* base, long long head_stride, unsigned token_stride, int head, int token) {
+    const unsigned short* r = base + (long long)head * head_stride + (long long)token * token_stride + 8 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) f[kk] = *(const u16x8*)(r + kk * 16);
+}
+
+template <int T, int D>
+GG_DEVICE float ggw_dot(const unsigned short* x, const unsigned short* y) {
+    float s = 0.f;
+    for (int c = 0; c < D; c += 8) {
+        const u16x8 a = *(const u16x8*)(x + c), b = *(const u16x8*)(y + c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = gg_fmaf(gg_elt_f<T>(a[e]), gg_elt_f<T>(b[e]), s);
+    }
+    return s;
+}
+// One row again, by one wave, from the keys it sees alone: tiles i0, i0 + step .. of TK keys, a key a lane for the scores, a feature a lane
+// for the output. fix[D] = sum of p v, relative to the maximum m, l the sum of p.
+template <int T, int D, int TK>
+GG_DEVICE void ggw_fix_row(const GgWinParams& p, const GgwRange& rg, int len, const unsigned char* keep, const unsigned short* q,
+                           const unsigned short* kb, const unsigned short* vb, int pos, int i0, int i1, int step, float* fix, float& m, float& l) {
+    constexpr int C = (D + 63) / 64;
+    const int lane = threadIdx.x & 63;
+    const float a2 = p.scale * GGW_LOG2E;
+    float acc[C];
+    m = -1.0e30f;
+    l = 0.f;
+    for (int c = 0; c < C; ++c) acc[c] = 0.f;
+    for (int i = i0; i < i1; i += step) {
+        const int j0 = ggw_tile_at(rg, i) * TK, j = j0 + lane;
+        const bool see = lane < TK && j < len && j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && (!keep || keep[j]);
+        const float x = see ? ggw_dot<T, D>(q, kb + (long long)j * p.kn) * a2 : -__builtin_inff();
+        float mx = x;
+        for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, gg_shfl_xor(mx, o));
+        const float mn = fmaxf(m, mx), corr = gg_exp2f(m - mn), pj = see ? gg_exp2f(x - mn) : 0.f;
+        l = l * corr + gg_wave_sum_all(pj);
+        m = mn;
+        for (int c = 0; c < C; ++c) acc[c] *= corr;
+        for (int k = 0; k < TK; ++k) {
+            const float pk = gg_readlane(pj, k);
+            if (pk == 0.f) continue;
+            for (int c = 0; c < C; ++c)
+                if (lane + 64 * c < D) acc[c] += pk * gg_elt_f<T>(vb[(long long)(j0 + k) * p.vn + lane + 64 * c]);
+        }
+    }
+    for (int c = 0; c < C; ++c)
+        if (lane + 64 * c < D) fix[lane + 64 * c] = acc[c];
+}
+// its values into the registers of the lanes that own the row
+template <int DB>
+GG_DEVICE void ggw_take_fix(f32x16* v, const float* fix, bool mine) {
+    const int hi = (threadIdx.x & 63) >> 5;
+    gg_wave_sync();
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float x = fix[db * 32 + (r & 3) + 8 * (r >> 2) + 4 * hi];
+            v[db][r] = mine ? x : v[db][r];
+        }
+    gg_wave_sync();
+}
+template <int T, int D, int TK>
+GG_DEVICE void ggw_fix_rows(const GgWinParams& p, const GgwWave& w, const GgwRange& rg, int len, int b, int kvh, const unsigned char* keep, int i0,
+                            int i1, int step, unsigned bad, float* fix, f32x16* ot, float& m, float& l) {
+    const int lane = threadIdx.x & 63, rows = p.n * p.g;
+    for (int k = 0; k < 32; ++k) {
+        if (!((bad >> k) & 1) || w.r0 + k >= rows) continue;
+        const int token = (w.r0 + k) / p.g, head = w.r0 + k - token * p.g, pos = token + len - p.n;
+        float fm, fl;
+        ggw_fix_row<T, D, TK>(p, rg, len, keep, p.q + b * p.qb + (long long)(kvh * p.g + head) * p.qh + (long long)token * p.qn,
+                              p.k + b * p.kb + kvh * p.kh, p.v + b * p.vb + kvh * p.vh, pos < 0 ? -2 * GGW_NONE : pos, i0, i1, step, fix, fm, fl);
+        const bool mine = (lane & 31) == k;
+        ggw_take_fix<D / 32>(ot, fix, mine);
+        if (mine) {
+            m = fm;
+            l = lane < 32 ? fl : 0.f;
+        }
+    }
+}
+
+// workgroup: 4 waves x 32 rows; key tiles of 64 fetched once for all of them by LDS-DMA, double buffered: one barrier a tile, behind
+// which the next tile's transfers start and run under this tile's arithmetic.
+// SPLIT: the tiles are dealt out to p.splits workgroups, which leave (m, l, O) for gg_win_join_kernel.
+template <int T, int D, bool SPLIT>
+GG_KERNEL GG_LAUNCH_BOUNDS2(256, D == 128 ? 2 : 3) void gg_win_fwd_kernel(GgWinParams p) {
+    constexpr int KK = D / 16, DB = D / 32;
+    GG_SHARED __attribute__((aligned(1024))) char sK[2][GgwTile<D>::BYTES];
+    GG_SHARED __attribute__((aligned(1024))) char sV[2][GgwTile<D>::BYTES];
+    GG_SHARED float sFix[4][D];
+
+    const int lane = threadIdx.x & 63, wave = gg_uniform(threadIdx.x >> 6), hi = lane >> 5;
+    int item = ggw_item();
+    int split = 0;
+    if (SPLIT) { split = item % p.splits; item /= p.splits; }
+    const int bkv = item / p.row_tiles, tile = item - bkv * p.row_tiles;
+    const int b = bkv / p.hk, kvh = bkv - b * p.hk;
+    const int rows = p.n * p.g;
+    const int len = ggw_len(p, b);
+    const int r0 = tile * 128, rl = r0 + 127 < rows - 1 ? r0 + 127 : rows - 1;
+    const GgwRange rg = ggw_range<64>(p, len, r0 / p.g, rl / p.g);
+    const int ta = SPLIT ? (int)((long long)rg.nt * split / p.splits) : 0, tb = SPLIT ? (int)((long long)rg.nt * (split + 1) / p.splits) : rg.nt;
+
+    const unsigned char* keep = p.keep ? p.keep + b * p.keep_b : nullptr;
+    const GgwWave w = ggw_wave(p, r0 + wave * 32, len, keep != nullptr);
+    const unsigned short* kb = p.k + b * p.kb + kvh * p.kh;
+    const unsigned short* vb = p.v + b * p.vb + kvh * p.vh;
+    u16x8 qf[KK];
+    ggw_load_row<KK>(qf, p.q + b * p.qb, p.qh, p.qn, kvh * p.g + w.row.head, w.row.token);
+    unsigned ko[D / 32], vo[D / 32];
+    ggw_dma_offsets<D>(ko, p.kn);
+    ggw_dma_offsets<D>(vo, p.vn);
+    auto fetch = [&](int i, int buf) {
+        const int j0 = ggw_tile_at(rg, i) * 64;
+        ggw_dma<D>(kb, j0, len, p.kn, ko, sK[buf], wave);
+        ggw_dma<D>(vb, j0, len, p.vn, vo, sV[buf], wave);
+    };
+    const float a2 = p.scale * GGW_LOG2E;
+    float m = -1.0e30f, l = 0.f;
+    f32x16 ot[DB], st[2];
+    u16x8 pf[4];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ot[db][r] = 0.f;
+    const GgwLane lanes = ggw_lane<D>();
+    gg_wait_vm<0>();                // (the rows above: the transfers' count starts at zero)
+    if (ta < tb) fetch(ta, 0);
+    for (int i = ta, buf = 0; i < tb; ++i, buf ^= 1) {
+        const int j0 = ggw_tile_at(rg, i) * 64;
+        gg_wait_vm<0>();
+        gg_barrier_lds();           // this tile is there for everyone, and everyone is through with the last one: its buffer is free
+        if (i + 1 < tb) fetch(i + 1, buf ^ 1);
+        if (!ggw_some(w, p.sinks, j0, j0 + 63)) continue;
+        const GgwLane lo = ggw_here(lanes);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[0][r] = st[1][r] = 0.f;
+        ggw_pipe<2 * KK>([&](int s) { return ggw_frag<D>(sK[buf], (s & 1) * 32, s >> 1, lo); },
+                         [&](int s, u16x8 x) { st[s & 1] = ggw_mfma<T>(x, qf[s >> 1], st[s & 1]); });
+        if (!ggw_whole(w, p.sinks, j0, j0 + 63)) ggw_mask(st, 2, w, p.sinks, j0, len, keep);
+        ggw_softmax<T, DB, 2>(st, pf, ot, m, l, a2);
+        ggw_pipe<4 * DB>([&](int s) { return ggw_frag_tr<D>(sV[buf], (s % DB) * 32, 16 * (s / DB), lo); },
+                         [&](int s, u16x8 x) { ot[s % DB] = ggw_mfma<T>(x, pf[s / DB], ot[s % DB]); });
+    }
+    const unsigned bad = ggw_not_finite<DB>(ot);
+    if (__builtin_expect(bad != 0, 0)) ggw_fix_rows<T, D, 64>(p, w, rg, len, b, kvh, keep, ta, tb, 1, bad, sFix[wave], ot, m, l);
+    ggw_write_rows<T, D, SPLIT>(p, w, bkv, split, ot, m, l);
+}
 
 // ---- forward with few rows ------------------------------------------------------------------------------------------
 // One new token: a handful of rows against a long cache - bound by reading K and V once. The four waves share the 32 rows and take key
@@ -437,10 +477,9 @@ walk:
 // LDS tile (the transpose read), no barrier in the loop; the waves' (m, l, O) are joined in LDS at the end, the splits' by
 // gg_win_join_kernel.
 template <int T, int D>
-GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_few_kernel(GgWinParams p) {
+GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_few_kernel(GgWinParams p) {
     constexpr int KK = D / 16, DB = D / 32;
     GG_SHARED __attribute__((aligned(16))) char sV[4][32 * D * 2];
-    GG_SHARED __attribute__((aligned(16))) unsigned char sBad[4][32 * (D / 8)];
     GG_SHARED float sM[4][32], sL[4][32];
     GG_SHARED __attribute__((aligned(16))) float sO[32][D + 4];
 
@@ -455,58 +494,38 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_few_kernel(GgWinParams p) {
     const int r0 = tile * 32, rl = r0 + 31 < rows - 1 ? r0 + 31 : rows - 1;
     const GgwRange rg = ggw_range<32>(p, len, r0 / p.g, rl / p.g);
     const int ta = (int)((long long)rg.nt * split / p.splits), tb = (int)((long long)rg.nt * (split + 1) / p.splits);
-    const GgwRow row = ggw_row(p, r0 + (lane & 31), len);
-    const int lo = row.pos - p.left, hij = row.in ? (row.pos + p.right < len - 1 ? row.pos + p.right : len - 1) : -1;
+    const unsigned char* keep = p.keep ? p.keep + b * p.keep_b : nullptr;
+    const GgwWave w = ggw_wave(p, r0, len, keep != nullptr);
     const unsigned short* kb = p.k + b * p.kb + kvh * p.kh;
     const unsigned short* vb = p.v + b * p.vb + kvh * p.vh;
-    const unsigned char* keep = p.keep ? p.keep + b * p.keep_b : nullptr;
-    u16x8 qf[KK];
-    {
-        const unsigned short* qr = p.q + b * p.qb + (long long)(kvh * p.g + row.head) * p.qh + (long long)row.token * p.qn + 8 * hi;
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) qf[kk] = *(const u16x8*)(qr + kk * 16);
-    }
+    u16x8 qf[KK], pf[2];
+    ggw_load_row<KK>(qf, p.q + b * p.qb, p.qh, p.qn, kvh * p.g + w.row.head, w.row.token);
     const float a2 = p.scale * GGW_LOG2E;
-    float m, l;
+    float m = -1.0e30f, l = 0.f;
     f32x16 ot[DB];
-
-    u16x8 kf[KK], vr[D / 16];
-    bool kept = true;
-    auto load = [&](int i) {
-        const int j0 = ggw_tile_at(rg, i) * 32, j = j0 + (lane & 31);
-        const bool ok = j <= rg.khi;                                            // (0 <= khi < len: the clamped row exists)
-        const unsigned short* kr = kb + (long long)(ok ? j : rg.khi) * p.kn + 8 * hi;
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) kf[kk] = *(const u16x8*)(kr + kk * 16);
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-            const int v = lane + 64 * s, jv = j0 + v / (D / 8), c8 = v % (D / 8);
-            vr[s] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-            if (ggw_in_range(rg, p.sinks, jv) && (!keep || keep[jv])) vr[s] = *(const u16x8*)(vb + (long long)jv * p.vn + c8 * 8);
-        }
-        if (keep) kept = ok && keep[j];
-    };
-    bool again = false;             // the second walk (wave-uniform)
-walk:
-    m = -1.0e30f;
-    l = 0.f;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) ot[db][r] = 0.f;
+
+    u16x8 kf[KK], vr[D / 16];
+    auto load = [&](int i) {        // (0 <= khi < len: the clamped rows exist; what they hold meets a masked score)
+        const int j0 = ggw_tile_at(rg, i) * 32, j = j0 + (lane & 31);
+        ggw_load_row<KK>(kf, kb, 0, p.kn, 0, j <= rg.khi ? j : rg.khi);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+            const int v = lane + 64 * s, jv = j0 + v / (D / 8), c8 = v % (D / 8);
+            vr[s] = *(const u16x8*)(vb + (long long)(jv <= rg.khi ? jv : rg.khi) * p.vn + c8 * 8);
+        }
+    };
+    const GgwLane lo = ggw_lane<D>();
     if (ta + wave < tb) load(ta + wave);
     for (int i = ta + wave; i < tb; i += 4) {
         const int j0 = ggw_tile_at(rg, i) * 32;
         gg_wave_sync();
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
-            const int v = lane + 64 * s;
-            if (again) {
-                const bool bad = ggw_bad8<T>(vr[s]);
-                if (bad) vr[s] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-                sBad[wave][v] = bad;
-            }
-            const int vrow = v / (D / 8);
+            const int v = lane + 64 * s, vrow = v / (D / 8);
             *(u16x8*)(sV[wave] + vrow * D * 2 + (((v % (D / 8)) ^ ggw_swz<D>(vrow)) << 4)) = vr[s];
         }
         gg_wave_sync();
@@ -515,48 +534,18 @@ walk:
         for (int r = 0; r < 16; ++r) st[r] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) st = ggw_mfma<T>(kf[kk], qf[kk], st);
-        unsigned bits = 0xffffffffu;
-        if (keep) bits = (unsigned)gg_ballot(kept);
-        bits >>= 4 * hi;
         if (i + 4 < tb) load(i + 4);
+        if (!ggw_whole(w, p.sinks, j0, j0 + 31)) ggw_mask(&st, 1, w, p.sinks, j0, len, keep);
+        ggw_softmax<T, DB, 1>(&st, pf, ot, m, l, a2);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int jr = (r & 3) + 8 * (r >> 2), j = j0 + jr + 4 * hi;
-            const bool see = j <= hij && (j >= lo || j < p.sinks) && ((bits >> jr) & 1);
-            st[r] = see ? st[r] : -__builtin_inff();
-        }
-        float mx = -__builtin_inff();
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[r]);
-        mx = gg_max_xor32(mx) * a2;
-        if (gg_wave_any(mx > m + GGW_TAU)) {
-            const float mn = fmaxf(m, mx), corr = gg_exp2f(m - mn);
-            l *= corr;
-            m = mn;
-#pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) ot[db][r] *= corr;
-        }
-        float sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            st[r] = gg_exp2f(gg_fmaf(st[r], a2, -m));
-            sum += st[r];
-        }
-        l += sum;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const u16x8 pf = ggw_pack8<T>(st, c);
-#pragma unroll
-            for (int db = 0; db < DB; ++db) ot[db] = ggw_mfma<T>(ggw_frag_tr<D>(sV[wave], db * 32, 16 * c, lane), pf, ot[db]);
-        }
-        if (again)
-            ggw_add_bad<T, D>(ot, sBad[wave], 32, j0, kb, p.kn, vb, p.vn, qf, a2, m, hi, [&](int j) { return j <= hij && (j >= lo || j < p.sinks) && (!keep || keep[j]); });
+            for (int db = 0; db < DB; ++db) ot[db] = ggw_mfma<T>(ggw_frag_tr<D>(sV[wave], db * 32, 16 * c, lo), pf[c], ot[db]);
     }
-    if (!again && gg_wave_any(ggw_not_finite<DB>(ot))) {
-        again = true;
-        goto walk;
+    const unsigned bad = ggw_not_finite<DB>(ot);
+    if (__builtin_expect(bad != 0, 0)) {
+        gg_wave_sync();             // (the wave's own tile is free)
+        ggw_fix_rows<T, D, 32>(p, w, rg, len, b, kvh, keep, ta + wave, tb, 4, bad, (float*)sV[wave], ot, m, l);
     }
     l = gg_sum_xor32(l);
     if (hi == 0) { sM[wave][lane] = m; sL[wave][lane] = l; }
@@ -603,25 +592,42 @@ walk:
     }
 }
 
-// the splits' (m, l, O) of a row joined: four features a thread
+// The splits' (m, l, O) of a row joined: four features a thread, p.join groups of threads a row that share its splits (few rows and many
+// splits: a thread that walked them all would wait for memory a dozen times over), the groups' sums added in order in LDS.
 template <int T, int D>
 GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_join_kernel(GgWinParams p) {
-    const int rows = p.n * p.g;
+    constexpr int Q = D / 4, R = 256 / Q;                   // threads a group, groups a workgroup
+    GG_SHARED __attribute__((aligned(16))) float sO[R][D + 4];
+    GG_SHARED float sM[R], sL[R];
+    const int rows = p.n * p.g, grp = threadIdx.x / Q, d = threadIdx.x % Q * 4, share = grp % p.join;
     const long long all = (long long)p.B * p.hk * rows;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, at = i / (D / 4);
-    const int d = (int)(i % (D / 4)) * 4;
-    if (at >= all) return;
+    const long long at0 = (long long)blockIdx.x * (R / p.join) + grp / p.join, at = at0 < all ? at0 : all - 1;
     float top = -1.0e30f;
-#pragma unroll 8
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[2 * (s * all + at)]);
+#pragma unroll 4
+    for (int s = share; s < p.splits; s += p.join) top = fmaxf(top, p.part_ml[2 * (s * all + at)]);
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < p.splits; ++s) {
+#pragma unroll 4
+    for (int s = share; s < p.splits; s += p.join) {
         const float f = gg_exp2f(p.part_ml[2 * (s * all + at)] - top);
         l += f * p.part_ml[2 * (s * all + at) + 1];
         x += f * *(const f32x4*)(p.part_o + (s * all + at) * D + d);
     }
+    if (p.join > 1) {
+        *(f32x4*)&sO[grp][d] = x;
+        if (d == 0) { sM[grp] = top; sL[grp] = l; }
+        gg_sync();
+        if (share) return;
+        for (int k = 1; k < p.join; ++k) top = fmaxf(top, sM[grp + k]);
+        x = f32x4{0.f, 0.f, 0.f, 0.f};
+        l = 0.f;
+        for (int k = 0; k < p.join; ++k) {
+            const float f = gg_exp2f(sM[grp + k] - top);
+            l += f * sL[grp + k];
+            x += f * *(const f32x4*)&sO[grp + k][d];
+        }
+    }
+    if (at0 >= all) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int bkv = (int)(at / rows), r = (int)(at - (long long)bkv * rows);
     const int b = bkv / p.hk, kvh = bkv - b * p.hk, token = r / p.g, head = r - token * p.g;
@@ -634,13 +640,65 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_join_kernel(GgWinParams p) {
 
 // ---- backward, part 1: dq and D ---------------------------------------------------------------------------------------
 // the forward's mapping and transfers; K is read as rows (scores) and transposed (dq), V as rows (dP)
-template <int T, int D, int NW>
-GG_KERNEL GG_LAUNCH_BOUNDS2(64 * NW, 2) void gg_win_dq_kernel(GgWinParams p) {
+template <int T, int D>
+GG_DEVICE void ggw_write_dq(const GgWinParams& p, const GgwWave& w, int b, int hq, const f32x16* dqt) {
+    if (w.r >= p.n * p.g) return;
+    unsigned short* row = p.dq + (((long long)b * p.n + w.row.token) * p.h + hq) * D + 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int gq = 0; gq < 4; ++gq) {
+            u16x4 o4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o4[e] = gg_elt<T>(dqt[db][4 * gq + e] * p.scale);
+            *(u16x4*)(row + db * 32 + 8 * gq) = o4;
+        }
+}
+// dS of one 32-key block from its scores and dP - D, in the scores' place
+GG_DEVICE void ggw_ds(f32x16& st, const f32x16& dp, float a2, float lse, bool masked, const GgwWave& w, int sinks, int j, unsigned long long bits) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st[r] = gg_exp2f(gg_fmaf(st[r], a2, -lse)) * dp[r];
+    if (masked) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int jr = (r & 3) + 8 * (r >> 2);
+            st[r] = ggw_sees(w, sinks, j + jr) && ((bits >> jr) & 1) ? st[r] : 0.f;
+        }
+    }
+}
+
+// one row's dq again, by one wave, from the keys it sees alone: fix[D] = sum of dS k
+template <int T, int D>
+GG_DEVICE void ggw_fix_dq(const GgWinParams& p, const GgwRange& rg, int len, const unsigned char* keep, const unsigned short* q,
+                          const unsigned short* g, const unsigned short* kb, const unsigned short* vb, int pos, float lse, float dsum, float* fix) {
+    constexpr int C = (D + 63) / 64;
+    const int lane = threadIdx.x & 63;
+    const float a2 = p.scale * GGW_LOG2E;
+    float acc[C];
+    for (int c = 0; c < C; ++c) acc[c] = 0.f;
+    for (int i = 0; i < rg.nt; ++i) {
+        const int j0 = ggw_tile_at(rg, i) * 64, j = j0 + lane;
+        const bool see = j < len && j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && (!keep || keep[j]);
+        float ds = 0.f;
+        if (see) ds = gg_exp2f(ggw_dot<T, D>(q, kb + (long long)j * p.kn) * a2 - lse) * (ggw_dot<T, D>(g, vb + (long long)j * p.vn) - dsum);
+        const unsigned long long bits = gg_ballot(see);
+        for (int k = 0; k < 64; ++k) {
+            const float dk = gg_readlane(ds, k);
+            if (!((bits >> k) & 1)) continue;
+            for (int c = 0; c < C; ++c)
+                if (lane + 64 * c < D) acc[c] += dk * gg_elt_f<T>(kb[(long long)(j0 + k) * p.kn + lane + 64 * c]);
+        }
+    }
+    for (int c = 0; c < C; ++c)
+        if (lane + 64 * c < D) fix[lane + 64 * c] = acc[c];
+}
+
+template <int T, int D>
+GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dq_kernel(GgWinParams p) {
     constexpr int KK = D / 16, DB = D / 32;
     GG_SHARED __attribute__((aligned(1024))) char sK[2][GgwTile<D>::BYTES];
     GG_SHARED __attribute__((aligned(1024))) char sV[2][GgwTile<D>::BYTES];
-    GG_SHARED __attribute__((aligned(16))) unsigned char sBad[64 * (D / 8)];
-    GG_SHARED int sAgain;
+    GG_SHARED float sFix[4][D];
 
     const int lane = threadIdx.x & 63, wave = gg_uniform(threadIdx.x >> 6), hi = lane >> 5;
     const int item = ggw_item();
@@ -648,7 +706,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(64 * NW, 2) void gg_win_dq_kernel(GgWinParams p) {
     const int b = bkv / p.hk, kvh = bkv - b * p.hk;
     const int rows = p.n * p.g;
     const int len = ggw_len(p, b);
-    const int r0 = tile * (32 * NW), rl = r0 + 32 * NW - 1 < rows - 1 ? r0 + 32 * NW - 1 : rows - 1;
+    const int r0 = tile * 128, rl = r0 + 127 < rows - 1 ? r0 + 127 : rows - 1;
     const GgwRange rg = ggw_range<64>(p, len, r0 / p.g, rl / p.g);
     const unsigned char* keep = p.keep ? p.keep + b * p.keep_b : nullptr;
     const GgwWave w = ggw_wave(p, r0 + wave * 32, len, keep != nullptr);
@@ -659,55 +717,38 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(64 * NW, 2) void gg_win_dq_kernel(GgWinParams p) {
     const long long at = (long long)bkv * rows + (w.r < rows ? w.r : rows - 1);
     u16x8 qf[KK], gf[KK];
     float dsum = 0.f;
-    {
-        const unsigned short* qr = p.q + b * p.qb + hq * p.qh + (long long)w.row.token * p.qn + 8 * hi;
-        const unsigned short* gr = p.d_o + b * p.gb + hq * p.gh + (long long)w.row.token * p.gn + 8 * hi;
+    ggw_load_row<KK>(qf, p.q + b * p.qb, p.qh, p.qn, hq, w.row.token);
+    ggw_load_row<KK>(gf, p.d_o + b * p.gb, p.gh, p.gn, hq, w.row.token);
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            qf[kk] = *(const u16x8*)(qr + kk * 16);
-            gf[kk] = *(const u16x8*)(gr + kk * 16);
-            const u16x8 of = *(const u16x8*)(p.o + orow + 8 * hi + kk * 16);
+    for (int kk = 0; kk < KK; ++kk) {
+        const u16x8 of = *(const u16x8*)(p.o + orow + 8 * hi + kk * 16);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dsum += gg_elt_f<T>(gf[kk][e]) * gg_elt_f<T>(of[e]);
-        }
+        for (int e = 0; e < 8; ++e) dsum += gg_elt_f<T>(gf[kk][e]) * gg_elt_f<T>(of[e]);
     }
     dsum = gg_sum_xor32(dsum);
     const float lse = p.lse[at], a2 = p.scale * GGW_LOG2E;
     if (hi == 0 && w.r < rows) p.dvec[at] = dsum;
-    unsigned ko[GgwDma<D, NW>::N], vo[GgwDma<D, NW>::N];
-    ggw_dma_offsets<D, NW>(ko, p.kn);
-    ggw_dma_offsets<D, NW>(vo, p.vn);
+    unsigned ko[D / 32], vo[D / 32];
+    ggw_dma_offsets<D>(ko, p.kn);
+    ggw_dma_offsets<D>(vo, p.vn);
     auto fetch = [&](int i, int buf) {
         const int j0 = ggw_tile_at(rg, i) * 64;
-        ggw_dma<D, NW>(kb + (long long)j0 * p.kn, len - j0, p.kn, ko, sK[buf], wave);
-        ggw_dma<D, NW>(vb + (long long)j0 * p.vn, len - j0, p.vn, vo, sV[buf], wave);
+        ggw_dma<D>(kb, j0, len, p.kn, ko, sK[buf], wave);
+        ggw_dma<D>(vb, j0, len, p.vn, vo, sV[buf], wave);
     };
     f32x16 dqt[DB];
-    bool again = false;             // the second walk: a row that sees a key with a NaN or an infinity gets NaN, the others go without that key
-    float nan = 0.f;
-walk:
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dqt[db][r] = 0.f;
-    if (threadIdx.x == 0) sAgain = 0;
-    if (!again && rg.nt > 0) {
-        gg_wait_vm<0>();            // (the rows above: the transfers' count starts at zero)
-        fetch(0, 0);
-    }
+    const GgwLane lanes = ggw_lane<D>();
+    gg_wait_vm<0>();                // (the rows above: the transfers' count starts at zero)
+    if (rg.nt > 0) fetch(0, 0);
     for (int i = 0, buf = 0; i < rg.nt; ++i, buf ^= 1) {
         const int j0 = ggw_tile_at(rg, i) * 64;
-        if (!again) {
-            gg_wait_vm<0>();
-            gg_barrier_lds();
-            if (i + 1 < rg.nt) fetch(i + 1, buf ^ 1);
-        } else {
-            gg_sync();
-            auto in = [&](int j) { return ggw_in_range(rg, p.sinks, j) && (!keep || keep[j]); };
-            ggw_stage_clean<T, D, NW>(sK[buf], sBad, false, [&](int row) { return in(j0 + row) ? kb + (long long)(j0 + row) * p.kn : nullptr; });
-            ggw_stage_clean<T, D, NW>(sV[buf], sBad, true, [&](int row) { return in(j0 + row) ? vb + (long long)(j0 + row) * p.vn : nullptr; });
-            gg_sync();
-        }
+        gg_wait_vm<0>();
+        gg_barrier_lds();           // this tile is there for everyone, and everyone is through with the last one: its buffer is free
+        if (i + 1 < rg.nt) fetch(i + 1, buf ^ 1);
         if (!ggw_some(w, p.sinks, j0, j0 + 63)) continue;
         const bool masked = !ggw_whole(w, p.sinks, j0, j0 + 63);
         unsigned long long bits = ~0ull;
@@ -716,60 +757,80 @@ walk:
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb) {
             f32x16 st, dp;
+            const GgwLane lo = ggw_here(lanes);
+            // scores and dP in turn, then dq: one stream of operands from the LDS each
+            ggw_pipe<2 * KK>([&](int s) { return ggw_frag<D>(s & 1 ? sV[buf] : sK[buf], jb * 32, s >> 1, lo); },
+                             [&](int s, u16x8 x) {
+                                 if (s < 2) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = -dsum; }
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
-                st = ggw_mfma<T>(ggw_frag<D>(sK[buf], jb * 32, kk, lane), qf[kk], st);
-                dp = ggw_mfma<T>(ggw_frag<D>(sV[buf], jb * 32, kk, lane), gf[kk], dp);
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) st[r] = gg_exp2f(gg_fmaf(st[r], a2, -lse)) * dp[r];
-            if (masked) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int jr = jb * 32 + (r & 3) + 8 * (r >> 2);
-                    const bool see = ggw_sees(w, p.sinks, j0 + jr + 4 * hi) && ((bits >> jr) & 1);
-                    st[r] = see ? st[r] : 0.f;
-                }
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const u16x8 sf = ggw_pack8<T>(st, c);
-#pragma unroll
-                for (int db = 0; db < DB; ++db) dqt[db] = ggw_mfma<T>(ggw_frag_tr<D>(sK[buf], db * 32, jb * 32 + 16 * c, lane), sf, dqt[db]);
-            }
-        }
-        if (again)
-            for (int jr = 0; jr < 64; ++jr)
-                if (ggw_any_bad<D>(sBad, jr) && ggw_sees(w, p.sinks, j0 + jr) && (!keep || keep[j0 + jr])) nan = __builtin_nanf("");
-    }
-    if (!again) {
-        gg_sync();
-        if (ggw_not_finite<DB>(dqt)) sAgain = 1;
-        gg_sync();
-        if (sAgain) {
-            again = true;
-            gg_sync();
-            goto walk;
+                                     for (int r = 0; r < 16; ++r) (s ? dp : st)[r] = s ? -dsum : 0.f;
+                                 }
+                                 if (s & 1) dp = ggw_mfma<T>(x, gf[s >> 1], dp);
+                                 else st = ggw_mfma<T>(x, qf[s >> 1], st);
+                             });
+            ggw_ds(st, dp, a2, lse, masked, w, p.sinks, j0 + jb * 32 + 4 * hi, bits >> (jb * 32));
+            const u16x8 sf[2] = {ggw_pack8<T>(st, 0), ggw_pack8<T>(st, 1)};
+            ggw_pipe<2 * DB>([&](int s) { return ggw_frag_tr<D>(sK[buf], (s % DB) * 32, jb * 32 + 16 * (s / DB), lo); },
+                             [&](int s, u16x8 x) { dqt[s % DB] = ggw_mfma<T>(x, sf[s / DB], dqt[s % DB]); });
         }
     }
-    if (w.r >= rows) return;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int gq = 0; gq < 4; ++gq) {
-            u16x4 o4;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o4[e] = gg_elt<T>(dqt[db][4 * gq + e] * p.scale + nan);
-            *(u16x4*)(p.dq + orow + db * 32 + 8 * gq + 4 * hi) = o4;
+    const unsigned bad = ggw_not_finite<DB>(dqt);
+    if (__builtin_expect(bad != 0, 0))
+        for (int k = 0; k < 32; ++k) {
+            if (!((bad >> k) & 1) || w.r0 + k >= rows) continue;
+            const int token = (w.r0 + k) / p.g, head = kvh * p.g + w.r0 + k - token * p.g, pos = token + len - p.n;
+            ggw_fix_dq<T, D>(p, rg, len, keep, p.q + b * p.qb + head * p.qh + (long long)token * p.qn,
+                             p.d_o + b * p.gb + head * p.gh + (long long)token * p.gn, kb, vb, pos < 0 ? -2 * GGW_NONE : pos, gg_readlane(lse, k),
+                             gg_readlane(dsum, k), sFix[wave]);
+            ggw_take_fix<DB>(dqt, sFix[wave], (lane & 31) == k);
         }
+    ggw_write_dq<T, D>(p, w, b, hq, dqt);
 }
 
 // ---- backward, part 2: dk, dv -----------------------------------------------------------------------------------------
 // workgroup: 4 waves x 32 keys, row tiles of 64 (Q and dO by LDS-DMA, double buffered, each read as rows and transposed). The key tiles that hold sinks are seen by
 // every later row: their rows are cut into p.sink_chunks chunks, each a workgroup of its own that leaves fp32 sums for
 // gg_win_sink_kernel.  part_o: [B*hk][sink_tiles][chunks][2][128][D].
+// one key's dk and dv again, by one wave, from the rows ra .. rb that see it alone: fix[2 D] = sum of dS q, sum of P dO
+template <int T, int D>
+GG_DEVICE void ggw_fix_dkv(const GgWinParams& p, const unsigned short* qb, const unsigned short* gb, const unsigned short* k, const unsigned short* v,
+                           int j, int shift, long long stat, int ra, int rb, float* fix) {
+    constexpr int C = (D + 63) / 64;
+    const int lane = threadIdx.x & 63;
+    const float a2 = p.scale * GGW_LOG2E;
+    float dk[C], dv[C];
+    for (int c = 0; c < C; ++c) dk[c] = dv[c] = 0.f;
+    for (int i0 = ra; i0 <= rb; i0 += 64) {
+        const int r = i0 + lane, rc = r <= rb ? r : rb, tok = rc / p.g, hd = rc - tok * p.g, pos = tok + shift;
+        const float lse = p.lse[stat + rc];
+        const bool see = r <= rb && lse < __builtin_inff() && j <= pos + p.right && (j >= pos - p.left || j < p.sinks);
+        float pr = 0.f, ds = 0.f;
+        if (see || (r <= rb && lse != lse)) {
+            const long long qo = hd * p.qh + (long long)tok * p.qn, go = hd * p.gh + (long long)tok * p.gn;
+            pr = gg_exp2f(ggw_dot<T, D>(qb + qo, k) * a2 - lse);
+            ds = pr * (ggw_dot<T, D>(gb + go, v) - p.dvec[stat + rc]);
+        }
+        const unsigned long long bits = gg_ballot(r <= rb && !(lse == __builtin_inff()) && j <= pos + p.right && (j >= pos - p.left || j < p.sinks));
+        for (int t = 0; t < 64; ++t) {
+            const float st = gg_readlane(ds, t), pt = gg_readlane(pr, t);
+            if (!((bits >> t) & 1)) continue;
+            const int rt = i0 + t, tk = rt / p.g, h = rt - tk * p.g;
+            const unsigned short* qr = qb + h * p.qh + (long long)tk * p.qn;
+            const unsigned short* gr = gb + h * p.gh + (long long)tk * p.gn;
+            for (int c = 0; c < C; ++c)
+                if (lane + 64 * c < D) {
+                    dk[c] += st * gg_elt_f<T>(qr[lane + 64 * c]);
+                    dv[c] += pt * gg_elt_f<T>(gr[lane + 64 * c]);
+                }
+        }
+    }
+    for (int c = 0; c < C; ++c)
+        if (lane + 64 * c < D) {
+            fix[lane + 64 * c] = dk[c];
+            fix[D + lane + 64 * c] = dv[c];
+        }
+}
+
 template <int T, int D>
 GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
     constexpr int KK = D / 16, DB = D / 32;
@@ -778,8 +839,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
     GG_SHARED __attribute__((aligned(16))) float sLse[2][64];
     GG_SHARED __attribute__((aligned(16))) float sD[2][64];
     GG_SHARED __attribute__((aligned(16))) int sPos[2][64];
-    GG_SHARED __attribute__((aligned(16))) unsigned char sBad[64 * (D / 8)];
-    GG_SHARED int sAgain;
+    GG_SHARED float sFix[4][2 * D];
 
     const int lane = threadIdx.x & 63, wave = gg_uniform(threadIdx.x >> 6), hi = lane >> 5;
     const int per = p.sink_tiles * p.sink_chunks + p.row_tiles - p.sink_tiles;
@@ -835,6 +895,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
     constexpr int NV = D / 32;
     const int step_t = 64 / p.g, step_h = 64 - step_t * p.g;
     int vt[NV], vh[NV];
+    int ft = 0, fh = 0;                     // (uniform) the next tile's first row
     int rt = 0, rh = 0;                     // the row whose statistics this thread fetches (threads 0 .. 63)
     auto start = [&](int i0) {
 #pragma unroll
@@ -846,25 +907,32 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
         const int r = i0 + (int)(threadIdx.x & 63);
         rt = (int)((unsigned)r / (unsigned)p.g);
         rh = r - rt * p.g;
+        ft = (int)((unsigned)i0 / (unsigned)p.g);
+        fh = i0 - ft * p.g;
     };
+    const GgwLane lanes = ggw_lane<D>();
     float r_lse = 0.f, r_d = 0.f;
     int r_pos = 0;
     auto fetch = [&](int i0, int buf) {
-        const int t0 = (int)((unsigned)i0 / (unsigned)p.g);
+        const int t0 = ft;
         const GgBufS bq = gg_make_bufs(qb + (long long)t0 * p.qn, GGW_SPAN), bg = gg_make_bufs(gb + (long long)t0 * p.gn, GGW_SPAN);
 #pragma unroll
         for (int s = 0; s < NV; ++s) {
             const int v = threadIdx.x + 256 * s, row = v / (D / 8), c = (v % (D / 8)) ^ ggw_swz<D>(row);
             // (rows behind the last one: an offset that the buffer's bounds check turns into zeros)
             const bool in = i0 + row <= (int)rb;
-            const unsigned oq = in ? (unsigned)(((long long)(vt[s] - t0) * p.qn + (long long)vh[s] * p.qh) * 2) + (c << 4) : GGW_SPAN;
-            const unsigned og = in ? (unsigned)(((long long)(vt[s] - t0) * p.gn + (long long)vh[s] * p.gh) * 2) + (c << 4) : GGW_SPAN;
+            const unsigned dt = vt[s] - t0, dh = vh[s];
+            const unsigned oq = in ? (dt * p.qn + dh * (unsigned)p.qh) * 2 + (c << 4) : GGW_SPAN;
+            const unsigned og = in ? (dt * p.gn + dh * (unsigned)p.gh) * 2 + (c << 4) : GGW_SPAN;
             gg_bufs_load_lds16(bq, oq, 0, sQ[buf] + (wave + 4 * s) * 1024);
             gg_bufs_load_lds16(bg, og, 0, sG[buf] + (wave + 4 * s) * 1024);
             vt[s] += step_t;
             vh[s] += step_h;
             if (vh[s] >= p.g) { vh[s] -= p.g; ++vt[s]; }
         }
+        ft += step_t;
+        fh += step_h;
+        if (fh >= p.g) { fh -= p.g; ++ft; }
     };
     auto stats = [&](int i0) {              // lse = +inf: a row that is not there or sees nothing
         const int r = i0 + (int)(threadIdx.x & 63);
@@ -877,56 +945,52 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
         rh += step_h;
         if (rh >= p.g) { rh -= p.g; ++rt; }
     };
-    bool again = false;             // the second walk: a key that a row with a NaN or an infinity sees gets NaN, the others go without that row
-    float nan = 0.f;
-walk:
 #pragma unroll
     for (int i = 0; i < 2 * DB; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
-    if (threadIdx.x == 0) sAgain = 0;
     if (ra <= rb) {
         start((int)ra);
         stats((int)ra);
-        if (!again) fetch((int)ra, 0);
+        gg_wait_vm<0>();            // (this wave's keys: the transfers' count starts at zero)
+        fetch((int)ra, 0);
     }
+    // a row's distance from its tile's first row to tokens: x / g for x < g + 64 by a reciprocal rounded up (exact: x g < 2^32)
+    const unsigned recip = p.g > 1 ? (unsigned)(0xffffffffu / (unsigned)p.g) + 1u : 0u;
+    auto tokens = [&](int x) { return recip ? (int)(((unsigned long long)(unsigned)x * recip) >> 32) : x; };
+    int ct = 0, ch = 0;
+    if (ra <= rb) { ct = (int)((unsigned)(int)ra / (unsigned)p.g); ch = (int)ra - ct * p.g; }
     for (int i0 = (int)ra, buf = 0; i0 <= (int)rb; i0 += 64, buf ^= 1) {
+        const int t0 = ct, h0 = ch;
+        ct += step_t;
+        ch += step_h;
+        if (ch >= p.g) { ch -= p.g; ++ct; }
         if (threadIdx.x < 64) { sLse[buf][threadIdx.x] = r_lse; sD[buf][threadIdx.x] = r_d; sPos[buf][threadIdx.x] = r_pos; }
-        if (!again) {
-            gg_wait_vm<0>();
-            gg_barrier_lds();
-            if (i0 + 64 <= (int)rb) {
-                stats(i0 + 64);
-                fetch(i0 + 64, buf ^ 1);
-            }
-        } else {
-            gg_sync();
-            auto at = [&](const unsigned short* base, long long hs, long long ns, int row) -> const unsigned short* {
-                const int r = i0 + row, tok = (int)((unsigned)r / (unsigned)p.g);
-                if (r > (int)rb || !(sLse[buf][row] < __builtin_inff())) return nullptr;
-                return base + (long long)tok * ns + (long long)(r - tok * p.g) * hs;
-            };
-            ggw_stage_clean<T, D, 4>(sQ[buf], sBad, false, [&](int row) { return at(qb, p.qh, p.qn, row); });
-            ggw_stage_clean<T, D, 4>(sG[buf], sBad, true, [&](int row) { return at(gb, p.gh, p.gn, row); });
-            if (i0 + 64 <= (int)rb) stats(i0 + 64);
-            gg_sync();
+        gg_wait_vm<0>();
+        gg_barrier_lds();
+        if (i0 + 64 <= (int)rb) {
+            stats(i0 + 64);
+            fetch(i0 + 64, buf ^ 1);
         }
 #pragma unroll
         for (int ib = 0; ib < 2; ++ib) {
             // the 32 rows' positions: all there, and the wave's 32 keys all seen by all of them?
             const int r1 = i0 + ib * 32 + 31;
             if (i0 + ib * 32 > (int)rb) break;
-            const int plo = (i0 + ib * 32) / p.g + shift, phi = (r1 <= (int)rb ? r1 : (int)rb) / p.g + shift;
+            const int plo = t0 + tokens(h0 + ib * 32) + shift, phi = t0 + tokens(h0 + (r1 <= (int)rb ? ib * 32 + 31 : (int)rb - i0)) + shift;
             if (kj0 > phi + p.right || (wlast < plo - p.left && kj0 >= p.sinks) || kj0 >= len) continue;
             const bool full = whole && r1 <= (int)rb && wlast <= plo + p.right && (kj0 >= phi - p.left || wlast < p.sinks);
             f32x16 st, dp;
+            const GgwLane lo = ggw_here(lanes);
+            ggw_pipe<2 * KK>([&](int s) { return ggw_frag<D>(s & 1 ? sG[buf] : sQ[buf], ib * 32, s >> 1, lo); },
+                             [&](int s, u16x8 x) {
+                                 if (s < 2) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = 0.f; }
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
-                st = ggw_mfma<T>(ggw_frag<D>(sQ[buf], ib * 32, kk, lane), kf[kk], st);
-                dp = ggw_mfma<T>(ggw_frag<D>(sG[buf], ib * 32, kk, lane), vf[kk], dp);
-            }
+                                     for (int r = 0; r < 16; ++r) (s ? dp : st)[r] = 0.f;
+                                 }
+                                 if (s & 1) dp = ggw_mfma<T>(x, vf[s >> 1], dp);
+                                 else st = ggw_mfma<T>(x, kf[s >> 1], st);
+                             });
 #pragma unroll
             for (int gq = 0; gq < 4; ++gq) {
                 const int at = ib * 32 + 8 * gq + 4 * hi;
@@ -946,32 +1010,27 @@ walk:
                         dp[r] = see ? dp[r] : 0.f;
                     }
             }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const u16x8 pf = ggw_pack8<T>(st, c), sf = ggw_pack8<T>(dp, c);
-#pragma unroll
-                for (int db = 0; db < DB; ++db) {
-                    dvt[db] = ggw_mfma<T>(ggw_frag_tr<D>(sG[buf], db * 32, ib * 32 + 16 * c, lane), pf, dvt[db]);
-                    dkt[db] = ggw_mfma<T>(ggw_frag_tr<D>(sQ[buf], db * 32, ib * 32 + 16 * c, lane), sf, dkt[db]);
-                }
-            }
-            if (again)
-                for (int ir = ib * 32; ir < ib * 32 + 32; ++ir)
-                    if (ggw_any_bad<D>(sBad, ir)) {
-                        const int pos = sPos[buf][ir];
-                        if (kept && kj <= pos + p.right && (kj >= pos - p.left || kj < p.sinks)) nan = __builtin_nanf("");
-                    }
+            const u16x8 pf[2] = {ggw_pack8<T>(st, 0), ggw_pack8<T>(st, 1)}, sf[2] = {ggw_pack8<T>(dp, 0), ggw_pack8<T>(dp, 1)};
+            ggw_pipe<4 * DB>([&](int s) { return ggw_frag_tr<D>(s & 1 ? sQ[buf] : sG[buf], (s / 2 % DB) * 32, ib * 32 + 16 * (s / (2 * DB)), lo); },
+                             [&](int s, u16x8 x) {
+                                 const int db = s / 2 % DB, c = s / (2 * DB);
+                                 if (s & 1) dkt[db] = ggw_mfma<T>(x, sf[c], dkt[db]);
+                                 else dvt[db] = ggw_mfma<T>(x, pf[c], dvt[db]);
+                             });
         }
     }
-    if (!again) {
-        gg_sync();
-        if (ggw_not_finite<2 * DB>(acc)) sAgain = 1;
-        gg_sync();
-        if (sAgain) {
-            again = true;
-            gg_sync();
-            goto walk;
+    const unsigned bad = ggw_not_finite<2 * DB>(acc);
+    if (__builtin_expect(bad != 0, 0))
+        for (int k = 0; k < 32; ++k) {
+            const int j = kj0 + k;
+            if (!((bad >> k) & 1) || j >= len || (keep && !keep[j])) continue;          // (a key that nobody sees ends as zeros below)
+            ggw_fix_dkv<T, D>(p, qb, gb, p.k + b * p.kb + kvh * p.kh + (long long)j * p.kn, p.v + b * p.vb + kvh * p.vh + (long long)j * p.vn, j, shift,
+                              (long long)bkv * rows, (int)ra, (int)rb, sFix[wave]);
+            ggw_take_fix<2 * DB>(acc, sFix[wave], (lane & 31) == k);
         }
+    if (__builtin_expect(bad != 0, 0) && !kept) {
+        for (int i = 0; i < 2 * DB; ++i)
+            for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     }
     if (chunked) {
         float* po = p.part_o + ((((long long)bkv * p.sink_tiles + tile) * p.sink_chunks + chunk) * 2 * 128 + wave * 32 + (lane & 31)) * D;
@@ -980,8 +1039,8 @@ walk:
 #pragma unroll
             for (int gq = 0; gq < 4; ++gq) {
                 const int d = db * 32 + 8 * gq + 4 * hi;
-                *(f32x4*)(po + d) = f32x4{dkt[db][4 * gq] + nan, dkt[db][4 * gq + 1] + nan, dkt[db][4 * gq + 2] + nan, dkt[db][4 * gq + 3] + nan};
-                *(f32x4*)(po + 128 * D + d) = f32x4{dvt[db][4 * gq] + nan, dvt[db][4 * gq + 1] + nan, dvt[db][4 * gq + 2] + nan, dvt[db][4 * gq + 3] + nan};
+                *(f32x4*)(po + d) = f32x4{dkt[db][4 * gq], dkt[db][4 * gq + 1], dkt[db][4 * gq + 2], dkt[db][4 * gq + 3]};
+                *(f32x4*)(po + 128 * D + d) = f32x4{dvt[db][4 * gq], dvt[db][4 * gq + 1], dvt[db][4 * gq + 2], dvt[db][4 * gq + 3]};
             }
         return;
     }
@@ -994,8 +1053,8 @@ walk:
             u16x4 k4, v4;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                k4[e] = gg_elt<T>(dkt[db][4 * gq + e] * p.scale + nan);
-                v4[e] = gg_elt<T>(dvt[db][4 * gq + e] + nan);
+                k4[e] = gg_elt<T>(dkt[db][4 * gq + e] * p.scale);
+                v4[e] = gg_elt<T>(dvt[db][4 * gq + e]);
             }
             *(u16x4*)(p.dk + krow + db * 32 + 8 * gq + 4 * hi) = k4;
             *(u16x4*)(p.dv + krow + db * 32 + 8 * gq + 4 * hi) = v4;

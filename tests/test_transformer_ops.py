@@ -417,6 +417,9 @@ ATT_GPU = ATT_CPU + [
     (2, 2, 2, 500, 500, 64, (63, 64), 64),
     (1, 1, 1, 1500, 1500, 32, (3, 0), 200),
     (65, 1, 1, 17, 19, 64, (4, 2), 1),
+    (128, 2, 2, 33, 130, 128, (70, 30), 2),             # eight waves a workgroup
+    (2, 128, 128, 300, 700, 128, (200, 9), 3),
+    (1, 64, 32, 1100, 1100, 128, (None, 0), 0),
 ]
 
 
@@ -523,6 +526,7 @@ def test_window_attention_nan_reaches_only_who_sees_it(where):
         clean = [t.detach().requires_grad_() for t in (q, k, v)]
         oc = ops.impl.window_attention(*clean, **kw)
         gc = torch.autograd.grad(oc, clean, do)
+        exact = att_ref(q, k, v, 0.2, seen(1, n, 40, (None, 0), 0, None, None, where), do)
         rows = torch.arange(n) < n - 2                          # key 38 is seen by the last two of the queries
         for spoil in ('k', 'v'):
             for fill in (math.nan, math.inf):
@@ -530,7 +534,7 @@ def test_window_attention_nan_reaches_only_who_sees_it(where):
                 (k2 if spoil == 'k' else v2)[0, 0, 38, 5] = fill
                 bad = [t.detach().requires_grad_() for t in (q, k2, v2)]
                 o = ops.impl.window_attention(*bad, **kw)
-                assert torch.equal(oc[:, :, rows], o[:, :, rows]), (n, spoil, fill)
+                within(o[:, :, rows], exact[0][0][:, :, rows], exact[0][1][:, :, rows], 'o')
                 late = o[:, :, ~rows]
                 if spoil == 'v':
                     others = [i for i in range(32) if i != 5]
@@ -541,7 +545,7 @@ def test_window_attention_nan_reaches_only_who_sees_it(where):
                     up = (q[:, :, ~rows][..., 5] > 0)[..., None].expand_as(late)
                     assert torch.equal(torch.isfinite(late), ~up)
                 dq, dk, dv = torch.autograd.grad(o, bad, do)
-                assert torch.equal(dq[:, :, rows], gc[0][:, :, rows])
+                within(dq[:, :, rows], exact[1][0][:, :, rows], exact[1][1][:, :, rows], 'dq')
         # query 1 of n sees keys 0 .. 40 - n + 1
         last = 40 - n + 1
         for spoil in ('q', 'do'):
@@ -550,8 +554,9 @@ def test_window_attention_nan_reaches_only_who_sees_it(where):
             bad = [t.detach().requires_grad_() for t in (q2, k, v)]
             o = ops.impl.window_attention(*bad, **kw)
             dq, dk, dv = torch.autograd.grad(o, bad, do2)
-            for got, ref in ((dk, gc[1]), (dv, gc[2])):
-                assert torch.equal(got[:, :, last + 1:], ref[:, :, last + 1:]) and not torch.isfinite(got[:, :, :last + 1, 7]).any()
+            for got, (ref, tol) in ((dk, exact[2]), (dv, exact[3])):
+                within(got[:, :, last + 1:], ref[:, :, last + 1:], tol[:, :, last + 1:], spoil)
+                assert not torch.isfinite(got[:, :, :last + 1, 7]).any()
             others = torch.ones(h, n, dtype=torch.bool)
             others[0, 1] = False
             assert torch.equal(dq[0][others], gc[0][0][others])
