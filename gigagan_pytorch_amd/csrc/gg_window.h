@@ -890,13 +890,26 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
 
     const unsigned short* qb = p.q + b * p.qb + (long long)kvh * p.g * p.qh;
     const unsigned short* gb = p.d_o + b * p.gb + (long long)kvh * p.g * p.gh;
-    // this thread's vectors of a row tile: row index -> (token, head) kept up from tile to tile, addresses relative to the tile's first
-    // token (host: they fit 32 bits)
+    // This thread's vectors of a row tile, as 32-bit offsets from the tile's first token (host: they fit). Where g divides 64 every tile
+    // starts at a token's first head and the offsets stay what they are; else the vectors' (token, head) are kept up from tile to tile.
     constexpr int NV = D / 32;
     const int step_t = 64 / p.g, step_h = 64 - step_t * p.g;
     int vt[NV], vh[NV];
+    unsigned oq[NV], og[NV];
     int ft = 0, fh = 0;                     // (uniform) the next tile's first row
     int rt = 0, rh = 0;                     // the row whose statistics this thread fetches (threads 0 .. 63)
+    auto offsets = [&]() {
+#pragma unroll
+        for (int s = 0; s < NV; ++s) {
+            const int v = threadIdx.x + 256 * s, c = (v % (D / 8)) ^ ggw_swz<D>(v / (D / 8));
+            const unsigned dt = vt[s] - ft, dh = vh[s];
+            oq[s] = (dt * p.qn + dh * (unsigned)p.qh) * 2 + (c << 4);
+            og[s] = (dt * p.gn + dh * (unsigned)p.gh) * 2 + (c << 4);
+            vt[s] += step_t;
+            vh[s] += step_h;
+            if (vh[s] >= p.g) { vh[s] -= p.g; ++vt[s]; }
+        }
+    };
     auto start = [&](int i0) {
 #pragma unroll
         for (int s = 0; s < NV; ++s) {
@@ -909,37 +922,33 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
         rh = r - rt * p.g;
         ft = (int)((unsigned)i0 / (unsigned)p.g);
         fh = i0 - ft * p.g;
+        offsets();
     };
     const GgwLane lanes = ggw_lane<D>();
     float r_lse = 0.f, r_d = 0.f;
     int r_pos = 0;
     auto fetch = [&](int i0, int buf) {
-        const int t0 = ft;
-        const GgBufS bq = gg_make_bufs(qb + (long long)t0 * p.qn, GGW_SPAN), bg = gg_make_bufs(gb + (long long)t0 * p.gn, GGW_SPAN);
+        const GgBufS bq = gg_make_bufs(qb + (unsigned long long)(unsigned)ft * p.qn, GGW_SPAN), bg = gg_make_bufs(gb + (unsigned long long)(unsigned)ft * p.gn, GGW_SPAN);
+        const bool all = i0 + 63 <= (int)rb;
 #pragma unroll
         for (int s = 0; s < NV; ++s) {
-            const int v = threadIdx.x + 256 * s, row = v / (D / 8), c = (v % (D / 8)) ^ ggw_swz<D>(row);
             // (rows behind the last one: an offset that the buffer's bounds check turns into zeros)
-            const bool in = i0 + row <= (int)rb;
-            const unsigned dt = vt[s] - t0, dh = vh[s];
-            const unsigned oq = in ? (dt * p.qn + dh * (unsigned)p.qh) * 2 + (c << 4) : GGW_SPAN;
-            const unsigned og = in ? (dt * p.gn + dh * (unsigned)p.gh) * 2 + (c << 4) : GGW_SPAN;
-            gg_bufs_load_lds16(bq, oq, 0, sQ[buf] + (wave + 4 * s) * 1024);
-            gg_bufs_load_lds16(bg, og, 0, sG[buf] + (wave + 4 * s) * 1024);
-            vt[s] += step_t;
-            vh[s] += step_h;
-            if (vh[s] >= p.g) { vh[s] -= p.g; ++vt[s]; }
+            const bool in = all || i0 + (int)(threadIdx.x + 256 * s) / (D / 8) <= (int)rb;
+            gg_bufs_load_lds16(bq, in ? oq[s] : GGW_SPAN, 0, sQ[buf] + (wave + 4 * s) * 1024);
+            gg_bufs_load_lds16(bg, in ? og[s] : GGW_SPAN, 0, sG[buf] + (wave + 4 * s) * 1024);
         }
         ft += step_t;
         fh += step_h;
         if (fh >= p.g) { fh -= p.g; ++ft; }
+        if (step_t * p.g != 64) offsets();
     };
+    const float *lse = p.lse + (long long)bkv * rows, *dvec = p.dvec + (long long)bkv * rows;
     auto stats = [&](int i0) {              // lse = +inf: a row that is not there or sees nothing
         const int r = i0 + (int)(threadIdx.x & 63);
         const bool in = r <= (int)rb;
-        const long long at = (long long)bkv * rows + (in ? r : (int)rb);
-        r_lse = in ? p.lse[at] : __builtin_inff();
-        r_d = in ? p.dvec[at] : 0.f;
+        const unsigned at = in ? r : (int)rb;
+        r_lse = in ? lse[at] : __builtin_inff();
+        r_d = in ? dvec[at] : 0.f;
         r_pos = in ? rt + shift : -2 * GGW_NONE;
         rt += step_t;
         rh += step_h;
