@@ -119,11 +119,11 @@ GG_DEVICE u16x8 ggw_frag_tr(const char* tile, int d0, int rb, const GgwLane& o) 
     return u16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// N products whose A operands come from the LDS, GGW_AHEAD operands read ahead of their use and the order kept
-#define GGW_AHEAD 4
-template <int N, class Read, class Use>
+// N products whose A operands come from the LDS, AHEAD operands read ahead of their use and the order kept (2, 4, 6, 8 ahead: forward at
+// head 64 106, 101, 108, 109 us; four, and two where the accumulators leave no registers)
+template <int N, int AHEAD = 4, class Read, class Use>
 GG_DEVICE void ggw_pipe(Read read, Use use) {
-    constexpr int A = GGW_AHEAD < N ? GGW_AHEAD : N;
+    constexpr int A = AHEAD < N ? AHEAD : N;
     u16x8 f[A];
 #pragma unroll
     for (int s = 0; s < A; ++s) f[s] = read(s);
@@ -404,7 +404,10 @@ GG_DEVICE void ggw_fix_rows(const GgWinParams& p, const GgwWave& w, const GgwRan
 }
 
 // workgroup: 4 waves x 32 rows; key tiles of 64 fetched once for all of them by LDS-DMA, double buffered: one barrier a tile, behind
-// which the next tile's transfers start and run under this tile's arithmetic.
+// which the next tile's transfers start and run under this tile's arithmetic. What bounds it is the LDS: every product takes a kilobyte
+// operand from it (attend-long without those reads 1515 of 2145 us, without the softmax 1751, without the transfers 1875). Measured and
+// not kept: two 32-row blocks a wave for each operand read (half the reads, but one wave a SIMD: 2604), eight waves a tile in two
+// groups half a tile apart (2330), wave priorities (no change).
 // SPLIT: the tiles are dealt out to p.splits workgroups, which leave (m, l, O) for gg_win_join_kernel.
 template <int T, int D, bool SPLIT>
 GG_KERNEL GG_LAUNCH_BOUNDS2(256, D == 128 ? 2 : 3) void gg_win_fwd_kernel(GgWinParams p) {
@@ -991,7 +994,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
             const bool full = whole && r1 <= (int)rb && wlast <= plo + p.right && (kj0 >= phi - p.left || wlast < p.sinks);
             f32x16 st, dp;
             const GgwLane lo = ggw_here(lanes);
-            ggw_pipe<2 * KK>([&](int s) { return ggw_frag<D>(s & 1 ? sG[buf] : sQ[buf], ib * 32, s >> 1, lo); },
+            ggw_pipe<2 * KK, D == 128 ? 2 : 4>([&](int s) { return ggw_frag<D>(s & 1 ? sG[buf] : sQ[buf], ib * 32, s >> 1, lo); },
                              [&](int s, u16x8 x) {
                                  if (s < 2) {
 #pragma unroll
@@ -1020,7 +1023,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
                     }
             }
             const u16x8 pf[2] = {ggw_pack8<T>(st, 0), ggw_pack8<T>(st, 1)}, sf[2] = {ggw_pack8<T>(dp, 0), ggw_pack8<T>(dp, 1)};
-            ggw_pipe<4 * DB>([&](int s) { return ggw_frag_tr<D>(s & 1 ? sQ[buf] : sG[buf], (s / 2 % DB) * 32, ib * 32 + 16 * (s / (2 * DB)), lo); },
+            ggw_pipe<4 * DB, D == 128 ? 2 : 4>([&](int s) { return ggw_frag_tr<D>(s & 1 ? sQ[buf] : sG[buf], (s / 2 % DB) * 32, ib * 32 + 16 * (s / (2 * DB)), lo); },
                              [&](int s, u16x8 x) {
                                  const int db = s / 2 % DB, c = s / (2 * DB);
                                  if (s & 1) dkt[db] = ggw_mfma<T>(x, sf[c], dkt[db]);
