@@ -4,6 +4,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import math
+import struct
 
 import torch
 
@@ -1394,7 +1395,7 @@ def _same_device(what: str, first: torch.Tensor, *rest):
 
 def _on_device(L, t: torch.Tensor):
     """the launch's device made current where it is not (a launch goes to the current device, whatever device its stream is of)"""
-    if L.is_emulator or t.device.index == torch.cuda.current_device():
+    if L.is_emulator or t.device.index == torch._C._cuda_getDevice():
         return contextlib.nullcontext()
     return torch.cuda.device(t.device)
 
@@ -1417,7 +1418,8 @@ LAYERNORM_MAX_C = 16384
 
 
 def layernorm_fwd(x: torch.Tensor, w: torch.Tensor, b, eps: float, stats: bool):
-    """x (..., C) bf16 / fp16 / fp32, w and b (C,) fp32 -> (y like x, contiguous; mean, rstd (rows,) fp32 or None)."""
+    """x (..., C) bf16 / fp16 / fp32, w and b (C,) fp32 -> (y like x, contiguous; the rows' mean and 1 / deviation
+    (2, rows) fp32, or None)."""
     L = _C.lib()
     L.require(x, w, b)
     dt = _row_type('layernorm_fwd', x)
@@ -1426,22 +1428,24 @@ def layernorm_fwd(x: torch.Tensor, w: torch.Tensor, b, eps: float, stats: bool):
     _same_device('layernorm_fwd', x, w, b)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     rows = y.numel() // Cc
-    mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else (None, None)
+    st = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else None
     if rows:
         x2 = _rows2(x)
+        at = st.data_ptr() if stats else 0
         with _on_device(L, x):
-            rc = L.lib.gg_layernorm_fwd(ptr(x2), x2.stride(0), ptr(w), ptr(b), ptr(y), ptr(mean), ptr(rstd), rows, Cc, eps, dt, L.stream(x))
+            rc = L.lib.gg_layernorm_fwd(x2.data_ptr(), x2.stride(0), w.data_ptr(), ptr(b), y.data_ptr(), at, at and at + 4 * rows, rows, Cc, eps, dt,
+                                        L.stream(x))
         L.check(rc, 'gg_layernorm_fwd')
-    return y, mean, rstd
+    return y, st
 
 
-def layernorm_bwd(x: torch.Tensor, dy: torch.Tensor, w: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, want_db: bool):
+def layernorm_bwd(x: torch.Tensor, dy: torch.Tensor, w: torch.Tensor, stats: torch.Tensor, want_db: bool):
     """-> (dx like x, contiguous; dw (C,) fp32; db (C,) fp32 or None)."""
     L = _C.lib()
-    L.require(x, dy, w, mean, rstd)
+    L.require(x, dy, w, stats)
     dt = _row_type('layernorm_bwd', x)
     assert dy.dtype == x.dtype and dy.shape == x.shape
-    _same_device('layernorm_bwd', x, dy, w, mean, rstd)
+    _same_device('layernorm_bwd', x, dy, w, stats)
     Cc = x.shape[-1]
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     rows = dx.numel() // Cc
@@ -1453,8 +1457,8 @@ def layernorm_bwd(x: torch.Tensor, dy: torch.Tensor, w: torch.Tensor, mean: torc
     db = torch.empty_like(dw) if want_db else None
     part = torch.empty((L.lib.gg_layernorm_blocks(rows, Cc), 2, Cc), dtype=torch.float32, device=x.device)
     with _on_device(L, x):
-        rc = L.lib.gg_layernorm_bwd(ptr(x2), x2.stride(0), ptr(g2), g2.stride(0), ptr(w), ptr(mean), ptr(rstd), ptr(dx), ptr(part), ptr(dw),
-                                    ptr(db), rows, Cc, dt, L.stream(x))
+        rc = L.lib.gg_layernorm_bwd(x2.data_ptr(), x2.stride(0), g2.data_ptr(), g2.stride(0), w.data_ptr(), stats.data_ptr(),
+                                    stats.data_ptr() + 4 * rows, dx.data_ptr(), part.data_ptr(), dw.data_ptr(), ptr(db), rows, Cc, dt, L.stream(x))
     L.check(rc, 'gg_layernorm_bwd')
     return dx, dw, db
 
@@ -1500,6 +1504,9 @@ class RotarySpec:
         return RotarySpec, (self.sections, self.theta, self.shared, self.interleaved)
 
 
+_ROTARY_PACK = struct.Struct('@4P6qP3q2P12i').pack         # gg_rotary_desc
+
+
 def _heads4(t: torch.Tensor) -> torch.Tensor:
     """(B, h, n, d) with unit feature stride, copied where it has another"""
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
@@ -1519,13 +1526,11 @@ def rotary(q: torch.Tensor, k, positions: torch.Tensor, spec: RotarySpec, invers
     q = _heads4(q)
     k = None if k is None else _heads4(k)
     ps = positions.stride() if positions.dim() == 3 else (0, *positions.stride())
-    D = _C.RotaryDesc(q=ptr(q), k=ptr(k), yq=ptr(outs[0]), yk=ptr(outs[1]), q_strides=(C.c_int64 * 3)(*q.stride()[:3]),
-                      k_strides=(C.c_int64 * 3)(*(k.stride()[:3] if k is not None else (0, 0, 0))), positions=ptr(positions),
-                      p_strides=(C.c_int64 * 3)(*ps), freqs=C.addressof(spec._freqs), axes=C.addressof(spec._axes),
-                      pos_type=_POS_TYPES[positions.dtype], dtype=dt, B=B, n=n, hq=h, hk=hk, d=d, pairs=spec.pairs,
-                      n_axes=len(spec.sections), interleaved=int(spec.interleaved), inverse=int(inverse))
+    D = _ROTARY_PACK(q.data_ptr(), ptr(k) or 0, outs[0].data_ptr(), ptr(outs[1]) or 0, *q.stride()[:3], *(k.stride()[:3] if k is not None else (0, 0, 0)),
+                     positions.data_ptr(), *ps, C.addressof(spec._freqs), C.addressof(spec._axes), _POS_TYPES[positions.dtype], dt, B, n, h, hk, d,
+                     spec.pairs, len(spec.sections), spec.interleaved, inverse, 0)
     with _on_device(L, q):
-        rc = L.lib.gg_rotary(C.byref(D), L.stream(q))
+        rc = L.lib.gg_rotary(D, L.stream(q))
     L.check(rc, 'gg_rotary')
     return tuple(outs)
 
@@ -1534,24 +1539,29 @@ WINDOW_HEAD_DIMS = (32, 64, 128)
 
 
 def _strides3(t: torch.Tensor):
-    return (C.c_int64 * 3)(*(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])))
+    s0, s1, s2, _ = t.stride()
+    n0, n1, n2, _ = t.shape
+    return (s0 if n0 > 1 else 0, s1 if n1 > 1 else 0, s2 if n2 > 1 else 0)
 
 
 def _attend4(t: torch.Tensor, group: int = 0) -> torch.Tensor:
     """(B, h, n, d) as the window kernels read it (unit feature stride, strides of whole 16-byte vectors below their limits, aligned), or
     a copy that is; `group`: query heads a key head, for queries"""
-    s = [x if n > 1 else 0 for x, n in zip(t.stride(), t.shape)]
-    ok = (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not (s[0] | s[1] | s[2]) & 7 and s[2] < 1 << 24
-          and (not group or s[1] * group < 1 << 30))
+    s0, s1, s2 = _strides3(t)
+    ok = (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not (s0 | s1 | s2) & 7 and s2 < 1 << 24
+          and (not group or s1 * group < 1 << 30))
     return t if ok else t.transpose(1, 2).clone(memory_format=torch.contiguous_format).transpose(1, 2)
 
 
-def _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask):
+_WINDOW_PACK = struct.Struct('@10P12q2Pq10ifi').pack         # gg_window_desc (a packed string costs a fifth of a ctypes structure)
+
+
+def _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask, d_o=None, dq=None, dk=None, dv=None, dvec=None):
     B, h, n, d = q.shape
-    return _C.WindowDesc(q=ptr(q), k=ptr(k), v=ptr(v), o=ptr(o), lse=ptr(lse), q_strides=_strides3(q), k_strides=_strides3(k),
-                         v_strides=_strides3(v), lengths=ptr(lengths), key_mask=ptr(key_mask),
-                         mask_stride=0 if key_mask is None or B == 1 else key_mask.stride(0), B=B, n=n, m=k.shape[2], h=h, hk=k.shape[1], d=d,
-                         left=left, right=right, sinks=sinks, dtype=_ROW_TYPES[q.dtype], scale=scale)
+    return _WINDOW_PACK(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ptr(lse) or 0, ptr(d_o) or 0, ptr(dq) or 0, ptr(dk) or 0,
+                        ptr(dv) or 0, ptr(dvec) or 0, *_strides3(q), *_strides3(k), *_strides3(v), *((0, 0, 0) if d_o is None else _strides3(d_o)),
+                        ptr(lengths) or 0, ptr(key_mask) or 0, 0 if key_mask is None or B == 1 else key_mask.stride(0), B, n, k.shape[2], h,
+                        k.shape[1], d, left, right, sinks, _ROW_TYPES[q.dtype], scale, 0)
 
 
 def window_fwd(q, k, v, scale: float, left: int, right: int, sinks: int, lengths, key_mask, want_lse: bool):
@@ -1569,9 +1579,9 @@ def window_fwd(q, k, v, scale: float, left: int, right: int, sinks: int, lengths
     q, k, v = _attend4(q, h // k.shape[1]), _attend4(k), _attend4(v)
     D = _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask)
     with _on_device(L, q):
-        nbytes = L.lib.gg_window_workspace_bytes(C.byref(D), 0)
+        nbytes = L.lib.gg_window_workspace_bytes(D, 0)
         ws = _workspace(nbytes, q) if nbytes else None
-        rc = L.lib.gg_window_fwd(C.byref(D), ptr(ws), nbytes, L.stream(q))
+        rc = L.lib.gg_window_fwd(D, ptr(ws), nbytes, L.stream(q))
     L.check(rc, 'gg_window_fwd')
     return o.transpose(1, 2), lse
 
@@ -1592,13 +1602,12 @@ def window_bwd(q, k, v, o, lse, d_o, scale: float, left: int, right: int, sinks:
             t.zero_()
         return views
     q, k, v, d_o = _attend4(q, h // hk), _attend4(k), _attend4(v), _attend4(d_o, h // hk)
-    D = _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask)
     dvec = torch.empty_like(lse)
-    D.d_o, D.g_strides, D.dq, D.dk, D.dv, D.dvec = ptr(d_o), _strides3(d_o), ptr(dq), ptr(dk), ptr(dv), ptr(dvec)
+    D = _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask, d_o, dq, dk, dv, dvec)
     with _on_device(L, q):
-        nbytes = L.lib.gg_window_workspace_bytes(C.byref(D), 1)
+        nbytes = L.lib.gg_window_workspace_bytes(D, 1)
         ws = _workspace(nbytes, q) if nbytes else None
-        rc = L.lib.gg_window_bwd(C.byref(D), ptr(ws), nbytes, L.stream(q))
+        rc = L.lib.gg_window_bwd(D, ptr(ws), nbytes, L.stream(q))
     L.check(rc, 'gg_window_bwd')
     return views
 

@@ -744,26 +744,36 @@ class RmsNormBwdFn(Function):
         return gx, gg, dgamma, None, (v if ctx.needs_input_grad[4] else None)     # dx = ... + carry: d/d(carry) is v itself
 
 
+def _vector_f32(t):
+    """a norm's weight or bias as the kernels read it: fp32, dense (the parameter itself where it is)"""
+    return t if t is None or (t.dtype == torch.float32 and t.is_contiguous()) else t.detach().float().contiguous()
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class LayerNormFn(Function):
     """layer norm over the last axis in one pass (gg_layernorm.h); backward: dx and the workgroups' sums of dw, db in one pass over x
     and dy, their total in a second launch. First order."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        w32, b32 = (None if t is None else t.detach().float().contiguous() for t in (weight, bias))
-        y, mean, rstd = K.layernorm_fwd(x, w32, b32, eps, any(ctx.needs_input_grad))
-        ctx.has_bias = bias is not None
+        y, stats = K.layernorm_fwd(x, _vector_f32(weight), _vector_f32(bias), eps, True)
         ctx.bias_dtype = None if bias is None else bias.dtype
-        if mean is not None:
-            ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.save_for_backward(x, weight, stats)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        dx, dw, db = K.layernorm_bwd(x, dy.to(x.dtype), weight.float().contiguous(), mean, rstd, ctx.has_bias)
-        return dx, dw.to(weight.dtype), (db.to(ctx.bias_dtype) if ctx.has_bias else None), None
+        x, weight, stats = ctx.saved_tensors
+        dx, dw, db = K.layernorm_bwd(x, dy if dy.dtype == x.dtype else dy.to(x.dtype), _vector_f32(weight), stats, ctx.bias_dtype is not None)
+        if dw.dtype != weight.dtype:
+            dw = dw.to(weight.dtype)
+        if db is not None and db.dtype != ctx.bias_dtype:
+            db = db.to(ctx.bias_dtype)
+        return dx, dw, db, None
 
 
 class RotaryFn(Function):
@@ -781,7 +791,7 @@ class RotaryFn(Function):
     @staticmethod
     def backward(ctx, *grads):
         positions, = ctx.saved_tensors
-        gq, gk = (None if g is None else g.to(dt) for g, dt in zip((*grads, None)[:2], ctx.dtypes))
+        gq, gk = (g if g is None or g.dtype == dt else g.to(dt) for g, dt in zip((*grads, None)[:2], ctx.dtypes))
         out = RotaryFn.apply(gq, gk, positions, ctx.spec, not ctx.inverse)
         dq, dk = (out, None) if gk is None else out
         return dq, dk, None, None, None
@@ -893,17 +903,15 @@ class WindowAttnFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, key_mask, scale, left, right, sinks):
         ctx.cfg = (scale, left, right, sinks)
-        train = any(ctx.needs_input_grad[:3])
-        o, lse = K.window_fwd(q, k, v, *ctx.cfg, lengths, key_mask, train)
-        if train:
-            ctx.save_for_backward(q, k, v, lengths, key_mask, o, lse)
+        o, lse = K.window_fwd(q, k, v, *ctx.cfg, lengths, key_mask, True)
+        ctx.save_for_backward(q, k, v, lengths, key_mask, o, lse)
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o):
         q, k, v, lengths, key_mask, o, lse = ctx.saved_tensors
-        dq, dk, dv = K.window_bwd(q, k, v, o, lse, d_o.to(q.dtype), *ctx.cfg, lengths, key_mask)
+        dq, dk, dv = K.window_bwd(q, k, v, o, lse, d_o if d_o.dtype == q.dtype else d_o.to(q.dtype), *ctx.cfg, lengths, key_mask)
         return dq, dk, dv, None, None, None, None, None, None
 
 
@@ -1996,7 +2004,9 @@ class HipOps:
             if m > 1 and key_mask.stride(1) != 1:
                 key_mask = key_mask.contiguous()
         K._same_device('window_attention', q, k, v, lengths, key_mask)
-        return WindowAttnFn.apply(q, k, v, lengths, key_mask, scale, left, right, sinks)
+        if _wants_grad(q, k, v):
+            return WindowAttnFn.apply(q, k, v, lengths, key_mask, scale, left, right, sinks)
+        return K.window_fwd(q, k, v, scale, left, right, sinks, lengths, key_mask, False)[0]
 
     def self_attention(self, q, k, v, null_kv, *, heads, scale, l2):
         """SelfAttention.forward after the projections (gp.py:562-592); q, k, v logical (b, heads*d, x, y)."""
@@ -2057,7 +2067,9 @@ class HipOps:
                 continue
             if t is None or tuple(t.shape) != (C,) or not t.is_floating_point():
                 raise ValueError(f'layer_norm: {name} must be a floating tensor of shape ({C},)')
-        return LayerNormFn.apply(x, weight, bias, float(eps))
+        if _wants_grad(x, weight, bias):
+            return LayerNormFn.apply(x, weight, bias, float(eps))
+        return K.layernorm_fwd(x, _vector_f32(weight), _vector_f32(bias), float(eps), False)[0]
 
     def rotary(self, q, positions, spec, k=None):
         """rotary positions with several axes: feature pair i of every head turns by positions[..., axis(i)] * freq(i).
@@ -2084,7 +2096,10 @@ class HipOps:
         if tuple(positions.shape) not in ((n, A), (B, n, A)):
             raise ValueError(f'rotary: positions of shape ({n}, {A}) or ({B}, {n}, {A}) expected, got {tuple(positions.shape)}')
         K._same_device('rotary', q, k, positions)
-        return RotaryFn.apply(q, k, positions.detach(), spec, False)
+        if _wants_grad(q, k):
+            return RotaryFn.apply(q, k, positions.detach(), spec, False)
+        out = K.rotary(q, k, positions, spec)
+        return out[0] if k is None else out
 
     # -- unet pieces (unet_upsampler.py) -----------------------------------------------------------------
     def maxpool_highfreq(self, x):
