@@ -126,6 +126,7 @@ class Discriminator(nn.Module):
         attn_dim_head=64,
         attn_heads=8,
         self_attn_dot_product=False,
+        self_attn_rotary=False,        # rotary positions (row, column) in the self-attention blocks
         ff_mult=4,
         text_encoder=None,
         text_dim=None,
@@ -225,7 +226,7 @@ class Discriminator(nn.Module):
                 resnet_block,
                 residual_conv,
                 SelfAttentionBlock(dim_out, heads=attn_heads, dim_head=attn_dim_head, ff_mult=ff_mult,
-                                   dot_product=self_attn_dot_product) if has_attn else None,
+                                   dot_product=self_attn_dot_product, rotary=self_attn_rotary) if has_attn else None,
                 predictor,
                 aux_decoder,
                 Downsample(dim_out) if should_downsample else None,

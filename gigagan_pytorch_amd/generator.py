@@ -53,6 +53,7 @@ class Generator(BaseGenerator):
         self_attn_heads=8,
         self_attn_dot_product=True,
         self_attn_ff_mult=4,
+        self_attn_rotary=False,        # rotary positions (row, column) in the self-attention blocks
         cross_attn_resolutions=(32, 16),
         cross_attn_dim_head=64,
         cross_attn_heads=8,
@@ -129,7 +130,8 @@ class Generator(BaseGenerator):
             self_attn = cross_attn = None
             if has_self_attn:
                 self_attn = SelfAttentionBlock(dim_out, dim_head=self_attn_dim_head, heads=self_attn_heads,
-                                               ff_mult=self_attn_ff_mult, dot_product=self_attn_dot_product)
+                                               ff_mult=self_attn_ff_mult, dot_product=self_attn_dot_product,
+                                               rotary=self_attn_rotary)
             if has_cross_attn:
                 cross_attn = CrossAttentionBlock(dim_out, dim_context=text_encoder.dim, dim_head=cross_attn_dim_head,
                                                  heads=cross_attn_heads, ff_mult=cross_attn_ff_mult)

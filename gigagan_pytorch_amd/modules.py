@@ -136,6 +136,26 @@ class RMSNorm(nn.Module):
         return (F.normalize(x.float(), dim=-1) * self.scale * self.gamma).to(x.dtype)
 
 
+class LayerNorm(nn.Module):
+    """layer norm over the last axis (mean and variance, weight and bias): the text transformer's `norm='layer'`"""
+
+    def __init__(self, dim, eps=1e-5):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dim))
+        self.bias = nn.Parameter(torch.zeros(dim))
+
+    def forward(self, x):
+        return ops.impl.layer_norm(x, self.weight, self.bias, self.eps)
+
+
+def token_norm(kind, dim):
+    """the norm of a token sequence: 'rms' (the reference's RMSNorm) or 'layer'"""
+    if kind not in ('rms', 'layer'):
+        raise ValueError(f"norm must be 'rms' or 'layer', got {kind!r}")
+    return RMSNorm(dim) if kind == 'rms' else LayerNorm(dim)
+
+
 # ---- resampling ---------------------------------------------------------------------------------------------
 
 class Blur(nn.Module):
@@ -286,8 +306,14 @@ def self_attention_unfused(impl, q, k, v, null_kv, heads, scale, l2):
 
 
 class SelfAttention(nn.Module):
-    def __init__(self, dim, dim_head=64, heads=8, dot_product=False):
+    """`rotary=True`: queries and keys turn with their pixel's row and column (half of a head's feature pairs each) before they meet; the
+    null key has no position."""
+
+    def __init__(self, dim, dim_head=64, heads=8, dot_product=False, rotary=False):
         super().__init__()
+        if rotary and dim_head % 4:
+            raise ValueError(f'SelfAttention: rotary positions need heads of a multiple of 4 features, got {dim_head}')
+        self.rotary = ops.RotarySpec((dim_head // 4, dim_head // 4)) if rotary else None
         self.heads = heads
         self.scale = dim_head ** -0.5
         dim_inner = dim_head * heads
@@ -317,8 +343,24 @@ class SelfAttention(nn.Module):
             q, fmap = self.to_q(fmap, fork=True)
             k = q
         v = self.to_v(fmap)
+        if exists(self.rotary):
+            q, k = self._turned(q, None if k is q else k)
         out = ops.impl.self_attention(q, k, v, self.null_kv, heads=h, scale=self.scale, l2=not self.dot_product)
         return self.to_out(out, residual=residual)
+
+
+    def _turned(self, q, k):
+        """q and k (b, heads * d, x, y) turned by their pixels' positions; k None: the keys are the queries"""
+        b, _, x, y = q.shape
+        positions = ops.grid_positions((x, y), q.device)
+
+        def fmap(t):
+            return t.transpose(1, 2).reshape(b, x, y, -1).permute(0, 3, 1, 2)
+        if k is None:
+            q = fmap(ops.impl.rotary(_heads(q, self.heads), positions, self.rotary))
+            return q, q
+        q, k = ops.impl.rotary(_heads(q, self.heads), positions, self.rotary, k=_heads(k, self.heads))
+        return fmap(q), fmap(k)
 
 
 class CrossAttention(nn.Module):
@@ -351,11 +393,11 @@ def _gelu(x):
     return ops.impl.gelu(x)
 
 
-def FeedForward(dim, mult=4, channel_first=False):
+def FeedForward(dim, mult=4, channel_first=False, norm='rms'):
     dim_hidden = int(dim * mult)
     if channel_first:
         return nn.Sequential(ChannelRMSNorm(dim), Conv2d(dim, dim_hidden, 1), Act(_gelu), Conv2d(dim_hidden, dim, 1))
-    return nn.Sequential(RMSNorm(dim), Linear(dim, dim_hidden), Act(_gelu), Linear(dim_hidden, dim))
+    return nn.Sequential(token_norm(norm, dim), Linear(dim, dim_hidden), Act(_gelu), Linear(dim_hidden, dim))
 
 
 def _ff_residual(ff, x):
@@ -371,9 +413,9 @@ def _ff_residual(ff, x):
 
 
 class SelfAttentionBlock(nn.Module):
-    def __init__(self, dim, dim_head=64, heads=8, ff_mult=4, dot_product=False):
+    def __init__(self, dim, dim_head=64, heads=8, ff_mult=4, dot_product=False, rotary=False):
         super().__init__()
-        self.attn = SelfAttention(dim=dim, dim_head=dim_head, heads=heads, dot_product=dot_product)
+        self.attn = SelfAttention(dim=dim, dim_head=dim_head, heads=heads, dot_product=dot_product, rotary=rotary)
         self.ff = FeedForward(dim=dim, mult=ff_mult, channel_first=True)
 
     def forward(self, x):
@@ -397,15 +439,23 @@ class CrossAttentionBlock(nn.Module):
 # ---- text transformer (gp.py:659-867) — small (77 tokens); config 4 ----------------------------------------------
 
 class TextAttention(nn.Module):
-    def __init__(self, dim, dim_head=64, heads=8):
+    """norm='layer': a layer norm in front instead of the reference's RMSNorm. rotary=True: queries and keys turn with their token's place
+    (the null key has none). window=w or (left, right): a token sees the tokens that far to its sides, the null key and the first
+    token, which in turn sees every token - the text encoder's learned global token stands there and gathers the caption."""
+
+    def __init__(self, dim, dim_head=64, heads=8, norm='rms', rotary=False, window=None):
         super().__init__()
         self.heads = heads
         self.scale = dim_head ** -0.5
         dim_inner = dim_head * heads
-        self.norm = RMSNorm(dim)
+        self.norm = token_norm(norm, dim)
         self.to_qkv = Linear(dim, dim_inner * 3, bias=False)
         self.null_kv = nn.Parameter(torch.randn(2, heads, dim_head))
         self.to_out = Linear(dim_inner, dim, bias=False)
+        if rotary and dim_head % 2:
+            raise ValueError(f'TextAttention: rotary positions need heads of an even number of features, got {dim_head}')
+        self.rotary = ops.RotarySpec((dim_head // 2,)) if rotary else None
+        self.window = (window, window) if isinstance(window, int) else window
 
     def forward(self, encodings, mask=None):
         b, n, _ = encodings.shape
@@ -413,23 +463,32 @@ class TextAttention(nn.Module):
         x = self.norm(encodings)
         q, k, v = self.to_qkv(x).chunk(3, dim=-1)
         q, k, v = (t.reshape(b, n, h, -1).transpose(1, 2) for t in (q, k, v))
+        if exists(self.rotary):
+            q, k = ops.impl.rotary(q, ops.grid_positions((n,), q.device), self.rotary, k=k)
         nk, nv = (t[None, :, None, :].expand(b, -1, -1, -1).to(q.dtype) for t in self.null_kv)
         k = torch.cat((nk, k), dim=2)
         v = torch.cat((nv, v), dim=2)
         if exists(mask):
             mask = F.pad(mask, (1, 0), value=True)
-        out = ops.impl.attention(q, k, v, scale=self.scale, l2=False, key_mask=mask)
+        if exists(self.window):
+            kw = dict(scale=self.scale, key_mask=mask)
+            first = ops.impl.window_attention(q[:, :, :1], k, v, **kw)
+            rest = ops.impl.window_attention(q[:, :, 1:], k, v, window=self.window, sinks=2, **kw)      # keys 0, 1: null, first token
+            out = torch.cat((first, rest), dim=2)
+        else:
+            out = ops.impl.attention(q, k, v, scale=self.scale, l2=False, key_mask=mask)
         out = out.transpose(1, 2).reshape(b, n, -1)
         return self.to_out(out)
 
 
 class Transformer(nn.Module):
-    def __init__(self, dim, depth, dim_head=64, heads=8, ff_mult=4):
+    def __init__(self, dim, depth, dim_head=64, heads=8, ff_mult=4, norm='rms', rotary=False, window=None):
         super().__init__()
         self.layers = nn.ModuleList([
-            nn.ModuleList([TextAttention(dim=dim, dim_head=dim_head, heads=heads), FeedForward(dim=dim, mult=ff_mult)])
+            nn.ModuleList([TextAttention(dim=dim, dim_head=dim_head, heads=heads, norm=norm, rotary=rotary, window=window),
+                           FeedForward(dim=dim, mult=ff_mult, norm=norm)])
             for _ in range(depth)])
-        self.norm = RMSNorm(dim)
+        self.norm = token_norm(norm, dim)
 
     def forward(self, x, mask=None):
         for attn, ff in self.layers:

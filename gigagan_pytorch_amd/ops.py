@@ -1414,6 +1414,17 @@ class ResampleFn(Function):
 # --------------------------------------------------------------------------------------------------
 _prepared: dict = {}        # id(weights) -> coefficients / per-sample weights computed by HipOps.modconv_prepare for the running forward
 
+def grid_positions(sizes, device):
+    """positions (n, axes) int32 of a grid's n points in raster order: sizes (n,) a sequence, (height, width) a map, (time, height, width)
+    a video"""
+    flat = torch.arange(math.prod(sizes), device=device, dtype=torch.int32)
+    cols, step = [], 1
+    for s in reversed(sizes):
+        cols.append(flat // step % s if step > 1 else flat % s)
+        step *= s
+    return torch.stack(cols[::-1], dim=-1)
+
+
 class HipOps:
     """MI355X implementation: HIP kernels for contractions/resampling, torch glue for pointwise pieces."""
 

@@ -14,7 +14,9 @@ from .modules import Linear, Transformer, exists
 
 
 class TextEncoder(nn.Module):
-    def __init__(self, *, dim, depth, clip=None, dim_head=64, heads=8, clip_dim_latent=512):
+    """norm, rotary, window: the transformer's options (modules.TextAttention); the defaults are the reference's encoder."""
+
+    def __init__(self, *, dim, depth, clip=None, dim_head=64, heads=8, clip_dim_latent=512, norm='rms', rotary=False, window=None):
         super().__init__()
         self.dim = dim
         self.clip = clip
@@ -24,7 +26,7 @@ class TextEncoder(nn.Module):
                 p.requires_grad = False
         self.learned_global_token = nn.Parameter(torch.randn(dim))
         self.project_in = Linear(dim_latent, dim) if dim_latent != dim else nn.Identity()
-        self.transformer = Transformer(dim=dim, depth=depth, dim_head=dim_head, heads=heads)
+        self.transformer = Transformer(dim=dim, depth=depth, dim_head=dim_head, heads=heads, norm=norm, rotary=rotary, window=window)
 
     def forward(self, texts=None, text_encodings=None):
         assert exists(texts) ^ exists(text_encodings)

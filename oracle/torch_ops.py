@@ -130,6 +130,44 @@ class OracleOps:
         """skip-layer excitation multiply `x * excite` (reference gp.py:1023-1024 generator, :1812-1813 discriminator)."""
         return x * s.reshape(x.shape[0], x.shape[1], 1, 1).to(x.dtype)
 
+    # the transformer options that the reference does not have: layer norm, rotary positions, attention with a window and sinks,
+    # restated from their definitions (no code shared with the product)
+    def layer_norm(self, x, weight, bias=None, eps=1e-5):
+        x = x.float()
+        c = x - x.mean(-1, keepdim=True)
+        y = c / (c.square().mean(-1, keepdim=True) + eps).sqrt() * weight.float()
+        return y if bias is None else y + bias.float()
+
+    def rotary(self, q, positions, spec, k=None):
+        pos = positions if positions.dim() == 3 else positions[None]
+        ang = (pos.double()[..., spec.axes] * torch.tensor(spec.freqs, dtype=torch.float64, device=pos.device))[:, None]
+        c, s = ang.cos().float(), ang.sin().float()
+
+        def turn(x):
+            x, p = x.float(), spec.pairs
+            r, rest = x[..., :2 * p], x[..., 2 * p:]
+            a, b = (r[..., 0::2], r[..., 1::2]) if spec.interleaved else (r[..., :p], r[..., p:])
+            a, b = a * c - b * s, a * s + b * c
+            r = torch.stack((a, b), -1).flatten(-2) if spec.interleaved else torch.cat((a, b), -1)
+            return torch.cat((r, rest), -1)
+        return turn(q) if k is None else (turn(q), turn(k))
+
+    def window_attention(self, q, k, v, *, scale, window=(None, None), sinks=0, key_mask=None, lengths=None):
+        B, h, n, d = q.shape
+        m = k.shape[2]
+        left, right = (n + m if t is None else t for t in window)
+        end = torch.full((B,), m, device=q.device) if lengths is None else lengths.long()
+        p = (end[:, None] - n + torch.arange(n, device=q.device))[:, :, None]
+        j = torch.arange(m, device=q.device)[None, None]
+        ok = (p >= 0) & (j < end[:, None, None]) & (j <= p + right) & ((j >= p - left) | (j < sinks))
+        if key_mask is not None:
+            ok = ok & key_mask[:, None]
+        q, k, v = (_r(t.float(), self.bf16) for t in (q, k, v))
+        k, v = (t.repeat_interleave(h // k.shape[1], 1) for t in (k, v))
+        sim = (q @ k.transpose(-1, -2) * scale).masked_fill(~ok[:, None], -torch.finfo(torch.float32).max)
+        attn = sim.softmax(-1) * ok[:, None]
+        return _r(attn, self.bf16) @ v
+
     # nn.GELU() in FeedForward, gp.py:731 (exact erf form)
     def gelu(self, x):
         return F.gelu(x.float())
