@@ -70,8 +70,8 @@ class RotaryDesc(C.Structure):       # mirrors gg_rotary_desc
 
 class WindowDesc(C.Structure):       # mirrors gg_window_desc
     _fields_ = [
-        ('q', C.c_void_p), ('k', C.c_void_p), ('v', C.c_void_p), ('o', C.c_void_p), ('lse', C.c_void_p),
-        ('d_o', C.c_void_p), ('dq', C.c_void_p), ('dk', C.c_void_p), ('dv', C.c_void_p), ('dvec', C.c_void_p),
+        ('q', C.c_void_p), ('k', C.c_void_p), ('v', C.c_void_p), ('o', C.c_void_p), ('o_lo', C.c_void_p),
+        ('lse', C.c_void_p), ('d_o', C.c_void_p), ('dq', C.c_void_p), ('dk', C.c_void_p), ('dv', C.c_void_p), ('dvec', C.c_void_p),
         ('q_strides', C.c_int64 * 3), ('k_strides', C.c_int64 * 3), ('v_strides', C.c_int64 * 3), ('g_strides', C.c_int64 * 3),
         ('lengths', C.c_void_p), ('key_mask', C.c_void_p), ('mask_stride', C.c_int64),
         ('B', C.c_int32), ('n', C.c_int32), ('m', C.c_int32), ('h', C.c_int32), ('hk', C.c_int32), ('d', C.c_int32),

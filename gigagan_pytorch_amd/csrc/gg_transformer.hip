@@ -177,7 +177,7 @@ static int gg_win_check(const char* who, const gg_window_desc* d, GgWinParams& p
     if (d->sinks < 0) return gg_fail(-3, "%s: negative sinks", who);
     const long long g = d->h / d->hk;
     if (d->m > (1 << 28) || (long long)d->n * g > (1 << 30)) return gg_fail(-2, "%s: more than 2^28 keys or 2^30 rows a head", who);
-    const void* ptrs[] = {d->q, d->k, d->v, d->o, d->d_o, d->dq, d->dk, d->dv};
+    const void* ptrs[] = {d->q, d->k, d->v, d->o, d->o_lo, d->d_o, d->dq, d->dk, d->dv};
     for (const void* x : ptrs)
         if ((unsigned long long)x & 15) return gg_fail(-4, "%s: operands must be 16-byte aligned", who);
     const int64_t* strides[] = {d->q_strides, d->k_strides, d->v_strides, d->d_o ? d->g_strides : d->q_strides};
@@ -193,7 +193,7 @@ static int gg_win_check(const char* who, const gg_window_desc* d, GgWinParams& p
     memset(&p, 0, sizeof(p));
     p.q = (const unsigned short*)d->q; p.k = (const unsigned short*)d->k; p.v = (const unsigned short*)d->v;
     p.d_o = (const unsigned short*)d->d_o;
-    p.o = (unsigned short*)d->o; p.dq = (unsigned short*)d->dq; p.dk = (unsigned short*)d->dk; p.dv = (unsigned short*)d->dv;
+    p.o = (unsigned short*)d->o; p.o_lo = (unsigned short*)d->o_lo; p.dq = (unsigned short*)d->dq; p.dk = (unsigned short*)d->dk; p.dv = (unsigned short*)d->dv;
     p.lse = d->lse; p.dvec = d->dvec;
     p.qb = d->q_strides[0]; p.qh = d->q_strides[1]; p.qn = (unsigned)d->q_strides[2];
     p.kb = d->k_strides[0]; p.kh = d->k_strides[1]; p.kn = (unsigned)d->k_strides[2];
@@ -251,7 +251,7 @@ extern "C" int gg_window_bwd(const gg_window_desc* d, void* workspace, size_t wo
     GgWinParams p;
     int rc = gg_win_check("gg_window_bwd", d, p);
     if (rc) return rc;
-    if (!d->d_o || !d->dq || !d->dk || !d->dv || !d->lse || !d->dvec) return gg_fail(-1, "gg_window_bwd: null pointer");
+    if (!d->o_lo || !d->d_o || !d->dq || !d->dk || !d->dv || !d->lse || !d->dvec) return gg_fail(-1, "gg_window_bwd: null pointer");
     const GgWinPlan w = gg_win_plan(d);
     if (w.bwd_bytes && (!workspace || workspace_bytes < w.bwd_bytes || ((unsigned long long)workspace & 15)))
         return gg_fail(-5, "gg_window_bwd: needs %zu workspace bytes, 16-byte aligned", w.bwd_bytes);

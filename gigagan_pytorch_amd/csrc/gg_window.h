@@ -29,7 +29,7 @@
 
 struct GgWinParams {
     const unsigned short *q, *k, *v, *d_o;
-    unsigned short *o, *dq, *dk, *dv;       // dense: o, dq [B][n][h][D]; dk, dv [B][m][hk][D]
+    unsigned short *o, *o_lo, *dq, *dk, *dv;        // dense: o, o_lo, dq [B][n][h][D]; dk, dv [B][m][hk][D]
     float* lse;                             // [B*hk][n*g]: log2 of the row's sum of 2^(scale log2e s); +inf for a row that sees nothing
     float* dvec;                            // [B*hk][n*g]: D_i
     long long qb, qh, kb, kh, vb, vh, gb, gh;       // element strides of q, k, v, dO: batch, head ...
@@ -289,6 +289,19 @@ GG_DEVICE void ggw_softmax(f32x16* st, u16x8* pf, f32x16* ot, float& m, float& l
 #pragma unroll
     for (int jc = 0; jc < 2 * N; ++jc) pf[jc] = ggw_pack8<T>(st[jc >> 1], jc & 1);
 }
+// four features of o; o_lo (training): what the rounding took off, for D (a row of few keys has dP close to D, and half a step of o in
+// D is then as large as their difference)
+template <int T>
+GG_DEVICE void ggw_store_o(const GgWinParams& p, long long at, f32x4 x) {
+    u16x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hi[e] = gg_elt<T>(x[e]);
+        lo[e] = gg_elt<T>(x[e] - gg_elt_f<T>(hi[e]));
+    }
+    *(u16x4*)(p.o + at) = hi;
+    if (p.o_lo) *(u16x4*)(p.o_lo + at) = lo;
+}
 // the wave's 32 rows: o and the log-sum-exp, or (SPLIT) what gg_win_join_kernel takes
 template <int T, int D, bool SPLIT>
 GG_DEVICE void ggw_write_rows(const GgWinParams& p, const GgwWave& w, int bkv, int split, const f32x16* ot, float m, float l) {
@@ -309,16 +322,12 @@ GG_DEVICE void ggw_write_rows(const GgWinParams& p, const GgwWave& w, int bkv, i
     }
     const int b = bkv / p.hk, kvh = bkv - b * p.hk;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    unsigned short* orow = p.o + (((long long)b * p.n + w.row.token) * p.h + kvh * p.g + w.row.head) * D;
+    const long long orow = (((long long)b * p.n + w.row.token) * p.h + kvh * p.g + w.row.head) * D;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-        for (int gq = 0; gq < 4; ++gq) {
-            u16x4 o4;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o4[e] = gg_elt<T>(ot[db][4 * gq + e] * inv);
-            *(u16x4*)(orow + db * 32 + 8 * gq + 4 * hi) = o4;
-        }
+        for (int gq = 0; gq < 4; ++gq)
+            ggw_store_o<T>(p, orow + db * 32 + 8 * gq + 4 * hi, f32x4{ot[db][4 * gq] * inv, ot[db][4 * gq + 1] * inv, ot[db][4 * gq + 2] * inv, ot[db][4 * gq + 3] * inv});
     if (hi == 0 && p.lse) p.lse[at] = l == 0.f ? __builtin_inff() : m + log2f(l);
 }
 template <int KK>
@@ -586,10 +595,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_few_kernel(GgWinParams p) {
         } else {
             const float inv = lt == 0.f ? 0.f : 1.f / lt;
             const int token = (int)((unsigned)r / (unsigned)p.g), head = r - token * p.g;
-            u16x4 o4;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o4[e] = gg_elt<T>(x[e] * inv);
-            *(u16x4*)(p.o + (((long long)b * p.n + token) * p.h + kvh * p.g + head) * D + d) = o4;
+            ggw_store_o<T>(p, (((long long)b * p.n + token) * p.h + kvh * p.g + head) * D + d, x * inv);
             if (d == 0 && p.lse) p.lse[at] = lt == 0.f ? __builtin_inff() : mt + log2f(lt);
         }
     }
@@ -634,10 +640,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_join_kernel(GgWinParams p) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int bkv = (int)(at / rows), r = (int)(at - (long long)bkv * rows);
     const int b = bkv / p.hk, kvh = bkv - b * p.hk, token = r / p.g, head = r - token * p.g;
-    u16x4 o4;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o4[e] = gg_elt<T>(x[e] * inv);
-    *(u16x4*)(p.o + (((long long)b * p.n + token) * p.h + kvh * p.g + head) * D + d) = o4;
+    ggw_store_o<T>(p, (((long long)b * p.n + token) * p.h + kvh * p.g + head) * D + d, x * inv);
     if (d == 0 && p.lse) p.lse[at] = l == 0.f ? __builtin_inff() : top + log2f(l);
 }
 
@@ -724,9 +727,9 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dq_kernel(GgWinParams p) {
     ggw_load_row<KK>(gf, p.d_o + b * p.gb, p.gh, p.gn, hq, w.row.token);
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-        const u16x8 of = *(const u16x8*)(p.o + orow + 8 * hi + kk * 16);
+        const u16x8 of = *(const u16x8*)(p.o + orow + 8 * hi + kk * 16), ol = *(const u16x8*)(p.o_lo + orow + 8 * hi + kk * 16);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) dsum += gg_elt_f<T>(gf[kk][e]) * gg_elt_f<T>(of[e]);
+        for (int e = 0; e < 8; ++e) dsum = gg_fmaf(gg_elt_f<T>(gf[kk][e]), gg_elt_f<T>(of[e]) + gg_elt_f<T>(ol[e]), dsum);
     }
     dsum = gg_sum_xor32(dsum);
     const float lse = p.lse[at], a2 = p.scale * GGW_LOG2E;

@@ -1553,42 +1553,44 @@ def _attend4(t: torch.Tensor, group: int = 0) -> torch.Tensor:
     return t if ok else t.transpose(1, 2).clone(memory_format=torch.contiguous_format).transpose(1, 2)
 
 
-_WINDOW_PACK = struct.Struct('@10P12q2Pq10ifi').pack         # gg_window_desc (a packed string costs a fifth of a ctypes structure)
+_WINDOW_PACK = struct.Struct('@11P12q2Pq10ifi').pack         # gg_window_desc (a packed string costs a fifth of a ctypes structure)
 
 
-def _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask, d_o=None, dq=None, dk=None, dv=None, dvec=None):
+def _window_desc(q, k, v, o, o_lo, lse, scale, left, right, sinks, lengths, key_mask, d_o=None, dq=None, dk=None, dv=None, dvec=None):
     B, h, n, d = q.shape
-    return _WINDOW_PACK(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ptr(lse) or 0, ptr(d_o) or 0, ptr(dq) or 0, ptr(dk) or 0,
+    return _WINDOW_PACK(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ptr(o_lo) or 0, ptr(lse) or 0, ptr(d_o) or 0, ptr(dq) or 0, ptr(dk) or 0,
                         ptr(dv) or 0, ptr(dvec) or 0, *_strides3(q), *_strides3(k), *_strides3(v), *((0, 0, 0) if d_o is None else _strides3(d_o)),
                         ptr(lengths) or 0, ptr(key_mask) or 0, 0 if key_mask is None or B == 1 else key_mask.stride(0), B, n, k.shape[2], h,
                         k.shape[1], d, left, right, sinks, _ROW_TYPES[q.dtype], scale, 0)
 
 
-def window_fwd(q, k, v, scale: float, left: int, right: int, sinks: int, lengths, key_mask, want_lse: bool):
+def window_fwd(q, k, v, scale: float, left: int, right: int, sinks: int, lengths, key_mask, train: bool):
     """q (B, h, n, d), k, v (B, hk, m, d) bf16 / fp16; lengths (B,) int32, key_mask (B, m) bool, both optional; left / right -1 = no
-    bound -> (o as a (B, h, n, d) view of dense (B, n, h, d) storage, lse (B * hk, n * h / hk) fp32 in the log2 domain or None)."""
+    bound -> (o as a (B, h, n, d) view of dense (B, n, h, d) storage; for the backward (train), else None: o_lo, dense, what o's rounding
+    took off, and lse (B * hk, n * h / hk) fp32 in the log2 domain)."""
     L = _C.lib()
     L.require(q, k, v, lengths, key_mask)
     B, h, n, d = q.shape
     o = torch.empty((B, n, h, d), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B * k.shape[1], n * (h // k.shape[1])), dtype=torch.float32, device=q.device) if want_lse else None
+    o_lo = torch.empty_like(o) if train else None
+    lse = torch.empty((B * k.shape[1], n * (h // k.shape[1])), dtype=torch.float32, device=q.device) if train else None
     if not o.numel():
-        return o.transpose(1, 2), lse
+        return o.transpose(1, 2), o_lo, lse
     if not k.shape[2]:
-        return o.zero_().transpose(1, 2), (lse.fill_(math.inf) if want_lse else None)
+        return o.zero_().transpose(1, 2), (o_lo.zero_() if train else None), (lse.fill_(math.inf) if train else None)
     q, k, v = _attend4(q, h // k.shape[1]), _attend4(k), _attend4(v)
-    D = _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask)
+    D = _window_desc(q, k, v, o, o_lo, lse, scale, left, right, sinks, lengths, key_mask)
     with _on_device(L, q):
         nbytes = L.lib.gg_window_workspace_bytes(D, 0)
         ws = _workspace(nbytes, q) if nbytes else None
         rc = L.lib.gg_window_fwd(D, ptr(ws), nbytes, L.stream(q))
     L.check(rc, 'gg_window_fwd')
-    return o.transpose(1, 2), lse
+    return o.transpose(1, 2), o_lo, lse
 
 
-def window_bwd(q, k, v, o, lse, d_o, scale: float, left: int, right: int, sinks: int, lengths, key_mask):
-    """-> dq (B, h, n, d), dk, dv (B, hk, m, d) in the operands' type, as views of dense token-major storage; `o`, `lse` as window_fwd
-    returned them, d_o (B, h, n, d) with any strides."""
+def window_bwd(q, k, v, o, o_lo, lse, d_o, scale: float, left: int, right: int, sinks: int, lengths, key_mask):
+    """-> dq (B, h, n, d), dk, dv (B, hk, m, d) in the operands' type, as views of dense token-major storage; `o`, `o_lo`, `lse` as
+    window_fwd returned them, d_o (B, h, n, d) with any strides."""
     L = _C.lib()
     L.require(q, k, v, o, lse, d_o, lengths, key_mask)
     assert d_o.dtype == q.dtype and d_o.shape == q.shape
@@ -1603,7 +1605,7 @@ def window_bwd(q, k, v, o, lse, d_o, scale: float, left: int, right: int, sinks:
         return views
     q, k, v, d_o = _attend4(q, h // hk), _attend4(k), _attend4(v), _attend4(d_o, h // hk)
     dvec = torch.empty_like(lse)
-    D = _window_desc(q, k, v, o, lse, scale, left, right, sinks, lengths, key_mask, d_o, dq, dk, dv, dvec)
+    D = _window_desc(q, k, v, o, o_lo, lse, scale, left, right, sinks, lengths, key_mask, d_o, dq, dk, dv, dvec)
     with _on_device(L, q):
         nbytes = L.lib.gg_window_workspace_bytes(D, 1)
         ws = _workspace(nbytes, q) if nbytes else None

@@ -897,21 +897,22 @@ class FlashAttnGenFn(Function):
 
 
 class WindowAttnFn(Function):
-    """attention with a sliding window and sinks (gg_window.h): forward saves o and the rows' log-sum-exp, backward is two kernels (dq;
+    """attention with a sliding window and sinks (gg_window.h): forward saves o, the rest that its rounding took off, and the
+    rows' log-sum-exp, backward is two kernels (dq;
     dk and dv, summed over the query heads of a shared key head) that recompute P. First order."""
 
     @staticmethod
     def forward(ctx, q, k, v, lengths, key_mask, scale, left, right, sinks):
         ctx.cfg = (scale, left, right, sinks)
-        o, lse = K.window_fwd(q, k, v, *ctx.cfg, lengths, key_mask, True)
-        ctx.save_for_backward(q, k, v, lengths, key_mask, o, lse)
+        o, o_lo, lse = K.window_fwd(q, k, v, *ctx.cfg, lengths, key_mask, True)
+        ctx.save_for_backward(q, k, v, lengths, key_mask, o, o_lo, lse)
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o):
-        q, k, v, lengths, key_mask, o, lse = ctx.saved_tensors
-        dq, dk, dv = K.window_bwd(q, k, v, o, lse, d_o if d_o.dtype == q.dtype else d_o.to(q.dtype), *ctx.cfg, lengths, key_mask)
+        q, k, v, lengths, key_mask, o, o_lo, lse = ctx.saved_tensors
+        dq, dk, dv = K.window_bwd(q, k, v, o, o_lo, lse, d_o if d_o.dtype == q.dtype else d_o.to(q.dtype), *ctx.cfg, lengths, key_mask)
         return dq, dk, dv, None, None, None, None, None, None
 
 
