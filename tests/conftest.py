@@ -71,7 +71,7 @@ def _bind_library(request):
 @pytest.fixture
 def reference():
     """the unmodified reference package, importable only where /root/reference exists (not on the GPU box)."""
-    if not REFERENCE.exists():
+    if not (REFERENCE / 'gigagan_pytorch').exists():
         pytest.skip('/root/reference not present')
     stubs = str(ROOT / 'tests' / 'oracle_stubs')
     for p in (str(REFERENCE), stubs):
