@@ -128,7 +128,7 @@ extern "C" int gg_rotary(const gg_rotary_desc* d, void* stream) {
 struct GgWinPlan {
     bool few;                   // rows fit one 32-row tile: gg_win_few_kernel
     int row_tiles, splits, join;        // forward
-    int key_tiles, sink_tiles, sink_chunks;     // dk / dv
+    int key_tiles, sink_tiles, sink_chunks;     // dk / dv: the first sink_tiles have their rows cut into sink_chunks
     size_t fwd_bytes, bwd_bytes;
 };
 
@@ -145,7 +145,8 @@ static GgWinPlan gg_win_plan(const gg_window_desc* d) {
     long long span = left + right + (rows < tr ? rows : tr) / g + 1 + sinks;
     if (span > d->m) span = d->m;
     const long long tiles = (span + tk - 1) / tk;
-    // split the keys where the row tiles alone do not fill the 256 CUs twice over, down to two key tiles a wave
+    // split the keys where the row tiles alone do not fill the 256 CUs twice over, down to two key tiles a wave (one token, 8192 keys, two
+    // key heads: 7.4 us and 4.4 for the join)
     const long long blocks = heads * w.row_tiles, least = w.few ? 8 : 4;
     long long s = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks;
     if (s > tiles / least) s = tiles / least;
@@ -159,8 +160,18 @@ static GgWinPlan gg_win_plan(const gg_window_desc* d) {
     w.sink_tiles = (int)((sinks + 127) / 128);
     // the rows that an ordinary key tile sees set the size of a sink tile's chunks
     long long seen = (left + right + 128) * g;
-    if (seen < 512) seen = 512;
-    long long c = w.sink_tiles ? rows / seen : 1;
+    if (seen > rows) seen = rows;
+    long long c = w.sink_tiles ? rows / (seen < 512 ? 512 : seen) : 1;
+    // too few key tiles for the chip: every tile's rows are cut, down to two row tiles a workgroup (66 tiles of 11 row tiles: 44 us whole,
+    // 28 and 4 us in five chunks and their sum; 32 of 64: causal training of 4096 tokens 246 -> 188 us a pass)
+    const long long tiles_kv = heads * w.key_tiles;
+    if (tiles_kv < 256) {
+        const long long most = (seen + 127) / 128, want = (511 + tiles_kv) / tiles_kv, cut = want < most ? want : most;
+        if (cut > 1) {
+            w.sink_tiles = w.key_tiles;
+            if (c < cut) c = cut;
+        }
+    }
     if (c > 64) c = 64;
     w.sink_chunks = (int)(c < 1 ? 1 : c);
     w.bwd_bytes = w.sink_chunks > 1 ? (size_t)heads * w.sink_tiles * w.sink_chunks * 2 * 128 * d->d * sizeof(float) : 0;

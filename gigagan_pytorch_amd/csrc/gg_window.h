@@ -44,7 +44,7 @@ struct GgWinParams {
     float scale;
     int splits, join;                       // ... and the thread groups that join a row's splits
     int row_tiles;                          // row (dk / dv: key) tiles per (batch, key head)
-    int sink_tiles, sink_chunks;            // dk / dv: key tiles that hold sinks, and the row chunks each of them is split into
+    int sink_tiles, sink_chunks;            // dk / dv: the first key tiles (those that hold sinks; all, where there are few), each in row chunks
 };
 
 // ---- shared pieces -----------------------------------------------------------------------------------------------
@@ -414,9 +414,9 @@ GG_DEVICE void ggw_fix_rows(const GgWinParams& p, const GgwWave& w, const GgwRan
 
 // workgroup: 4 waves x 32 rows; key tiles of 64 fetched once for all of them by LDS-DMA, double buffered: one barrier a tile, behind
 // which the next tile's transfers start and run under this tile's arithmetic. What bounds it is the LDS: every product takes a kilobyte
-// operand from it (attend-long without those reads 1515 of 2145 us, without the softmax 1751, without the transfers 1875). Measured and
-// not kept: two 32-row blocks a wave for each operand read (half the reads, but one wave a SIMD: 2604), eight waves a tile in two
-// groups half a tile apart (2330), wave priorities (no change).
+// operand from it (32768 tokens, window 4096, 32 heads on 8 of 128: without those reads 1515 of 2145 us, without the softmax 1751, without the transfers 1875). Measured and
+// not kept: two 32-row blocks a wave for each operand read (half the reads, but one wave a SIMD: 2604 against 2010 in the same run),
+// eight waves a tile in two groups half a tile apart (2334 against 2114), wave priorities (no change).
 // SPLIT: the tiles are dealt out to p.splits workgroups, which leave (m, l, O) for gg_win_join_kernel.
 template <int T, int D, bool SPLIT>
 GG_KERNEL GG_LAUNCH_BOUNDS2(256, D == 128 ? 2 : 3) void gg_win_fwd_kernel(GgWinParams p) {
@@ -487,7 +487,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, D == 128 ? 2 : 3) void gg_win_fwd_kernel(GgWinP
 // One new token: a handful of rows against a long cache - bound by reading K and V once. The four waves share the 32 rows and take key
 // tiles of 32 in turn, each on its own: K goes from memory straight into the score product's operand registers, V through a wave-private
 // LDS tile (the transpose read), no barrier in the loop; the waves' (m, l, O) are joined in LDS at the end, the splits' by
-// gg_win_join_kernel.
+// gg_win_join_kernel. 64 sequences, 8 key heads of 128, window 4096: 199 us (5.2 TB/s).
 template <int T, int D>
 GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_few_kernel(GgWinParams p) {
     constexpr int KK = D / 16, DB = D / 32;
@@ -795,7 +795,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dq_kernel(GgWinParams p) {
 
 // ---- backward, part 2: dk, dv -----------------------------------------------------------------------------------------
 // workgroup: 4 waves x 32 keys, row tiles of 64 (Q and dO by LDS-DMA, double buffered, each read as rows and transposed). The key tiles that hold sinks are seen by
-// every later row: their rows are cut into p.sink_chunks chunks, each a workgroup of its own that leaves fp32 sums for
+// every later row (and where there are few key tiles, every one): their rows are cut into p.sink_chunks chunks, each a workgroup of its own that leaves fp32 sums for
 // gg_win_sink_kernel.  part_o: [B*hk][sink_tiles][chunks][2][128][D].
 // one key's dk and dv again, by one wave, from the rows ra .. rb that see it alone: fix[2 D] = sum of dS q, sum of P dO
 template <int T, int D>
