@@ -9,6 +9,9 @@
 
 #include <string.h>
 
+// a launch holds fewer than 2^32 threads along an axis
+static bool gg_grid_fits(long long blocks, int threads) { return blocks <= 0xffffffffll / threads; }
+
 // ---- layer norm ------------------------------------------------------------------------------------------------
 
 static int gg_ln_check(const char* who, const void* x, int64_t ldx, const float* w, int64_t rows, int32_t C, int32_t dtype) {
@@ -39,7 +42,7 @@ extern "C" int gg_layernorm_fwd(const void* x, int64_t ldx, const float* w, cons
     p.x = x; p.ldx = ldx; p.w = w; p.b = b; p.y = y; p.mean = mean; p.rstd = rstd; p.rows = rows; p.C = C; p.eps = eps;
 #define GG_LN_GO(TPR, NV)                                                                                                    \
     const long long rpb = TPR > 256 ? 1 : 256 / TPR, blocks = (rows + rpb - 1) / rpb;                                        \
-    if (blocks > 0x7fffffffll) return gg_fail(-2, "gg_layernorm_fwd: too many rows");                                        \
+    if (!gg_grid_fits(blocks, TPR > 256 ? TPR : 256)) return gg_fail(-2, "gg_layernorm_fwd: too many rows");                  \
     const dim3 grid((unsigned)blocks), block(TPR > 256 ? TPR : 256);                                                         \
     if (dtype == GG_ELT_BF16) GG_LAUNCH((gg_layernorm_fwd_kernel<GG_ELT_BF16, TPR, NV>), grid, block, (hipStream_t)stream, p);     \
     else if (dtype == GG_ELT_F16) GG_LAUNCH((gg_layernorm_fwd_kernel<GG_ELT_F16, TPR, NV>), grid, block, (hipStream_t)stream, p);  \
@@ -115,7 +118,7 @@ extern "C" int gg_rotary(const gg_rotary_desc* d, void* stream) {
     if (tb > fill) tb = fill;
     p.tb = (int)(tb < 1 ? 1 : tb);
     const long long grid = (long long)d->B * ((d->n + p.tb - 1) / p.tb);
-    if (grid > 0x7fffffffll) return gg_fail(-2, "gg_rotary: too many tokens");
+    if (!gg_grid_fits(grid, 256)) return gg_fail(-2, "gg_rotary: too many tokens");
     if (d->dtype == GG_ELT_BF16) GG_LAUNCH(gg_rotary_kernel<GG_ELT_BF16>, dim3((unsigned)grid), dim3(256), (hipStream_t)stream, p);
     else if (d->dtype == GG_ELT_F16) GG_LAUNCH(gg_rotary_kernel<GG_ELT_F16>, dim3((unsigned)grid), dim3(256), (hipStream_t)stream, p);
     else GG_LAUNCH(gg_rotary_kernel<GG_ELT_F32>, dim3((unsigned)grid), dim3(256), (hipStream_t)stream, p);
@@ -244,7 +247,7 @@ extern "C" int gg_window_fwd(const gg_window_desc* d, void* workspace, size_t wo
         p.part_ml = p.part_o + (long long)w.splits * all * d->d;
     }
     const long long grid = (long long)p.B * p.hk * w.row_tiles * w.splits;
-    if (grid > 0x7fffffffll || all * w.join / (1024 / d->d) >= 0x7fffffffll) return gg_fail(-2, "gg_window_fwd: too many rows");
+    if (!gg_grid_fits(grid, 256) || (w.splits > 1 && !gg_grid_fits(all * w.join / (1024 / d->d) + 1, 256))) return gg_fail(-2, "gg_window_fwd: too many rows");
     hipStream_t s = (hipStream_t)stream;
 #define GG_WIN_GO(T, D)                                                                                                       \
     if (w.few) GG_LAUNCH((gg_win_few_kernel<T, D>), dim3((unsigned)grid), dim3(256), s, p);                                     \
@@ -269,7 +272,8 @@ extern "C" int gg_window_bwd(const gg_window_desc* d, void* workspace, size_t wo
     const long long rows = (long long)p.n * p.g, heads = (long long)p.B * p.hk;
     const long long dq_tiles = (rows + 127) / 128, dq_grid = heads * dq_tiles;
     const long long kv_grid = heads * ((long long)w.sink_tiles * w.sink_chunks + w.key_tiles - w.sink_tiles);
-    if (dq_grid > 0x7fffffffll || kv_grid > 0x7fffffffll) return gg_fail(-2, "gg_window_bwd: too many rows");
+    if (!gg_grid_fits(dq_grid, 256) || !gg_grid_fits(kv_grid, 256) 
+        || (w.sink_chunks > 1 && !gg_grid_fits(heads * w.sink_tiles * (d->d / 8), 256))) return gg_fail(-2, "gg_window_bwd: too many rows");
     hipStream_t s = (hipStream_t)stream;
     p.part_o = (float*)workspace;
 #define GG_WIN_GO(T, D)                                                                                                       \

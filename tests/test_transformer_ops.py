@@ -562,6 +562,43 @@ def test_window_attention_nan_reaches_only_who_sees_it(where):
             assert torch.equal(dq[0][others], gc[0][0][others])
 
 
+# what the key tiles' row chunks can be: only the sinks' tiles are cut (256 key tiles or more, many rows), one and two such tiles, grouped
+# heads; every tile is cut; none is
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+@pytest.mark.parametrize('case', [(4, 8, 8, 1100, 1100, 32, (40, 0), 3), (10, 4, 4, 1100, 1200, 64, (30, 20), 130),
+                                  (8, 8, 4, 1100, 1100, 128, (40, 0), 3), (1, 3, 1, 700, 1500, 128, (600, 0), 2),
+                                  (16, 4, 4, 600, 600, 64, (100, 100), 0)])
+def test_window_attention_row_chunks(case, dtype):
+    att_run('cuda', case, dtype)
+
+
+@where
+@pytest.mark.parametrize('window', [(None, 0), (150, 0)])
+def test_window_attention_nan_and_row_chunks(where, window):
+    """300 rows, cut into chunks: a NaN query or gradient of a middle chunk reaches the keys that it sees, through the chunks' sum, and no
+    other key; bits are the same every time"""
+    g = gen(15, where)
+    n, at = 300, 200
+    q, k, v, do = qkv(1, 2, 1, n, n, 32, 'bf16', g)
+    ok = seen(1, n, n, window, 0, None, None, where)
+    exact = att_ref(q, k, v, 0.2, ok, do)
+    sees = ok[0, at]
+    for spoil in ('q', 'do'):
+        q2, do2 = q.clone(), do.clone()
+        (q2 if spoil == 'q' else do2)[0, 1, at, 7] = math.nan
+        runs = []
+        for _ in range(2):
+            leaves = [t.detach().requires_grad_() for t in (q2, k, v)]
+            o = ops.impl.window_attention(*leaves, scale=0.2, window=window)
+            runs.append(torch.autograd.grad(o, leaves, do2))
+        for got, (ref, tol) in ((runs[0][1], exact[2]), (runs[0][2], exact[3])):
+            within(got[:, :, ~sees], ref[:, :, ~sees], tol[:, :, ~sees], spoil)
+            assert not torch.isfinite(got[:, :, sees, 7]).any()
+        for a, b in zip(*runs):
+            assert torch.equal(torch.nan_to_num(a), torch.nan_to_num(b))
+
+
 @where
 def test_window_attention_nothing_to_see(where):
     """no queries, no keys, no batch"""
@@ -658,3 +695,25 @@ def test_c_entry_refusals():
     w.hk = 3
     assert L.gg_window_bwd(C.byref(w), None, 0, None) == -1
     assert b'gg_window_bwd' in L.gg_last_error()
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """a launch holds fewer than 2^32 threads: larger calls end in an error, before anything runs"""
+    import ctypes as C
+    from gigagan_pytorch_amd import _C
+    L = _C.lib().lib
+    t = torch.zeros(4096)
+    p = t.data_ptr()
+    assert L.gg_layernorm_fwd(p, 8, p, p, p, None, None, 1 << 31, 8, 1e-5, 0, None) == -2
+    assert b'too many rows' in L.gg_last_error()
+    spec = ops.RotarySpec((2, 2))
+    d = _C.RotaryDesc(q=p, yq=p, positions=p, freqs=C.addressof(spec._freqs), axes=C.addressof(spec._axes), B=1 << 15, n=1 << 15, hq=1024, d=8,
+                      pairs=4, n_axes=2)
+    assert L.gg_rotary(C.byref(d), None) == -2
+    assert b'too many tokens' in L.gg_last_error()
+    w = _C.WindowDesc(q=p, k=p, v=p, o=p, o_lo=p, lse=p, d_o=p, dq=p, dk=p, dv=p, dvec=p, B=1 << 12, n=1 << 20, m=128, h=1, hk=1, d=64,
+                      left=-1, right=-1, scale=1.0)
+    assert L.gg_window_fwd(C.byref(w), None, 0, None) == -2
+    assert b'too many rows' in L.gg_last_error()
+    assert L.gg_window_bwd(C.byref(w), None, 0, None) == -2
+    assert b'too many rows' in L.gg_last_error()
