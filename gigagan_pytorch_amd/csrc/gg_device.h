@@ -19,7 +19,6 @@
 #define GG_DEVICE __device__ __forceinline__
 #define GG_HOST_DEVICE __host__ __device__ __forceinline__
 #define GG_KERNEL __global__
-#define GG_NOINLINE __device__ __attribute__((noinline))      // a rare path whose registers must not weigh on the kernel that calls it
 #define GG_SHARED __shared__
 #define GG_LAUNCH_BOUNDS(n) __launch_bounds__(n)
 #define GG_LAUNCH_BOUNDS2(n, waves_per_simd) __launch_bounds__(n, waves_per_simd)   // caps the register allocation for that occupancy

@@ -15,7 +15,6 @@
 #define GG_DEVICE static inline
 #define GG_HOST_DEVICE static inline
 #define GG_KERNEL static
-#define GG_NOINLINE static __attribute__((noinline))
 #define GG_SHARED static
 #define GG_LAUNCH_BOUNDS(n)
 #define GG_LAUNCH_BOUNDS2(n, w)
