@@ -2313,3 +2313,8 @@ extern "C" int gg_comm_destroy(void) {
     gg_comm::g_rank = -1;
     return rc;
 }
+
+// The recipes compile gg_transformer.hip as a unit of its own beside this one (GG_UNITS); without it this file alone is the whole library.
+#ifndef GG_UNITS
+#include "gg_transformer.hip"
+#endif
