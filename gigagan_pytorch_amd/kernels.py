@@ -1452,7 +1452,7 @@ def layernorm_bwd(x: torch.Tensor, dy: torch.Tensor, w: torch.Tensor, stats: tor
     if not rows:
         z = torch.zeros((2, Cc), dtype=torch.float32, device=x.device)
         return dx, z[0], (z[1] if want_db else None)
-    x2, g2 = _rows2(x), _rows2(dy)
+    x2, g2, stats = _rows2(x), _rows2(dy), stats.contiguous()
     dw = torch.empty(Cc, dtype=torch.float32, device=x.device)
     db = torch.empty_like(dw) if want_db else None
     part = torch.empty((L.lib.gg_layernorm_blocks(rows, Cc), 2, Cc), dtype=torch.float32, device=x.device)
@@ -1590,7 +1590,7 @@ def window_fwd(q, k, v, scale: float, left: int, right: int, sinks: int, lengths
 
 def window_bwd(q, k, v, o, o_lo, lse, d_o, scale: float, left: int, right: int, sinks: int, lengths, key_mask):
     """-> dq (B, h, n, d), dk, dv (B, hk, m, d) in the operands' type, as views of dense token-major storage; `o`, `o_lo`, `lse` as
-    window_fwd returned them, d_o (B, h, n, d) with any strides."""
+    window_fwd returned them (in any layout), d_o (B, h, n, d) with any strides."""
     L = _C.lib()
     L.require(q, k, v, o, lse, d_o, lengths, key_mask)
     assert d_o.dtype == q.dtype and d_o.shape == q.shape
@@ -1604,6 +1604,8 @@ def window_bwd(q, k, v, o, o_lo, lse, d_o, scale: float, left: int, right: int, 
             t.zero_()
         return views
     q, k, v, d_o = _attend4(q, h // hk), _attend4(k), _attend4(v), _attend4(d_o, h // hk)
+    # dense as the forward left them (a saved-tensor hook may hand them back in another layout: a copy then)
+    o, o_lo, lse = o.transpose(1, 2).contiguous(), o_lo.contiguous(), lse.contiguous()
     dvec = torch.empty_like(lse)
     D = _window_desc(q, k, v, o, o_lo, lse, scale, left, right, sinks, lengths, key_mask, d_o, dq, dk, dv, dvec)
     with _on_device(L, q):

@@ -1,0 +1,58 @@
+"""The transformer operators as autograd nodes: saved tensors that come back in another layout, forward-mode derivatives, second
+derivatives. On the host-side emulator and on the GPU."""
+import pytest
+import torch
+
+from gigagan_pytorch_amd import ops
+
+WHERE = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
+where = pytest.mark.parametrize('where', WHERE)
+
+
+def rand(shape, where, seed, dtype=torch.float32):
+    g = torch.Generator(device=where).manual_seed(seed)
+    return torch.randn(shape, generator=g, device=where).to(dtype)
+
+
+def operators(where):
+    """(name, function of its leaves, leaves): every differentiable operator, small; `x` first"""
+    pos = ops.grid_positions((40,), where)
+    spec = ops.RotarySpec((16,))
+    qkv = [rand((2, h, 40, 32), where, 1 + h, torch.bfloat16) for h in (4, 2, 2)]
+    return [('layer_norm', ops.impl.layer_norm, [rand((5, 24), where, 1), rand((24,), where, 2), rand((24,), where, 3)]),
+            ('rotary', lambda q, k: torch.cat(ops.impl.rotary(q, pos, spec, k=k), 1), qkv[:2]),
+            ('window_attention', lambda q, k, v: ops.impl.window_attention(q, k, v, scale=0.2, window=(9, 3), sinks=1), qkv)]
+
+
+NAMES = ['layer_norm', 'rotary', 'window_attention']
+
+
+def operator(name, where):
+    return next(o for o in operators(where) if o[0] == name)[1:]
+
+
+# ---- saved-tensor hooks ----------------------------------------------------------------------------------------------
+
+@where
+@pytest.mark.parametrize('name', NAMES)
+@pytest.mark.parametrize('hook', ['clone', 'reversed', 'cpu'])
+def test_saved_tensors_in_another_layout(where, name, hook):
+    """hooks that give the saved tensors back contiguous, with the axes' order in memory turned round, and through host memory: the
+    gradients have the same bits"""
+    fn, leaves = operator(name, where)
+    leaves = [t.requires_grad_() for t in leaves]
+    y = fn(*leaves)
+    cot = rand(y.shape, where, 9, y.dtype)
+    ref = torch.autograd.grad(y, leaves, cot)
+
+    def turned(t):
+        if not t.dim():
+            return t
+        order = list(range(t.dim()))[::-1]
+        return t.detach().permute(order).clone(memory_format=torch.contiguous_format).permute(order)
+    with {'clone': lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(memory_format=torch.contiguous_format), lambda t: t),
+          'reversed': lambda: torch.autograd.graph.saved_tensors_hooks(turned, lambda t: t),
+          'cpu': lambda: torch.autograd.graph.save_on_cpu(pin_memory=where == 'cuda')}[hook]():
+        got = fn(*leaves)
+    for a, b in zip(torch.autograd.grad(got, leaves, cot), ref):
+        assert torch.equal(a, b)
