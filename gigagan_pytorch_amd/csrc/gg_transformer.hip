@@ -290,3 +290,14 @@ extern "C" int gg_window_bwd(const gg_window_desc* d, void* workspace, size_t wo
 #undef GG_WIN_GO
     return gg_check_launch();
 }
+
+#ifdef GG_HOST_EMULATION
+// for the tests: the rows that the dk / dv of the key tile at k0 visit (a case whose tensors no test can hold)
+extern "C" void gg_emu_window_rows(const gg_window_desc* d, int32_t len, int32_t k0, int32_t chunk, int32_t chunks, int32_t* rows) {
+    GgWinParams p;
+    if (gg_win_check("gg_emu_window_rows", d, p)) return;
+    const GgwRows r = ggw_rows(p, len, k0, chunk, chunks);
+    rows[0] = r.ra;
+    rows[1] = r.rb;
+}
+#endif

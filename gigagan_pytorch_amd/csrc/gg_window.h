@@ -797,6 +797,27 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dq_kernel(GgWinParams p) {
 // workgroup: 4 waves x 32 keys, row tiles of 64 (Q and dO by LDS-DMA, double buffered, each read as rows and transposed). The key tiles that hold sinks are seen by
 // every later row (and where there are few key tiles, every one): their rows are cut into p.sink_chunks chunks, each a workgroup of its own that leaves fp32 sums for
 // gg_win_sink_kernel.  part_o: [B*hk][sink_tiles][chunks][2][128][D].
+// the rows ra .. rb that see some key of the 128-key tile at k0, or their part `chunk` of `chunks` (whole 64-row tiles); none: ra > rb.
+// Compared as tokens before they become rows: keys far in front of every query are a token that, times g, 32 bits do not hold.
+struct GgwRows { int ra, rb; };
+GG_HOST_DEVICE GgwRows ggw_rows(const GgWinParams& p, int len, int k0, int chunk, int chunks) {
+    GgwRows r = {0, -1};
+    const int shift = len - p.n, klast = k0 + 127 < len - 1 ? k0 + 127 : len - 1;
+    int tlo = k0 - p.right - shift, thi = klast + p.left - shift;
+    if (k0 < p.sinks || thi > p.n - 1) thi = p.n - 1;
+    if (tlo < -shift) tlo = -shift;
+    if (tlo < 0) tlo = 0;
+    if (klast < k0 || thi < tlo) return r;
+    r.ra = tlo * p.g;
+    r.rb = thi * p.g + p.g - 1;
+    if (chunks > 1) {
+        const long long nt = ((long long)r.rb - r.ra + 64) / 64, c0 = nt * chunk / chunks, c1 = nt * (chunk + 1) / chunks;
+        const int z = r.ra + (int)(c1 * 64 - 1);
+        r.ra += (int)(c0 * 64);
+        r.rb = z < r.rb ? z : r.rb;
+    }
+    return r;
+}
 // one key's dk and dv again, by one wave, from the rows ra .. rb that see it alone: fix[2 D] = sum of dS q, sum of P dO
 template <int T, int D>
 GG_DEVICE void ggw_fix_dkv(const GgWinParams& p, const unsigned short* qb, const unsigned short* gb, const unsigned short* k, const unsigned short* v,
@@ -861,23 +882,8 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
     const int k0 = tile * 128;
     const unsigned char* keep = p.keep ? p.keep + b * p.keep_b : nullptr;
 
-    // the rows that see some key of the tile
-    const int klast = (k0 + 127 < len - 1 ? k0 + 127 : len - 1);
-    long long ra = 0, rb = -1;
-    if (klast >= k0) {
-        int tlo = k0 - p.right - shift, thi = klast + p.left - shift;
-        if (k0 < p.sinks || thi > p.n - 1) thi = p.n - 1;
-        if (tlo < -shift) tlo = -shift;
-        if (tlo < 0) tlo = 0;
-        ra = (long long)tlo * p.g;
-        rb = (long long)thi * p.g + p.g - 1;
-    }
-    if (tile < p.sink_tiles && rb >= ra) {
-        const long long nt = (rb - ra + 64) / 64, c0 = nt * chunk / p.sink_chunks, c1 = nt * (chunk + 1) / p.sink_chunks;
-        const long long a = ra + c0 * 64, z = ra + c1 * 64 - 1;
-        ra = a;
-        rb = z < rb ? z : rb;
-    }
+    const GgwRows rw = ggw_rows(p, len, k0, tile < p.sink_tiles ? chunk : 0, tile < p.sink_tiles ? p.sink_chunks : 1);
+    const int ra = rw.ra, rb = rw.rb;
 
     const int kj0 = k0 + wave * 32, kj = kj0 + (lane & 31), kjc = kj < p.m ? kj : p.m - 1;
     const bool kept = kj < len && (!keep || keep[kj]);
@@ -935,11 +941,11 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
     int r_pos = 0;
     auto fetch = [&](int i0, int buf) {
         const GgBufS bq = gg_make_bufs(qb + (unsigned long long)(unsigned)ft * p.qn, GGW_SPAN), bg = gg_make_bufs(gb + (unsigned long long)(unsigned)ft * p.gn, GGW_SPAN);
-        const bool all = i0 + 63 <= (int)rb;
+        const bool all = i0 + 63 <= rb;
 #pragma unroll
         for (int s = 0; s < NV; ++s) {
             // (rows behind the last one: an offset that the buffer's bounds check turns into zeros)
-            const bool in = all || i0 + (int)(threadIdx.x + 256 * s) / (D / 8) <= (int)rb;
+            const bool in = all || i0 + (int)(threadIdx.x + 256 * s) / (D / 8) <= rb;
             gg_bufs_load_lds16(bq, in ? oq[s] : GGW_SPAN, 0, sQ[buf] + (wave + 4 * s) * 1024);
             gg_bufs_load_lds16(bg, in ? og[s] : GGW_SPAN, 0, sG[buf] + (wave + 4 * s) * 1024);
         }
@@ -951,8 +957,8 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
     const float *lse = p.lse + (long long)bkv * rows, *dvec = p.dvec + (long long)bkv * rows;
     auto stats = [&](int i0) {              // lse = +inf: a row that is not there or sees nothing
         const int r = i0 + (int)(threadIdx.x & 63);
-        const bool in = r <= (int)rb;
-        const unsigned at = in ? r : (int)rb;
+        const bool in = r <= rb;
+        const unsigned at = in ? r : rb;
         r_lse = in ? lse[at] : __builtin_inff();
         r_d = in ? dvec[at] : 0.f;
         r_pos = in ? rt + shift : -2 * GGW_NONE;
@@ -965,17 +971,17 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     if (ra <= rb) {
-        start((int)ra);
-        stats((int)ra);
+        start(ra);
+        stats(ra);
         gg_wait_vm<0>();            // (this wave's keys: the transfers' count starts at zero)
-        fetch((int)ra, 0);
+        fetch(ra, 0);
     }
     // a row's distance from its tile's first row to tokens: x / g for x < g + 64 by a reciprocal rounded up (exact: x g < 2^32)
     const unsigned recip = p.g > 1 ? (unsigned)(0xffffffffu / (unsigned)p.g) + 1u : 0u;
     auto tokens = [&](int x) { return recip ? (int)(((unsigned long long)(unsigned)x * recip) >> 32) : x; };
     int ct = 0, ch = 0;
-    if (ra <= rb) { ct = (int)((unsigned)(int)ra / (unsigned)p.g); ch = (int)ra - ct * p.g; }
-    for (int i0 = (int)ra, buf = 0; i0 <= (int)rb; i0 += 64, buf ^= 1) {
+    if (ra <= rb) { ct = (int)((unsigned)ra / (unsigned)p.g); ch = ra - ct * p.g; }
+    for (int i0 = ra, buf = 0; i0 <= rb; i0 += 64, buf ^= 1) {
         const int t0 = ct, h0 = ch;
         ct += step_t;
         ch += step_h;
@@ -983,7 +989,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
         if (threadIdx.x < 64) { sLse[buf][threadIdx.x] = r_lse; sD[buf][threadIdx.x] = r_d; sPos[buf][threadIdx.x] = r_pos; }
         gg_wait_vm<0>();
         gg_barrier_lds();
-        if (i0 + 64 <= (int)rb) {
+        if (i0 + 64 <= rb) {
             stats(i0 + 64);
             fetch(i0 + 64, buf ^ 1);
         }
@@ -991,10 +997,10 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
         for (int ib = 0; ib < 2; ++ib) {
             // the 32 rows' positions: all there, and the wave's 32 keys all seen by all of them?
             const int r1 = i0 + ib * 32 + 31;
-            if (i0 + ib * 32 > (int)rb) break;
-            const int plo = t0 + tokens(h0 + ib * 32) + shift, phi = t0 + tokens(h0 + (r1 <= (int)rb ? ib * 32 + 31 : (int)rb - i0)) + shift;
+            if (i0 + ib * 32 > rb) break;
+            const int plo = t0 + tokens(h0 + ib * 32) + shift, phi = t0 + tokens(h0 + (r1 <= rb ? ib * 32 + 31 : rb - i0)) + shift;
             if (kj0 > phi + p.right || (wlast < plo - p.left && kj0 >= p.sinks) || kj0 >= len) continue;
-            const bool full = whole && r1 <= (int)rb && wlast <= plo + p.right && (kj0 >= phi - p.left || wlast < p.sinks);
+            const bool full = whole && r1 <= rb && wlast <= plo + p.right && (kj0 >= phi - p.left || wlast < p.sinks);
             f32x16 st, dp;
             const GgwLane lo = ggw_here(lanes);
             ggw_pipe<2 * KK, D == 128 ? 2 : 4>([&](int s) { return ggw_frag<D>(s & 1 ? sG[buf] : sQ[buf], ib * 32, s >> 1, lo); },
@@ -1040,7 +1046,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
             const int j = kj0 + k;
             if (!((bad >> k) & 1) || j >= len || (keep && !keep[j])) continue;          // (a key that nobody sees ends as zeros below)
             ggw_fix_dkv<T, D>(p, qb, gb, p.k + b * p.kb + kvh * p.kh + (long long)j * p.kn, p.v + b * p.vb + kvh * p.vh + (long long)j * p.vn, j, shift,
-                              (long long)bkv * rows, (int)ra, (int)rb, sFix[wave]);
+                              (long long)bkv * rows, ra, rb, sFix[wave]);
             ggw_take_fix<2 * DB>(acc, sFix[wave], (lane & 31) == k);
         }
     if (__builtin_expect(bad != 0, 0) && !kept) {

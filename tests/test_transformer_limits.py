@@ -1,0 +1,50 @@
+"""The transformer operators at the ends of what they accept: sizes that no test can hold are put to the host's arithmetic alone."""
+import ctypes as C
+import random
+
+import torch
+
+from gigagan_pytorch_amd import _C
+
+
+def window_desc(**kw):
+    """a descriptor that the checks accept: its pointers are never followed here"""
+    p = torch.zeros(4096).data_ptr()
+    d = dict(q=p, k=p, v=p, o=p, o_lo=p, lse=p, d_o=p, dq=p, dk=p, dv=p, dvec=p, B=1, n=1, m=1, h=1, hk=1, d=64, left=-1, right=-1, scale=1.0)
+    return _C.WindowDesc(**{**d, **kw})
+
+
+def test_the_rows_of_a_key_tile():
+    """the rows that a key tile's dk and dv visit, over the accepted range of keys (2^28) and rows (2^30): none where every query is far
+    behind the tile (keys 2^28 in front of sixteen heads' rows are row -2^32), and the chunks cut them without gap or overlap"""
+    lib = _C.lib().lib
+    rows = (C.c_int32 * 2)()
+    rng = random.Random(0)
+
+    def visited(d, length, k0, chunk=0, chunks=1):
+        lib.gg_emu_window_rows(C.byref(d), length, k0, chunk, chunks, rows)
+        return (rows[0], rows[1]) if rows[0] <= rows[1] else None
+    cases = [(1 << 28, 1, 16, 0, 0, 0, 0), (1 << 28, 5, 100, 7, 3, 0, 128), (1 << 28, 1 << 20, 1024, 0, 0, 0, 1 << 27)]
+    for _ in range(2000):
+        m, g = round(2 ** rng.uniform(0, 28)), round(2 ** rng.uniform(0, 12))
+        n = round(2 ** rng.uniform(0, 30)) // g + 1
+        n = min(n, (1 << 30) // g)
+        left, right = (rng.choice([-1, 0, round(2 ** rng.uniform(0, 28))]) for _ in range(2))
+        cases.append((m, n, g, left, right, rng.choice([0, 0, 1, round(2 ** rng.uniform(0, 28))]), round(2 ** rng.uniform(0, 28)) // 128 * 128 % m // 128 * 128))
+    none = 0
+    for m, n, g, left, right, sinks, k0 in cases:
+        length = rng.choice([m, m, rng.randint(0, m)])
+        d = window_desc(m=m, n=n, h=g, left=left, right=right, sinks=sinks)
+        # tokens whose position p = length - n + i >= 0 sees a key of the tile that is there
+        shift, last = length - n, min(k0 + 127, length - 1)
+        lo = max(0, -shift, k0 - right - shift if right >= 0 else 0)
+        hi = n - 1 if left < 0 or k0 < min(sinks, m) else min(n - 1, last + left - shift)
+        want = (lo * g, hi * g + g - 1) if last >= k0 and lo <= hi else None
+        none += want is None
+        assert visited(d, length, k0) == want, (m, n, g, left, right, sinks, k0, length)
+        if want:
+            chunks = rng.randint(2, 64)
+            parts = [p for p in (visited(d, length, k0, c, chunks) for c in range(chunks)) if p]
+            assert parts[0][0] == want[0] and parts[-1][1] == want[1]
+            assert all(b[0] == a[1] + 1 and (b[0] - want[0]) % 64 == 0 for a, b in zip(parts, parts[1:]))
+    assert none > 100
