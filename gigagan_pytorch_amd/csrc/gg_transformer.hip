@@ -181,16 +181,24 @@ static GgWinPlan gg_win_plan(const gg_window_desc* d) {
     return w;
 }
 
-static int gg_win_check(const char* who, const gg_window_desc* d, GgWinParams& p) {
-    if (!d || !d->q || !d->k || !d->v || !d->o) return gg_fail(-1, "%s: null pointer", who);
+// the sizes that gg_win_plan may be asked about: what it divides by is positive, what it multiplies stays in 64 bits
+static int gg_win_sizes(const char* who, const gg_window_desc* d) {
     if (d->B <= 0 || d->n <= 0 || d->m <= 0 || d->h <= 0 || d->hk <= 0 || d->h % d->hk)
         return gg_fail(-2, "%s: B, n, m, h and hk must be positive and h a multiple of hk", who);
     if (d->d != 32 && d->d != 64 && d->d != 128) return gg_fail(-2, "%s: heads of 32, 64 or 128 features (got %d)", who, d->d);
+    if (d->sinks < 0) return gg_fail(-3, "%s: negative sinks", who);
+    if (d->m > (1 << 28) || (long long)d->n * (d->h / d->hk) > (1 << 30)) return gg_fail(-2, "%s: more than 2^28 keys or 2^30 rows a head", who);
+    if (!gg_grid_fits((long long)d->B * d->hk, 256)) return gg_fail(-2, "%s: too many rows", who);      // (a workgroup a key head at least)
+    return 0;
+}
+
+static int gg_win_check(const char* who, const gg_window_desc* d, GgWinParams& p) {
+    if (!d || !d->q || !d->k || !d->v || !d->o) return gg_fail(-1, "%s: null pointer", who);
+    const int rc = gg_win_sizes(who, d);
+    if (rc) return rc;
     if (d->dtype != GG_ELT_BF16 && d->dtype != GG_ELT_F16) return gg_fail(-3, "%s: dtype must be bf16 (0) or half (1)", who);
     if (!(d->scale > 0.f) || d->scale > 1.0e30f) return gg_fail(-3, "%s: scale must be positive and finite", who);
-    if (d->sinks < 0) return gg_fail(-3, "%s: negative sinks", who);
     const long long g = d->h / d->hk;
-    if (d->m > (1 << 28) || (long long)d->n * g > (1 << 30)) return gg_fail(-2, "%s: more than 2^28 keys or 2^30 rows a head", who);
     const void* ptrs[] = {d->q, d->k, d->v, d->o, d->o_lo, d->d_o, d->dq, d->dk, d->dv};
     for (const void* x : ptrs)
         if ((unsigned long long)x & 15) return gg_fail(-4, "%s: operands must be 16-byte aligned", who);
@@ -221,7 +229,7 @@ static int gg_win_check(const char* who, const gg_window_desc* d, GgWinParams& p
 }
 
 extern "C" size_t gg_window_workspace_bytes(const gg_window_desc* d, int32_t backward) {
-    if (!d || d->B <= 0 || d->n <= 0 || d->m <= 0 || d->h <= 0 || d->hk <= 0 || d->d <= 0 || d->sinks < 0) return 0;
+    if (!d || gg_win_sizes("gg_window_workspace_bytes", d)) return 0;
     const GgWinPlan w = gg_win_plan(d);
     return backward ? w.bwd_bytes : w.fwd_bytes;
 }

@@ -48,3 +48,17 @@ def test_the_rows_of_a_key_tile():
             assert parts[0][0] == want[0] and parts[-1][1] == want[1]
             assert all(b[0] == a[1] + 1 and (b[0] - want[0]) % 64 == 0 for a, b in zip(parts, parts[1:]))
     assert none > 100
+
+
+def test_the_workspace_query_refuses_what_the_calls_refuse():
+    """sizes that no call takes have no workspace: fewer query heads than key heads, head sizes that are not there, products beyond 64 bits"""
+    lib = _C.lib().lib
+    big = 2 ** 31 - 1
+    for bad in (dict(h=1, hk=2), dict(h=3, hk=2), dict(d=48), dict(d=0), dict(m=big), dict(n=big, h=2), dict(B=big, hk=big, h=big), dict(sinks=-1), dict(n=0),
+                dict(hk=-1)):
+        d = window_desc(**bad)
+        for backward in (0, 1):
+            assert lib.gg_window_workspace_bytes(C.byref(d), backward) == 0, bad
+        assert lib.gg_window_fwd(C.byref(d), None, 0, None) < 0, bad
+        assert lib.gg_window_bwd(C.byref(d), None, 0, None) < 0, bad
+    assert lib.gg_window_workspace_bytes(C.byref(window_desc(m=8192)), 0) > 0
