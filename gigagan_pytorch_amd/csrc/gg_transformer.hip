@@ -188,6 +188,8 @@ static int gg_win_sizes(const char* who, const gg_window_desc* d) {
     if (d->d != 32 && d->d != 64 && d->d != 128) return gg_fail(-2, "%s: heads of 32, 64 or 128 features (got %d)", who, d->d);
     if (d->sinks < 0) return gg_fail(-3, "%s: negative sinks", who);
     if (d->m > (1 << 28) || (long long)d->n * (d->h / d->hk) > (1 << 30)) return gg_fail(-2, "%s: more than 2^28 keys or 2^30 rows a head", who);
+    // (dk / dv divides by a group's heads with a 32-bit reciprocal: exact for quotients of x < g + 64 while x g < 2^32)
+    if (d->h / d->hk > GG_WINDOW_MAX_GROUP) return gg_fail(-2, "%s: more than %d query heads a key head", who, GG_WINDOW_MAX_GROUP);
     if (!gg_grid_fits((long long)d->B * d->hk, 256)) return gg_fail(-2, "%s: too many rows", who);      // (a workgroup a key head at least)
     return 0;
 }

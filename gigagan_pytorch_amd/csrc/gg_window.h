@@ -976,7 +976,8 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
         gg_wait_vm<0>();            // (this wave's keys: the transfers' count starts at zero)
         fetch(ra, 0);
     }
-    // a row's distance from its tile's first row to tokens: x / g for x < g + 64 by a reciprocal rounded up (exact: x g < 2^32)
+    // a row's distance from its tile's first row to tokens: x / g for x < g + 64 by a reciprocal rounded up (exact: x g < 2^32, which the
+    // host checks)
     const unsigned recip = p.g > 1 ? (unsigned)(0xffffffffu / (unsigned)p.g) + 1u : 0u;
     auto tokens = [&](int x) { return recip ? (int)(((unsigned long long)(unsigned)x * recip) >> 32) : x; };
     int ct = 0, ch = 0;

@@ -1536,6 +1536,7 @@ def rotary(q: torch.Tensor, k, positions: torch.Tensor, spec: RotarySpec, invers
 
 
 WINDOW_HEAD_DIMS = (32, 64, 128)
+WINDOW_MAX_GROUP = 65504
 
 
 def _strides3(t: torch.Tensor):

@@ -2001,6 +2001,8 @@ class HipOps:
             raise ValueError(f'window_attention: shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit')
         if d not in K.WINDOW_HEAD_DIMS:
             raise ValueError(f'window_attention: heads of {K.WINDOW_HEAD_DIMS} features expected, got {d}')
+        if h // hk > K.WINDOW_MAX_GROUP:
+            raise ValueError(f'window_attention: at most {K.WINDOW_MAX_GROUP} query heads a key head expected, got {h // hk}')
         scale = float(scale)
         if not (0.0 < scale <= 1e30):
             raise ValueError(f'window_attention: scale must be positive and finite, got {scale}')

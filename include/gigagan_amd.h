@@ -519,18 +519,21 @@ typedef struct gg_rotary_desc {
 } gg_rotary_desc;
 int gg_rotary(const gg_rotary_desc* d, void* stream);
 
-/* attention with a sliding window and sinks (csrc/gg_window.h). q [B][h][n][d], k, v [B][hk][m][d], h a multiple of hk (grouped heads), d
- * 32, 64 or 128, bf16 or half, element strides {batch, head, token} in multiples of 8 with unit feature stride, 16-byte aligned, token
- * strides below GG_WINDOW_MAX_STRIDE (2^24) and head strides of q and d_o times h / hk below 64 times that. Query i of item b sits at position p = len_b - n + i, len_b = lengths[b] (device int32, clamped to 0 .. m) or m, and sees key j when
- * j < len_b, j <= p + right, (j >= p - left or j < sinks) and key_mask[b][j] (bytes, batch stride mask_stride; optional); left / right
- * < 0 = no bound. A query that sees no key, or at p < 0, gets zeros and no gradient.
+/* attention with a sliding window and sinks (csrc/gg_window.h). q [B][h][n][d], k, v [B][hk][m][d], h a multiple of hk (grouped heads, at
+ * most GG_WINDOW_MAX_GROUP a key head), d 32, 64 or 128, bf16 or half, element strides {batch, head, token} in multiples of 8 with unit
+ * feature stride, 16-byte aligned, token strides below GG_WINDOW_MAX_STRIDE (2^24) and head strides of q and d_o times h / hk below 64
+ * times that. Query i of item b sits at position p = len_b - n + i, len_b = lengths[b] (device int32, clamped to 0 .. m) or m, and sees
+ * key j when j < len_b, j <= p + right, (j >= p - left or j < sinks) and key_mask[b][j] (bytes, batch stride mask_stride; optional);
+ * left / right < 0 = no bound. A query that sees no key, or at p < 0, gets zeros and no gradient.
  *   forward:  o dense [B][n][h][d]; for the backward o_lo like o (what o's rounding took off) and lse fp32 [B*hk][n*h/hk] (log2 domain,
  *             +inf for a row that sees nothing), both optional
  *   backward: reads q, k, v, o, o_lo, lse and d_o (strides g_strides), writes dq dense [B][n][h][d], dk, dv dense [B][m][hk][d] (every element)
  *             and dvec fp32 [B*hk][n*h/hk] (scratch)
- * Both take a workspace of gg_window_workspace_bytes(d, backward) bytes (0: none, or sizes that the calls refuse), 16-byte aligned, free again when the call's work on
+ * Both take a workspace of gg_window_workspace_bytes(d, backward) bytes (0: none, or sizes that the calls refuse), 16-byte aligned, free
+ * again when the call's work on
  * `stream` is done. Results do not depend on what runs beside: no atomics. */
 #define GG_WINDOW_MAX_STRIDE (1 << 24)
+#define GG_WINDOW_MAX_GROUP 65504
 typedef struct gg_window_desc {
     const void* q; const void* k; const void* v; void* o; void* o_lo; float* lse;
     const void* d_o; void* dq; void* dk; void* dv; float* dvec;

@@ -2,9 +2,10 @@
 import ctypes as C
 import random
 
+import pytest
 import torch
 
-from gigagan_pytorch_amd import _C
+from gigagan_pytorch_amd import _C, ops
 
 
 def window_desc(**kw):
@@ -62,3 +63,18 @@ def test_the_workspace_query_refuses_what_the_calls_refuse():
         assert lib.gg_window_fwd(C.byref(d), None, 0, None) < 0, bad
         assert lib.gg_window_bwd(C.byref(d), None, 0, None) < 0, bad
     assert lib.gg_window_workspace_bytes(C.byref(window_desc(m=8192)), 0) > 0
+
+
+def test_groups_beyond_the_reciprocal_are_refused():
+    """dk / dv turns a row's distance in its tile into tokens by a multiplication with 2^32 / g rounded up: right up to 65504 heads a group,
+    wrong from 65537 on, where the call is refused"""
+    def quotients(g):
+        recip = 0xffffffff // g + 1
+        return all((x * recip >> 32) == x // g for x in (0, 1, g - 1, g, g + 1, g + 63))
+    assert all(quotients(g) for g in (2, 3, 63, 64, 65, 4097, 65503, 65504)) and not quotients(65537)
+    lib = _C.lib().lib
+    d = window_desc(h=65505)
+    assert lib.gg_window_fwd(C.byref(d), None, 0, None) == -2 and lib.gg_window_bwd(C.byref(d), None, 0, None) == -2
+    q, k = torch.zeros(1, 65505, 1, 32, dtype=torch.bfloat16), torch.zeros(1, 1, 1, 32, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match='heads a key head'):
+        ops.impl.window_attention(q, k, k, scale=1.0)
