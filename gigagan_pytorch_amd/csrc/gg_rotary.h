@@ -34,7 +34,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_rotary_kernel(GgRotParams p) {
     GG_SHARED __attribute__((aligned(16))) float sCos[GG_ROT_LDS_PAIRS];
     GG_SHARED __attribute__((aligned(16))) float sSin[GG_ROT_LDS_PAIRS];
     const GgRotParams* kp = gg_late_params(p);          // (the two tables are indexed per lane: read where they lie)
-    const int tiles = (p.n + p.tb - 1) / p.tb;
+    const int tiles = (p.n - 1) / p.tb + 1;
     const int b = blockIdx.x / tiles;
     const int t0 = (blockIdx.x - b * tiles) * p.tb;
     const int nt = p.n - t0 < p.tb ? p.n - t0 : p.tb;

@@ -41,7 +41,7 @@ extern "C" int gg_layernorm_fwd(const void* x, int64_t ldx, const float* w, cons
     memset(&p, 0, sizeof(p));
     p.x = x; p.ldx = ldx; p.w = w; p.b = b; p.y = y; p.mean = mean; p.rstd = rstd; p.rows = rows; p.C = C; p.eps = eps;
 #define GG_LN_GO(TPR, NV)                                                                                                    \
-    const long long rpb = TPR > 256 ? 1 : 256 / TPR, blocks = (rows + rpb - 1) / rpb;                                        \
+    const long long rpb = TPR > 256 ? 1 : 256 / TPR, blocks = (rows - 1) / rpb + 1;                                          \
     if (!gg_grid_fits(blocks, TPR > 256 ? TPR : 256)) return gg_fail(-2, "gg_layernorm_fwd: too many rows");                  \
     const dim3 grid((unsigned)blocks), block(TPR > 256 ? TPR : 256);                                                         \
     if (dtype == GG_ELT_BF16) GG_LAUNCH((gg_layernorm_fwd_kernel<GG_ELT_BF16, TPR, NV>), grid, block, (hipStream_t)stream, p);     \
@@ -54,7 +54,7 @@ extern "C" int gg_layernorm_fwd(const void* x, int64_t ldx, const float* w, cons
 
 extern "C" int32_t gg_layernorm_blocks(int64_t rows, int32_t C) {
     const long long rpb = C <= 128 ? 16 : (C <= 2048 ? 4 : 1);
-    const long long blocks = (rows + rpb - 1) / rpb;
+    const long long blocks = (rows - 1) / rpb + 1;
     return (int32_t)(blocks < 1 ? 1 : (blocks > 512 ? 512 : blocks));
 }
 
@@ -117,7 +117,7 @@ extern "C" int gg_rotary(const gg_rotary_desc* d, void* stream) {
     const long long fill = (long long)d->B * d->n / 1024;           // (few tokens: rather spread over the chip)
     if (tb > fill) tb = fill;
     p.tb = (int)(tb < 1 ? 1 : tb);
-    const long long grid = (long long)d->B * ((d->n + p.tb - 1) / p.tb);
+    const long long grid = (long long)d->B * ((d->n - 1) / p.tb + 1);
     if (!gg_grid_fits(grid, 256)) return gg_fail(-2, "gg_rotary: too many tokens");
     if (d->dtype == GG_ELT_BF16) GG_LAUNCH(gg_rotary_kernel<GG_ELT_BF16>, dim3((unsigned)grid), dim3(256), (hipStream_t)stream, p);
     else if (d->dtype == GG_ELT_F16) GG_LAUNCH(gg_rotary_kernel<GG_ELT_F16>, dim3((unsigned)grid), dim3(256), (hipStream_t)stream, p);

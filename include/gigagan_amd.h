@@ -530,8 +530,7 @@ int gg_rotary(const gg_rotary_desc* d, void* stream);
  *   backward: reads q, k, v, o, o_lo, lse and d_o (strides g_strides), writes dq dense [B][n][h][d], dk, dv dense [B][m][hk][d] (every element)
  *             and dvec fp32 [B*hk][n*h/hk] (scratch)
  * Both take a workspace of gg_window_workspace_bytes(d, backward) bytes (0: none, or sizes that the calls refuse), 16-byte aligned, free
- * again when the call's work on
- * `stream` is done. Results do not depend on what runs beside: no atomics. */
+ * again when the call's work on `stream` is done. Results do not depend on what runs beside: no atomics. */
 #define GG_WINDOW_MAX_STRIDE (1 << 24)
 #define GG_WINDOW_MAX_GROUP 65504
 typedef struct gg_window_desc {

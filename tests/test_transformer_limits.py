@@ -78,3 +78,28 @@ def test_groups_beyond_the_reciprocal_are_refused():
     q, k = torch.zeros(1, 65505, 1, 32, dtype=torch.bfloat16), torch.zeros(1, 1, 1, 32, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match='heads a key head'):
         ops.impl.window_attention(q, k, k, scale=1.0)
+
+
+@pytest.mark.gpu
+def test_rotary_of_as_many_tokens_as_a_size_holds():
+    """2^31 - 1 tokens of one pair (8 GiB): the tokens at both ends and across the 2^32-byte offsets turn as they do alone"""
+    n = 2 ** 31 - 1
+    spec = ops.RotarySpec((1,))
+    q = torch.zeros((1, 1, n, 2), dtype=torch.bfloat16, device='cuda')
+    pos = torch.full((1, 1), 2, dtype=torch.int32, device='cuda')
+    at = [0, 1, 1023, 1024, 2 ** 30 - 1, 2 ** 30, 2 ** 30 + 1, n - 1024, n - 1]
+    part = torch.randn(1, 1, len(at), 2, device='cuda').to(torch.bfloat16)
+    for i, t in enumerate(at):
+        q[:, :, t] = part[:, :, i]
+    y = ops.impl.rotary(q, pos.expand(n, 1), spec)
+    want = ops.impl.rotary(part, pos.expand(len(at), 1), spec)
+    assert all(torch.equal(y[:, :, t], want[:, :, i]) for i, t in enumerate(at))
+    assert not y[:, :, 2 ** 30 + 2:2 ** 30 + 4096].any() and not y[:, :, 2:1000].any()
+
+
+def test_row_counts_at_the_end_of_64_bits():
+    lib = _C.lib().lib
+    p = torch.zeros(4096).data_ptr()
+    top = 2 ** 63 - 1
+    assert lib.gg_layernorm_fwd(p, 8, p, p, p, None, None, top, 8, 1e-5, 0, None) == -2 and b'too many rows' in lib.gg_last_error()
+    assert [lib.gg_layernorm_blocks(r, 512) for r in (1, 4, 5, top - 1, top)] == [1, 1, 2, 512, 512]
