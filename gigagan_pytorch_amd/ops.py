@@ -753,6 +753,30 @@ def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+class FirstOrderFn(Function):
+    """the gradients of an operator without second derivatives, in a graph that may be differentiated again: handed through, an error where
+    they are differentiated. They hang on the operator's inputs and on the incoming gradient, so every way from them to a leaf leads
+    past the error (torch's once_differentiable hangs its error on copies: a second derivative for a named leaf goes round it, and its
+    term is lost without a word)."""
+
+    @staticmethod
+    def forward(ctx, what, n, *tensors):
+        ctx.what = what
+        return tensors[:n]
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f'{ctx.what}: second derivatives are not provided (a gradient taken with create_graph=True was differentiated)')
+
+
+def _first_order(what, grads, *inputs):
+    """`grads` of an operator's backward as they may be handed out: under create_graph=True they refuse to be differentiated"""
+    if not torch.is_grad_enabled():
+        return grads
+    out = iter(FirstOrderFn.apply(what, sum(g is not None for g in grads), *(g for g in grads if g is not None), *inputs))
+    return tuple(None if g is None else next(out) for g in grads)
+
+
 class LayerNormFn(Function):
     """layer norm over the last axis in one pass (gg_layernorm.h); backward: dx and the workgroups' sums of dw, db in one pass over x
     and dy, their total in a second launch. First order."""
@@ -765,15 +789,15 @@ class LayerNormFn(Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
-        dx, dw, db = K.layernorm_bwd(x, dy if dy.dtype == x.dtype else dy.to(x.dtype), _vector_f32(weight), stats, ctx.bias_dtype is not None)
-        if dw.dtype != weight.dtype:
-            dw = dw.to(weight.dtype)
-        if db is not None and db.dtype != ctx.bias_dtype:
-            db = db.to(ctx.bias_dtype)
-        return dx, dw, db, None
+        with torch.no_grad():
+            dx, dw, db = K.layernorm_bwd(x, dy if dy.dtype == x.dtype else dy.to(x.dtype), _vector_f32(weight), stats, ctx.bias_dtype is not None)
+            if dw.dtype != weight.dtype:
+                dw = dw.to(weight.dtype)
+            if db is not None and db.dtype != ctx.bias_dtype:
+                db = db.to(ctx.bias_dtype)
+        return (*_first_order('layer_norm', (dx, dw, db), x, weight, dy), None)
 
 
 class RotaryFn(Function):
@@ -899,9 +923,8 @@ class FlashAttnGenFn(Function):
 
 
 class WindowAttnFn(Function):
-    """attention with a sliding window and sinks (gg_window.h): forward saves o, the rest that its rounding took off, and the
-    rows' log-sum-exp, backward is two kernels (dq;
-    dk and dv, summed over the query heads of a shared key head) that recompute P. First order."""
+    """attention with a sliding window and sinks (gg_window.h): forward saves o, the rest that its rounding took off, and the rows'
+    log-sum-exp, backward is two kernels (dq; dk and dv, summed over the query heads of a shared key head) that recompute P. First order."""
 
     @staticmethod
     def forward(ctx, q, k, v, lengths, key_mask, scale, left, right, sinks):
@@ -911,11 +934,11 @@ class WindowAttnFn(Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_o):
         q, k, v, lengths, key_mask, o, o_lo, lse = ctx.saved_tensors
-        dq, dk, dv = K.window_bwd(q, k, v, o, o_lo, lse, d_o if d_o.dtype == q.dtype else d_o.to(q.dtype), *ctx.cfg, lengths, key_mask)
-        return dq, dk, dv, None, None, None, None, None, None
+        with torch.no_grad():
+            grads = K.window_bwd(q, k, v, o, o_lo, lse, d_o if d_o.dtype == q.dtype else d_o.to(q.dtype), *ctx.cfg, lengths, key_mask)
+        return (*_first_order('window_attention', grads, q, k, v, d_o), *[None] * 6)
 
 
 def _rows_view(t):

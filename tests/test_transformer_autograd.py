@@ -56,3 +56,34 @@ def test_saved_tensors_in_another_layout(where, name, hook):
         got = fn(*leaves)
     for a, b in zip(torch.autograd.grad(got, leaves, cot), ref):
         assert torch.equal(a, b)
+
+
+# ---- second derivatives ----------------------------------------------------------------------------------------------
+
+@where
+@pytest.mark.parametrize('name', ['layer_norm', 'window_attention'])
+@pytest.mark.parametrize('loss', ['linear', 'square'])
+@pytest.mark.parametrize('leaf', [0, 1])
+def test_second_derivatives_are_refused_by_name(where, name, loss, leaf):
+    """a loss linear in the operator's output (its gradient there is a constant) and one that is not, each with a second term that has a
+    second derivative of its own; the derivative asked for one leaf and accumulated for all"""
+    fn, leaves = operator(name, where)
+    leaves = [t.requires_grad_() for t in leaves]
+    y = fn(*leaves).float()
+    c = rand(y.shape, where, 4)
+    total = ((y if loss == 'linear' else y.pow(2)) * c).sum() + leaves[leaf].float().pow(3).sum()
+    g, = torch.autograd.grad(total, leaves[leaf], create_graph=True)
+    for second in (lambda: torch.autograd.grad(g.float().pow(2).sum(), leaves[leaf], retain_graph=True), lambda: g.float().sum().backward()):
+        with pytest.raises(RuntimeError, match=f'{name}: second derivatives'):
+            second()
+
+
+@where
+@pytest.mark.parametrize('name', ['layer_norm', 'window_attention'])
+def test_create_graph_alone_is_no_error(where, name):
+    """a gradient taken with create_graph=True that nobody differentiates has the bits of the ordinary one"""
+    fn, leaves = operator(name, where)
+    leaves = [t.requires_grad_() for t in leaves]
+    cot = rand(fn(*leaves).shape, where, 4, leaves[0].dtype)
+    for a, b in zip(torch.autograd.grad(fn(*leaves), leaves, cot, create_graph=True), torch.autograd.grad(fn(*leaves), leaves, cot)):
+        assert torch.equal(a, b) and a.requires_grad
