@@ -21,7 +21,7 @@ import weakref
 
 import torch
 import torch.nn.functional as F
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from . import kernels as K
 
@@ -749,8 +749,10 @@ def _vector_f32(t):
     return t if t is None or (t.dtype == torch.float32 and t.is_contiguous()) else t.detach().float().contiguous()
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _wants_node(*tensors):
+    """whether a call needs its autograd node: a gradient may be asked for - or forward-mode derivatives are on, which the node refuses
+    (the kernels alone would drop the tangents)"""
+    return forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
 
 class FirstOrderFn(Function):
@@ -2043,7 +2045,7 @@ class HipOps:
             if m > 1 and key_mask.stride(1) != 1:
                 key_mask = key_mask.contiguous()
         K._same_device('window_attention', q, k, v, lengths, key_mask)
-        if _wants_grad(q, k, v):
+        if _wants_node(q, k, v):
             return WindowAttnFn.apply(q, k, v, lengths, key_mask, scale, left, right, sinks)
         return K.window_fwd(q, k, v, scale, left, right, sinks, lengths, key_mask, False)[0]
 
@@ -2106,7 +2108,7 @@ class HipOps:
                 continue
             if t is None or tuple(t.shape) != (C,) or not t.is_floating_point():
                 raise ValueError(f'layer_norm: {name} must be a floating tensor of shape ({C},)')
-        if _wants_grad(x, weight, bias):
+        if _wants_node(x, weight, bias):
             return LayerNormFn.apply(x, weight, bias, float(eps))
         return K.layernorm_fwd(x, _vector_f32(weight), _vector_f32(bias), float(eps), False)[0]
 
@@ -2135,7 +2137,7 @@ class HipOps:
         if tuple(positions.shape) not in ((n, A), (B, n, A)):
             raise ValueError(f'rotary: positions of shape ({n}, {A}) or ({B}, {n}, {A}) expected, got {tuple(positions.shape)}')
         K._same_device('rotary', q, k, positions)
-        if _wants_grad(q, k):
+        if _wants_node(q, k):
             return RotaryFn.apply(q, k, positions.detach(), spec, False)
         out = K.rotary(q, k, positions, spec)
         return out[0] if k is None else out

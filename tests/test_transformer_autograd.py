@@ -87,3 +87,23 @@ def test_create_graph_alone_is_no_error(where, name):
     cot = rand(fn(*leaves).shape, where, 4, leaves[0].dtype)
     for a, b in zip(torch.autograd.grad(fn(*leaves), leaves, cot, create_graph=True), torch.autograd.grad(fn(*leaves), leaves, cot)):
         assert torch.equal(a, b) and a.requires_grad
+
+
+# ---- forward mode ------------------------------------------------------------------------------------------------------
+
+@where
+@pytest.mark.parametrize('name', NAMES)
+@pytest.mark.parametrize('leaf', [0, 1])
+def test_forward_mode_is_refused(where, name, leaf):
+    """a tangent is not dropped: the operators have no forward-mode derivatives and say so; without tangents the calls work as ever"""
+    fn, leaves = operator(name, where)
+    with torch.no_grad():
+        ref = fn(*leaves)
+        with torch.autograd.forward_ad.dual_level():
+            assert torch.equal(fn(*leaves), ref)
+            dual = list(leaves)
+            dual[leaf] = torch.autograd.forward_ad.make_dual(leaves[leaf], torch.ones_like(leaves[leaf]))
+            with pytest.raises(NotImplementedError):
+                fn(*dual)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda t: fn(*leaves[:leaf], t, *leaves[leaf + 1:]), (leaves[leaf],), (torch.ones_like(leaves[leaf]),))
