@@ -900,7 +900,8 @@ class FlashAttnGenFn(Function):
     """the general fused attention (gg_attention.h GEN: the unet's Attend attend.py:64-110, CrossAttention gp.py:617-655, the text
     transformer's attention gp.py:659-722): q (B, n, heads*64), k / v (B, m, heads*64) bf16 views with a free row pitch, optional
     null key / value (heads, 64), optional per-key bias (B, m) fp32 (key-padding mask as -1e30; a constant: no gradient). No
-    (B*heads, n, m) probability tensor exists in either direction. First order."""
+    (B*heads, n, m) probability tensor exists in either direction. A backward that is recorded itself (`create_graph=True`) runs in
+    products and softmax passes that can be differentiated again (_attention_grads)."""
 
     @staticmethod
     def forward(ctx, q, k, v, k0, v0, kbias, heads, alpha):
@@ -912,16 +913,52 @@ class FlashAttnGenFn(Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_o):
         q, k, v, k0, v0, kbias, o, lse = ctx.saved_tensors
         heads, alpha = ctx.cfg
+        if torch.is_grad_enabled():
+            return (*_attention_grads(q, k, v, k0, v0, kbias, d_o, heads, alpha), None, None, None)
         k0b = None if k0 is None else k0.to(ACT_DTYPE).contiguous()
         v0b = None if v0 is None else v0.to(ACT_DTYPE).contiguous()
         dq, dk, dv, dk0, dv0, _ = K.attn_gen_bwd(q, k, v, k0b, v0b, kbias, o, lse, d_o.to(ACT_DTYPE).contiguous(), heads, alpha)
         if k0 is not None:
             dk0, dv0 = dk0.to(k0.dtype), dv0.to(v0.dtype)
         return dq, dk, dv, dk0, dv0, None, None, None
+
+
+def _attention_grads(q, k, v, k0, v0, kbias, d_o, heads, alpha):
+    """FlashAttnGenFn's (dq, dk, dv, dk0, dv0) as a function that autograd differentiates: P again, dP = dO V^T, the softmax's backward pass, and
+    the three products with it"""
+    B, n = q.shape[:2]
+    m = k.shape[1]
+    lead = 0 if k0 is None else 1               # the null key and value come first
+    mp = _round8(m + lead)
+
+    def split(t):               # (B, len, heads * 64) -> (B * heads, len, 64)
+        return t.to(ACT_DTYPE).reshape(B, -1, heads, 64).transpose(1, 2).reshape(B * heads, -1, 64)
+
+    def keys(t, null):          # ... with the null row in front and zeros up to a multiple of 8
+        t = split(t)
+        if null is not None:
+            t = torch.cat((null.to(ACT_DTYPE)[None, :, None].expand(B, heads, 1, 64).reshape(B * heads, 1, 64), t), dim=1)
+        return F.pad(t, (0, 0, 0, mp - m - lead)).contiguous()
+
+    def merge(t):
+        return t.reshape(B, heads, -1, 64).transpose(1, 2).reshape(B, -1, heads * 64)
+    qs, gs, ks, vs = split(q).contiguous(), split(d_o).contiguous(), keys(k, k0), keys(v, v0)
+    bias = None
+    if kbias is not None:
+        bias = F.pad(kbias, (lead, mp - m - lead))[:, None].expand(B, heads, mp).reshape(B * heads, mp).contiguous()
+    P = AttnProbsFn.apply(qs, ks, bias, alpha, m + lead)
+    dP = GemmFn.apply(gs, vs, True, True, (n, mp, 64), None, None, 1.0, False)
+    dx, _ = SoftmaxBwdFn.apply(P, dP.contiguous(), alpha, m + lead, False)
+    dq = GemmFn.apply(dx, ks, True, False, (n, 64, mp), None, None, 1.0, False)
+    dk = GemmFn.apply(dx, qs, False, False, (mp, 64, n), None, None, 1.0, False)
+    dv = GemmFn.apply(P, gs, False, False, (mp, 64, n), None, None, 1.0, False)
+    dk0 = dv0 = None
+    if lead:
+        dk0, dv0 = (t[:, 0].float().reshape(B, heads, 64).sum(0).to(r.dtype) for t, r in ((dk, k0), (dv, v0)))
+    return merge(dq), merge(dk[:, lead:lead + m]), merge(dv[:, lead:lead + m]), dk0, dv0
 
 
 class WindowAttnFn(Function):
