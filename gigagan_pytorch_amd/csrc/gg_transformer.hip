@@ -161,22 +161,30 @@ static GgWinPlan gg_win_plan(const gg_window_desc* d) {
     w.fwd_bytes = w.splits > 1 ? (size_t)w.splits * heads * rows * (d->d + 2) * sizeof(float) : 0;
     w.key_tiles = (d->m + 127) / 128;
     w.sink_tiles = (int)((sinks + 127) / 128);
-    // the rows that an ordinary key tile sees set the size of a sink tile's chunks
+    // dk / dv, first rule: the sinks' tiles, which every row sees, are cut into chunks no longer than an ordinary key tile's work (`seen`
+    // rows) - but no shorter than a chip's share of all the work (512 workgroups at a time): many sink tiles fill the chip uncut, and
+    // the chunks are 1024 at most, however many sinks there are
     long long seen = (left + right + 128) * g;
     if (seen > rows) seen = rows;
+    const long long tiles_kv = heads * w.key_tiles, share = heads * (w.sink_tiles * rows + (w.key_tiles - w.sink_tiles) * seen) / 512 + 1;
     long long c = w.sink_tiles ? rows / (seen < 512 ? 512 : seen) : 1;
-    // too few key tiles for the chip: every tile's rows are cut, down to two row tiles a workgroup (66 tiles of 11 row tiles: 44 us whole,
-    // 28 and 4 us in five chunks and their sum; 32 of 64: causal training of 4096 tokens 246 -> 188 us a pass)
-    const long long tiles_kv = heads * w.key_tiles;
+    if (c > (rows + share - 1) / share) c = (rows + share - 1) / share;
+    if (c < 1) c = 1;
+    if (c > 64) c = 64;
+    // Second rule, where there are too few key tiles for the chip: every tile's rows are cut, down to two row tiles a workgroup (66 tiles of
+    // 11 row tiles: 44 us whole, 28 and 4 us in five chunks and their sum; 32 of 64: causal training of 4096 tokens 246 -> 188 us a
+    // pass), into 1024 chunks at most, unless the first rule's longest workgroup is no longer
     if (tiles_kv < 256) {
-        const long long most = (seen + 127) / 128, want = (511 + tiles_kv) / tiles_kv, cut = want < most ? want : most;
-        if (cut > 1) {
+        const long long most = (seen + 127) / 128, want = (511 + tiles_kv) / tiles_kv, room = 1024 / tiles_kv;
+        long long cut = want < most ? want : most;
+        if (cut < c) cut = c < room ? c : room;
+        const long long longest = w.sink_tiles == w.key_tiles || rows / c > seen ? rows / c : seen;
+        if (cut > 1 && (w.sink_tiles ? rows : seen) / cut < (w.sink_tiles ? longest : seen)) {
             w.sink_tiles = w.key_tiles;
-            if (c < cut) c = cut;
+            c = cut;
         }
     }
-    if (c > 64) c = 64;
-    w.sink_chunks = (int)(c < 1 ? 1 : c);
+    w.sink_chunks = (int)c;
     w.bwd_bytes = w.sink_chunks > 1 ? (size_t)heads * w.sink_tiles * w.sink_chunks * 2 * 128 * d->d * sizeof(float) : 0;
     return w;
 }

@@ -7,6 +7,8 @@ import torch
 
 from gigagan_pytorch_amd import _C, ops
 
+where = pytest.mark.parametrize('where', ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+
 
 def window_desc(**kw):
     """a descriptor that the checks accept: its pointers are never followed here"""
@@ -103,3 +105,44 @@ def test_row_counts_at_the_end_of_64_bits():
     top = 2 ** 63 - 1
     assert lib.gg_layernorm_fwd(p, 8, p, p, p, None, None, top, 8, 1e-5, 0, None) == -2 and b'too many rows' in lib.gg_last_error()
     assert [lib.gg_layernorm_blocks(r, 512) for r in (1, 4, 5, top - 1, top)] == [1, 1, 2, 512, 512]
+
+
+def test_the_backward_workspace_is_bounded():
+    """at most 1024 chunks of a key tile's fp32 dk and dv (128 MiB with 128 features), however many sinks, rows and heads there are; the
+    cases with many sinks asked for 1 to 16 GiB once"""
+    lib = _C.lib().lib
+
+    def workspace(B, hk, g, n, m, d, left, right, sinks):
+        return lib.gg_window_workspace_bytes(C.byref(window_desc(B=B, h=hk * g, hk=hk, n=n, m=m, d=d, left=left, right=right, sinks=sinks)), 1)
+    cases = [(1, 8, 4, 16384, 16384, 128, 127, 0, 4096), (4, 8, 4, 16384, 16384, 128, 127, 0, 4096), (8, 8, 1, 32768, 32768, 128, 127, 0, 1024),
+             (8, 8, 1, 32768, 32768, 128, 127, 0, 4096), (1, 8, 1, 16384, 16384, 64, 0, 0, 8192), (1, 8, 4, 16384, 16384, 128, 127, 0, 16384),
+             (1, 1, 8, 32640, 32640, 128, 0, 0, 1)]
+    rng = random.Random(1)
+
+    def log(bits):
+        return round(2 ** rng.uniform(0, bits))
+    for _ in range(5000):
+        m = log(20)
+        n = rng.choice([m, log(20)])
+        cases.append((log(6), log(5), log(4), n, m, rng.choice([32, 64, 128]), rng.choice([-1, log(18) - 1]), rng.choice([-1, 0, log(10)]), rng.choice([0, log(18)])))
+    for case in cases:
+        assert workspace(*case) <= 1024 * 2 * 128 * case[5] * 4, case
+    # what was measured keeps its chunks: 11 tiles x 6, one tile x 2, 32 tiles x 16
+    for case, chunks in (((3, 2, 3, 777, 1291, 32, 100, 7, 3), 6 * 11 * 6), ((4, 8, 1, 1100, 1100, 32, 40, 0, 3), 32 * 2),
+                         ((1, 1, 1, 4096, 4096, 64, -1, 0, 0), 32 * 16), ((8, 8, 1, 4096, 4096, 64, 512, 512, 0), 0)):
+        assert workspace(*case) == chunks * 2 * 128 * case[5] * 4, case
+
+
+@where
+@pytest.mark.parametrize('case', [(1, 2, 1, 700, 40, 32, (3, 0), 40), (1, 1, 1, 300, 300, 32, (2, 1), 300), (1, 2, 2, 600, 260, 32, (0, 0), 129)])
+def test_many_sinks(where, case):
+    """all keys sinks, more rows than keys, a sink tile that is cut beside key tiles that are not: gradients against the definition"""
+    from test_transformer_ops import att_run
+    att_run(where, case, 'bf16')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('case', [(4, 32, 8, 600, 1500, 64, (31, 0), 1300), (1, 8, 1, 2048, 2048, 128, (15, 0), 1), (2, 4, 2, 3000, 3000, 32, (0, 0), 1000)])
+def test_many_sinks_and_heads(case):
+    from test_transformer_ops import att_run
+    att_run('cuda', case, 'bf16')
