@@ -369,9 +369,10 @@ GG_DEVICE void ggw_fix_row(const GgWinParams& p, const GgwRange& rg, int len, co
         l = l * corr + gg_wave_sum_all(pj);
         m = mn;
         for (int c = 0; c < C; ++c) acc[c] *= corr;
+        const unsigned long long bits = gg_ballot(see);         // (not where p > 0: a NaN value counts where its probability underflows too)
         for (int k = 0; k < TK; ++k) {
             const float pk = gg_readlane(pj, k);
-            if (pk == 0.f) continue;
+            if (!((bits >> k) & 1)) continue;
             for (int c = 0; c < C; ++c)
                 if (lane + 64 * c < D) acc[c] += pk * gg_elt_f<T>(vb[(long long)(j0 + k) * p.vn + lane + 64 * c]);
         }
