@@ -4,6 +4,7 @@
 //     key j   when   j < len_b,   j <= p + right,   j >= p - left or j < sinks,   keep[b][j]
 // (a query at a negative position is padding and sees nothing).
 //     o_i = sum_j P_ij v_j,   P = softmax over the seen keys of scale q_i.k_j;   a query that sees no key gets zeros and no gradient.
+//     (a query that sees keys of score -inf alone: 0 / 0, NaN, as in any softmax; scale log2e s beyond fp32 counts as infinite)
 //     backward: D_i = dO_i.o_i,  dS_ij = P_ij (dO_i.v_j - D_i),  dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,  dv_j = sum_i P_ij dO_i
 //
 // Grouped heads: g = h / hk query heads read one key head. The kernels' ROWS are the (token, head of the group) pairs of one (batch,
@@ -18,20 +19,26 @@
 // NaN and infinities. Where a row does not see a key its probability is an exact zero, but zero times a NaN in the shared tile is NaN.
 // Keys behind the sequence's end are staged as zeros. For the rest every wave looks at its own result once, at the end: rows (dk / dv:
 // keys) whose result is not finite are computed again one by one, from memory and from what they see alone (ggw_fix_*). Finite inputs
-// never come there.
+// come there only with far scores.
+//
+// Far scores. P is exp2(fma(s, scale log2e, -m)): the rounding of m moves it by a factor of 2^(m 2^-24), and a log-sum-exp of 32 bits
+// forgets log2 of the sum beside a large m. From |m| = GGW_FAR on, where that is 2^(1/16), a row is computed again as well, with the
+// product rounded before the difference. Its log-sum-exp is m alone; dq finds log2 of the sum anew and leaves it for dk and dv.
 #pragma once
 #include "gg_element.h"
 
 #define GGW_NONE 0x20000000          // "no bound" of a window side, and (negated, doubled) the position of a row that is not there
 #define GGW_SPAN 0xf0000000u         // buffer length behind a row tile's first token; an offset of this size reads zeros
 #define GGW_LOG2E 1.4426950408889634f
+#define GGW_FAR 1048576.0f           // (see above)
+#define GGW_LOW (-3.402823466e38f)   // where the running maximum starts: any finite score is above it, or is it
 #define GGW_TAU 8.0f                 // the running maximum moves when a score exceeds it by 2^8: fewer rescales of the output, P <= 2^8
 
 struct GgWinParams {
     const unsigned short *q, *k, *v, *d_o;
     unsigned short *o, *o_lo, *dq, *dk, *dv;        // dense: o, o_lo, dq [B][n][h][D]; dk, dv [B][m][hk][D]
-    float* lse;                             // [B*hk][n*g]: log2 of the row's sum of 2^(scale log2e s); +inf for a row that sees nothing
-    float* dvec;                            // [B*hk][n*g]: D_i
+    float* lse;                             // [B*hk][n*g]: log2 of the row's sum of 2^(scale log2e s); +inf for a row that sees nothing, NaN for 0 / 0
+    float* dvec;                            // [2][B*hk][n*g]: D_i; of far rows log2 of the sum that lse does not hold
     long long qb, qh, kb, kh, vb, vh, gb, gh;       // element strides of q, k, v, dO: batch, head ...
     unsigned qn, kn, vn, gn;                        // ... and token (below 2^24)
     const int* lengths;                     // [B] or null (= m)
@@ -73,6 +80,11 @@ GG_DEVICE unsigned ggw_not_finite(const f32x16* v) {
         for (int r = 0; r < 16; ++r) s = gg_fmaf(v[i][r], 0.f, s);
     s = gg_sum_xor32(s);
     return (unsigned)gg_ballot(s != s);
+}
+// a condition of either lane of a row, as bits of the wave's 32 rows
+GG_DEVICE unsigned ggw_rows32(bool x) {
+    const unsigned long long b = gg_ballot(x);
+    return (unsigned)b | (unsigned)(b >> 32);
 }
 // A tile is 64 rows of D features as the LDS-DMA deposits them: wave instruction after wave instruction of 64 x 16 bytes, rows back to
 // back. No padding is possible, so the 16-byte vectors of a row are permuted instead: vector c lies at position c ^ ggw_swz(row) (the
@@ -241,12 +253,13 @@ GG_DEVICE bool ggw_sees(const GgwWave& w, int sinks, int j) { return j <= w.hi &
 
 // ---- forward -------------------------------------------------------------------------------------------------------
 
-// scores that their row does not see become -inf; keep: this item's key mask or null
-GG_DEVICE void ggw_mask(f32x16* st, int blocks, const GgwWave& w, int sinks, int j0, int len, const unsigned char* keep) {
+// scores that their row does not see become -inf; keep: this item's key mask or null. Returns whether the lane saw a key.
+GG_DEVICE bool ggw_mask(f32x16* st, int blocks, const GgwWave& w, int sinks, int j0, int len, const unsigned char* keep) {
     const int lane = threadIdx.x & 63, hi = lane >> 5;
     unsigned long long bits = ~0ull;
     if (keep) bits = gg_ballot(j0 + lane < len && keep[j0 + lane]);
     bits >>= 4 * hi;
+    bool saw = false;
 #pragma unroll
     for (int jb = 0; jb < 2; ++jb)
         if (jb < blocks) {
@@ -255,8 +268,10 @@ GG_DEVICE void ggw_mask(f32x16* st, int blocks, const GgwWave& w, int sinks, int
                 const int jr = jb * 32 + (r & 3) + 8 * (r >> 2);
                 const bool see = ggw_sees(w, sinks, j0 + jr + 4 * hi) && ((bits >> jr) & 1);
                 st[jb][r] = see ? st[jb][r] : -__builtin_inff();
+                saw |= see;
             }
         }
+    return saw;
 }
 // one softmax step over N 32-key blocks of scores: running maximum m (log2 domain), this lane's part of the row's sum l, the probabilities
 // packed as the next product's operands. The maximum moves (and O with it) only when a score exceeds it by 2^GGW_TAU.
@@ -302,11 +317,20 @@ GG_DEVICE void ggw_store_o(const GgWinParams& p, long long at, f32x4 x) {
     *(u16x4*)(p.o + at) = hi;
     if (p.o_lo) *(u16x4*)(p.o_lo + at) = lo;
 }
+// A row that saw no key: zeros, and +inf for its log-sum-exp (its P is zero everywhere in the backward). A row that saw keys and has
+// l = 0 saw scores of -inf alone: NaN. Where rows are joined, a part that saw no key has the maximum -inf, any other GGW_LOW or more.
+GG_DEVICE float ggw_inverse(float l, bool saw) { return l == 0.f ? (saw ? __builtin_nanf("") : 0.f) : 1.f / l; }
+GG_DEVICE bool ggw_far(float m) { return fabsf(m) >= GGW_FAR && fabsf(m) < __builtin_inff(); }
+GG_DEVICE float ggw_lse(float m, float l, bool saw) {
+    if (l == 0.f) return saw ? __builtin_nanf("") : __builtin_inff();
+    return l == l && ggw_far(m) ? m : m + log2f(l);
+}
 // the wave's 32 rows: o and the log-sum-exp, or (SPLIT) what gg_win_join_kernel takes
 template <int T, int D, bool SPLIT>
-GG_DEVICE void ggw_write_rows(const GgWinParams& p, const GgwWave& w, int bkv, int split, const f32x16* ot, float m, float l) {
+GG_DEVICE void ggw_write_rows(const GgWinParams& p, const GgwWave& w, int bkv, int split, const f32x16* ot, float m, float l, bool saw) {
     const int hi = (threadIdx.x & 63) >> 5, rows = p.n * p.g;
     l = gg_sum_xor32(l);
+    saw = gg_max_xor32(saw ? 1.f : 0.f) > 0.f;
     if (w.r >= rows) return;
     const long long at = (long long)bkv * rows + w.r;
     if (SPLIT) {
@@ -317,18 +341,18 @@ GG_DEVICE void ggw_write_rows(const GgWinParams& p, const GgwWave& w, int bkv, i
 #pragma unroll
             for (int gq = 0; gq < 4; ++gq)
                 *(f32x4*)(po + db * 32 + 8 * gq + 4 * hi) = f32x4{ot[db][4 * gq], ot[db][4 * gq + 1], ot[db][4 * gq + 2], ot[db][4 * gq + 3]};
-        if (hi == 0) { p.part_ml[2 * sp] = m; p.part_ml[2 * sp + 1] = l; }
+        if (hi == 0) { p.part_ml[2 * sp] = saw ? m : -__builtin_inff(); p.part_ml[2 * sp + 1] = l; }
         return;
     }
     const int b = bkv / p.hk, kvh = bkv - b * p.hk;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = ggw_inverse(l, saw);
     const long long orow = (((long long)b * p.n + w.row.token) * p.h + kvh * p.g + w.row.head) * D;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
         for (int gq = 0; gq < 4; ++gq)
             ggw_store_o<T>(p, orow + db * 32 + 8 * gq + 4 * hi, f32x4{ot[db][4 * gq] * inv, ot[db][4 * gq + 1] * inv, ot[db][4 * gq + 2] * inv, ot[db][4 * gq + 3] * inv});
-    if (hi == 0 && p.lse) p.lse[at] = l == 0.f ? __builtin_inff() : m + log2f(l);
+    if (hi == 0 && p.lse) p.lse[at] = ggw_lse(m, l, saw);
 }
 template <int KK>
 GG_DEVICE void ggw_load_row(u16x8* f, const unsigned short* base, long long head_stride, unsigned token_stride, int head, int token) {
@@ -347,6 +371,13 @@ GG_DEVICE float ggw_dot(const unsigned short* x, const unsigned short* y) {
     }
     return s;
 }
+// a score in log2 units, rounded before anything is taken from it (the same bits for a pair wherever it is computed again)
+template <int T, int D>
+GG_DEVICE float ggw_score(const unsigned short* q, const unsigned short* k, float a2) {
+#pragma clang fp contract(off)
+    const float s = ggw_dot<T, D>(q, k);
+    return s * a2;
+}
 // One row again, by one wave, from the keys it sees alone: tiles i0, i0 + step .. of TK keys, a key a lane for the scores, a feature a lane
 // for the output. fix[D] = sum of p v, relative to the maximum m, l the sum of p.
 template <int T, int D, int TK>
@@ -356,13 +387,13 @@ GG_DEVICE void ggw_fix_row(const GgWinParams& p, const GgwRange& rg, int len, co
     const int lane = threadIdx.x & 63;
     const float a2 = p.scale * GGW_LOG2E;
     float acc[C];
-    m = -1.0e30f;
+    m = GGW_LOW;
     l = 0.f;
     for (int c = 0; c < C; ++c) acc[c] = 0.f;
     for (int i = i0; i < i1; i += step) {
         const int j0 = ggw_tile_at(rg, i) * TK, j = j0 + lane;
         const bool see = lane < TK && j < len && j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && (!keep || keep[j]);
-        const float x = see ? ggw_dot<T, D>(q, kb + (long long)j * p.kn) * a2 : -__builtin_inff();
+        const float x = see ? ggw_score<T, D>(q, kb + (long long)j * p.kn, a2) : -__builtin_inff();
         float mx = x;
         for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, gg_shfl_xor(mx, o));
         const float mn = fmaxf(m, mx), corr = gg_exp2f(m - mn), pj = see ? gg_exp2f(x - mn) : 0.f;
@@ -453,7 +484,8 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, D == 128 ? 2 : 3) void gg_win_fwd_kernel(GgWinP
         ggw_dma<D>(vb, j0, len, p.vn, vo, sV[buf], wave);
     };
     const float a2 = p.scale * GGW_LOG2E;
-    float m = -1.0e30f, l = 0.f;
+    float m = GGW_LOW, l = 0.f;
+    bool saw = false;
     f32x16 ot[DB], st[2];
     u16x8 pf[4];
 #pragma unroll
@@ -474,14 +506,14 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, D == 128 ? 2 : 3) void gg_win_fwd_kernel(GgWinP
         for (int r = 0; r < 16; ++r) st[0][r] = st[1][r] = 0.f;
         ggw_pipe<2 * KK>([&](int s) { return ggw_frag<D>(sK[buf], (s & 1) * 32, s >> 1, lo); },
                          [&](int s, u16x8 x) { st[s & 1] = ggw_mfma<T>(x, qf[s >> 1], st[s & 1]); });
-        if (!ggw_whole(w, p.sinks, j0, j0 + 63)) ggw_mask(st, 2, w, p.sinks, j0, len, keep);
+        saw |= ggw_whole(w, p.sinks, j0, j0 + 63) ? true : ggw_mask(st, 2, w, p.sinks, j0, len, keep);
         ggw_softmax<T, DB, 2>(st, pf, ot, m, l, a2);
         ggw_pipe<4 * DB>([&](int s) { return ggw_frag_tr<D>(sV[buf], (s % DB) * 32, 16 * (s / DB), lo); },
                          [&](int s, u16x8 x) { ot[s % DB] = ggw_mfma<T>(x, pf[s / DB], ot[s % DB]); });
     }
-    const unsigned bad = ggw_not_finite<DB>(ot);
+    const unsigned bad = ggw_not_finite<DB>(ot) | ggw_rows32(saw && ggw_far(m));
     if (__builtin_expect(bad != 0, 0)) ggw_fix_rows<T, D, 64>(p, w, rg, len, b, kvh, keep, ta, tb, 1, bad, sFix[wave], ot, m, l);
-    ggw_write_rows<T, D, SPLIT>(p, w, bkv, split, ot, m, l);
+    ggw_write_rows<T, D, SPLIT>(p, w, bkv, split, ot, m, l, saw);
 }
 
 // ---- forward with few rows ------------------------------------------------------------------------------------------
@@ -514,7 +546,8 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_few_kernel(GgWinParams p) {
     u16x8 qf[KK], pf[2];
     ggw_load_row<KK>(qf, p.q + b * p.qb, p.qh, p.qn, kvh * p.g + w.row.head, w.row.token);
     const float a2 = p.scale * GGW_LOG2E;
-    float m = -1.0e30f, l = 0.f;
+    float m = GGW_LOW, l = 0.f;
+    bool saw = false;
     f32x16 ot[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -548,24 +581,25 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_few_kernel(GgWinParams p) {
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) st = ggw_mfma<T>(kf[kk], qf[kk], st);
         if (i + 4 < tb) load(i + 4);
-        if (!ggw_whole(w, p.sinks, j0, j0 + 31)) ggw_mask(&st, 1, w, p.sinks, j0, len, keep);
+        saw |= ggw_whole(w, p.sinks, j0, j0 + 31) ? true : ggw_mask(&st, 1, w, p.sinks, j0, len, keep);
         ggw_softmax<T, DB, 1>(&st, pf, ot, m, l, a2);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int db = 0; db < DB; ++db) ot[db] = ggw_mfma<T>(ggw_frag_tr<D>(sV[wave], db * 32, 16 * c, lo), pf[c], ot[db]);
     }
-    const unsigned bad = ggw_not_finite<DB>(ot);
+    const unsigned bad = ggw_not_finite<DB>(ot) | ggw_rows32(saw && ggw_far(m));
     if (__builtin_expect(bad != 0, 0)) {
         gg_wave_sync();             // (the wave's own tile is free)
         ggw_fix_rows<T, D, 32>(p, w, rg, len, b, kvh, keep, ta + wave, tb, 4, bad, (float*)sV[wave], ot, m, l);
     }
     l = gg_sum_xor32(l);
-    if (hi == 0) { sM[wave][lane] = m; sL[wave][lane] = l; }
+    saw = gg_max_xor32(saw ? 1.f : 0.f) > 0.f;
+    if (hi == 0) { sM[wave][lane] = saw ? m : -__builtin_inff(); sL[wave][lane] = l; }
     gg_sync();
     const int q = lane & 31;
-    float top = sM[0][q];
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, sM[w][q]);
+    float top = GGW_LOW;
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, sM[w][q]);
     const float f = gg_exp2f(m - top);
     for (int w = 0; w < 4; ++w) {
         if (wave == w)
@@ -586,7 +620,8 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_few_kernel(GgWinParams p) {
         if (r >= rows) break;
         float mt = sM[0][rr], lt = 0.f;
         for (int w = 1; w < 4; ++w) mt = fmaxf(mt, sM[w][rr]);
-        for (int w = 0; w < 4; ++w) lt += sL[w][rr] * gg_exp2f(sM[w][rr] - mt);
+        const bool any = mt >= GGW_LOW;
+        for (int w = 0; w < 4; ++w) lt += sL[w][rr] * gg_exp2f(sM[w][rr] - fmaxf(mt, GGW_LOW));
         const f32x4 x = *(const f32x4*)&sO[rr][d];
         const long long at = (long long)bkv * rows + r;
         if (p.splits > 1) {
@@ -594,10 +629,10 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_few_kernel(GgWinParams p) {
             *(f32x4*)(p.part_o + sp * D + d) = x;
             if (d == 0) { p.part_ml[2 * sp] = mt; p.part_ml[2 * sp + 1] = lt; }
         } else {
-            const float inv = lt == 0.f ? 0.f : 1.f / lt;
+            const float inv = ggw_inverse(lt, any);
             const int token = (int)((unsigned)r / (unsigned)p.g), head = r - token * p.g;
             ggw_store_o<T>(p, (((long long)b * p.n + token) * p.h + kvh * p.g + head) * D + d, x * inv);
-            if (d == 0 && p.lse) p.lse[at] = lt == 0.f ? __builtin_inff() : mt + log2f(lt);
+            if (d == 0 && p.lse) p.lse[at] = ggw_lse(mt, lt, any);
         }
     }
 }
@@ -612,14 +647,15 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_join_kernel(GgWinParams p) {
     const int rows = p.n * p.g, grp = threadIdx.x / Q, d = threadIdx.x % Q * 4, share = grp % p.join;
     const long long all = (long long)p.B * p.hk * rows;
     const long long at0 = (long long)blockIdx.x * (R / p.join) + grp / p.join, at = at0 < all ? at0 : all - 1;
-    float top = -1.0e30f;
+    float top = -__builtin_inff();
 #pragma unroll 4
     for (int s = share; s < p.splits; s += p.join) top = fmaxf(top, p.part_ml[2 * (s * all + at)]);
+    float base = fmaxf(top, GGW_LOW);
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
 #pragma unroll 4
     for (int s = share; s < p.splits; s += p.join) {
-        const float f = gg_exp2f(p.part_ml[2 * (s * all + at)] - top);
+        const float f = gg_exp2f(p.part_ml[2 * (s * all + at)] - base);
         l += f * p.part_ml[2 * (s * all + at) + 1];
         x += f * *(const f32x4*)(p.part_o + (s * all + at) * D + d);
     }
@@ -629,20 +665,22 @@ GG_KERNEL GG_LAUNCH_BOUNDS(256) void gg_win_join_kernel(GgWinParams p) {
         gg_sync();
         if (share) return;
         for (int k = 1; k < p.join; ++k) top = fmaxf(top, sM[grp + k]);
+        base = fmaxf(top, GGW_LOW);
         x = f32x4{0.f, 0.f, 0.f, 0.f};
         l = 0.f;
         for (int k = 0; k < p.join; ++k) {
-            const float f = gg_exp2f(sM[grp + k] - top);
+            const float f = gg_exp2f(sM[grp + k] - base);
             l += f * sL[grp + k];
             x += f * *(const f32x4*)&sO[grp + k][d];
         }
     }
     if (at0 >= all) return;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const bool saw = top >= GGW_LOW;
+    const float inv = ggw_inverse(l, saw);
     const int bkv = (int)(at / rows), r = (int)(at - (long long)bkv * rows);
     const int b = bkv / p.hk, kvh = bkv - b * p.hk, token = r / p.g, head = r - token * p.g;
     ggw_store_o<T>(p, (((long long)b * p.n + token) * p.h + kvh * p.g + head) * D + d, x * inv);
-    if (d == 0 && p.lse) p.lse[at] = l == 0.f ? __builtin_inff() : top + log2f(l);
+    if (d == 0 && p.lse) p.lse[at] = ggw_lse(top, l, saw);
 }
 
 // ---- backward, part 1: dq and D ---------------------------------------------------------------------------------------
@@ -674,20 +712,30 @@ GG_DEVICE void ggw_ds(f32x16& st, const f32x16& dp, float a2, float lse, bool ma
     }
 }
 
-// one row's dq again, by one wave, from the keys it sees alone: fix[D] = sum of dS k
+// one row's dq again, by one wave, from the keys it sees alone: fix[D] = sum of dS k. Of a far row (lse its largest score) log2 of the
+// sum first, which is returned.
 template <int T, int D>
-GG_DEVICE void ggw_fix_dq(const GgWinParams& p, const GgwRange& rg, int len, const unsigned char* keep, const unsigned short* q,
+GG_DEVICE float ggw_fix_dq(const GgWinParams& p, const GgwRange& rg, int len, const unsigned char* keep, const unsigned short* q,
                           const unsigned short* g, const unsigned short* kb, const unsigned short* vb, int pos, float lse, float dsum, float* fix) {
     constexpr int C = (D + 63) / 64;
     const int lane = threadIdx.x & 63;
     const float a2 = p.scale * GGW_LOG2E;
     float acc[C];
     for (int c = 0; c < C; ++c) acc[c] = 0.f;
+    auto sees = [&](int j) { return j < len && j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && (!keep || keep[j]); };
+    float log_sum = 0.f;
+    if (ggw_far(lse)) {
+        for (int i = 0; i < rg.nt; ++i) {
+            const int j = ggw_tile_at(rg, i) * 64 + lane;
+            log_sum += gg_wave_sum_all(sees(j) ? gg_exp2f(ggw_score<T, D>(q, kb + (long long)j * p.kn, a2) - lse) : 0.f);
+        }
+        log_sum = log2f(log_sum);
+    }
     for (int i = 0; i < rg.nt; ++i) {
         const int j0 = ggw_tile_at(rg, i) * 64, j = j0 + lane;
-        const bool see = j < len && j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && (!keep || keep[j]);
+        const bool see = sees(j);
         float ds = 0.f;
-        if (see) ds = gg_exp2f(ggw_dot<T, D>(q, kb + (long long)j * p.kn) * a2 - lse) * (ggw_dot<T, D>(g, vb + (long long)j * p.vn) - dsum);
+        if (see) ds = gg_exp2f(ggw_score<T, D>(q, kb + (long long)j * p.kn, a2) - lse - log_sum) * (ggw_dot<T, D>(g, vb + (long long)j * p.vn) - dsum);
         const unsigned long long bits = gg_ballot(see);
         for (int k = 0; k < 64; ++k) {
             const float dk = gg_readlane(ds, k);
@@ -698,6 +746,7 @@ GG_DEVICE void ggw_fix_dq(const GgWinParams& p, const GgwRange& rg, int len, con
     }
     for (int c = 0; c < C; ++c)
         if (lane + 64 * c < D) fix[lane + 64 * c] = acc[c];
+    return log_sum;
 }
 
 template <int T, int D>
@@ -781,14 +830,16 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dq_kernel(GgWinParams p) {
                              [&](int s, u16x8 x) { dqt[s % DB] = ggw_mfma<T>(x, sf[s / DB], dqt[s % DB]); });
         }
     }
-    const unsigned bad = ggw_not_finite<DB>(dqt);
+    const unsigned bad = ggw_not_finite<DB>(dqt) | ggw_rows32(ggw_far(lse));
     if (__builtin_expect(bad != 0, 0))
         for (int k = 0; k < 32; ++k) {
             if (!((bad >> k) & 1) || w.r0 + k >= rows) continue;
             const int token = (w.r0 + k) / p.g, head = kvh * p.g + w.r0 + k - token * p.g, pos = token + len - p.n;
-            ggw_fix_dq<T, D>(p, rg, len, keep, p.q + b * p.qb + head * p.qh + (long long)token * p.qn,
+            const float log_sum = ggw_fix_dq<T, D>(
+                             p, rg, len, keep, p.q + b * p.qb + head * p.qh + (long long)token * p.qn,
                              p.d_o + b * p.gb + head * p.gh + (long long)token * p.gn, kb, vb, pos < 0 ? -2 * GGW_NONE : pos, gg_readlane(lse, k),
                              gg_readlane(dsum, k), sFix[wave]);
+            if (lane == 0) p.dvec[(long long)p.B * p.hk * rows + (long long)bkv * rows + w.r0 + k] = log_sum;
             ggw_take_fix<DB>(dqt, sFix[wave], (lane & 31) == k);
         }
     ggw_write_dq<T, D>(p, w, b, hq, dqt);
@@ -835,7 +886,8 @@ GG_DEVICE void ggw_fix_dkv(const GgWinParams& p, const unsigned short* qb, const
         float pr = 0.f, ds = 0.f;
         if (see || (r <= rb && lse != lse)) {
             const long long qo = hd * p.qh + (long long)tok * p.qn, go = hd * p.gh + (long long)tok * p.gn;
-            pr = gg_exp2f(ggw_dot<T, D>(qb + qo, k) * a2 - lse);
+            const float log_sum = ggw_far(lse) ? p.dvec[(long long)p.B * p.hk * p.n * p.g + stat + rc] : 0.f;
+            pr = gg_exp2f(ggw_score<T, D>(qb + qo, k, a2) - lse - log_sum);
             ds = pr * (ggw_dot<T, D>(gb + go, v) - p.dvec[stat + rc]);
         }
         const unsigned long long bits = gg_ballot(r <= rb && !(lse == __builtin_inff()) && j <= pos + p.right && (j >= pos - p.left || j < p.sinks));
@@ -940,6 +992,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
     const GgwLane lanes = ggw_lane<D>();
     float r_lse = 0.f, r_d = 0.f;
     int r_pos = 0;
+    bool far = false;
     auto fetch = [&](int i0, int buf) {
         const GgBufS bq = gg_make_bufs(qb + (unsigned long long)(unsigned)ft * p.qn, GGW_SPAN), bg = gg_make_bufs(gb + (unsigned long long)(unsigned)ft * p.gn, GGW_SPAN);
         const bool all = i0 + 63 <= rb;
@@ -961,6 +1014,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
         const bool in = r <= rb;
         const unsigned at = in ? r : rb;
         r_lse = in ? lse[at] : __builtin_inff();
+        far |= ggw_far(r_lse);
         r_d = in ? dvec[at] : 0.f;
         r_pos = in ? rt + shift : -2 * GGW_NONE;
         rt += step_t;
@@ -1042,7 +1096,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
                              });
         }
     }
-    const unsigned bad = ggw_not_finite<2 * DB>(acc);
+    const unsigned bad = gg_wave_any(far) ? ~0u : ggw_not_finite<2 * DB>(acc);       // (a far row may have reached any key)
     if (__builtin_expect(bad != 0, 0))
         for (int k = 0; k < 32; ++k) {
             const int j = kj0 + k;

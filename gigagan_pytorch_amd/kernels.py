@@ -1607,7 +1607,7 @@ def window_bwd(q, k, v, o, o_lo, lse, d_o, scale: float, left: int, right: int, 
     q, k, v, d_o = _attend4(q, h // hk), _attend4(k), _attend4(v), _attend4(d_o, h // hk)
     # dense as the forward left them (a saved-tensor hook may hand them back in another layout: a copy then)
     o, o_lo, lse = o.transpose(1, 2).contiguous(), o_lo.contiguous(), lse.contiguous()
-    dvec = torch.empty_like(lse)
+    dvec = torch.empty((2, *lse.shape), dtype=torch.float32, device=q.device)
     D = _window_desc(q, k, v, o, o_lo, lse, scale, left, right, sinks, lengths, key_mask, d_o, dq, dk, dv, dvec)
     with _on_device(L, q):
         nbytes = L.lib.gg_window_workspace_bytes(D, 1)

@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define GG_ABI_VERSION 13
+#define GG_ABI_VERSION 14
 
 int gg_version(void);
 const char* gg_last_error(void);
@@ -526,9 +526,9 @@ int gg_rotary(const gg_rotary_desc* d, void* stream);
  * key j when j < len_b, j <= p + right, (j >= p - left or j < sinks) and key_mask[b][j] (bytes, batch stride mask_stride; optional);
  * left / right < 0 = no bound. A query that sees no key, or at p < 0, gets zeros and no gradient.
  *   forward:  o dense [B][n][h][d]; for the backward o_lo like o (what o's rounding took off) and lse fp32 [B*hk][n*h/hk] (log2 domain,
- *             +inf for a row that sees nothing), both optional
+ *             +inf for a row that sees nothing, NaN for one whose seen scores are all -inf), both optional
  *   backward: reads q, k, v, o, o_lo, lse and d_o (strides g_strides), writes dq dense [B][n][h][d], dk, dv dense [B][m][hk][d] (every element)
- *             and dvec fp32 [B*hk][n*h/hk] (scratch)
+ *             and dvec fp32 [2][B*hk][n*h/hk] (scratch; one such array before ABI 14)
  * Both take a workspace of gg_window_workspace_bytes(d, backward) bytes (0: none, or sizes that the calls refuse), 16-byte aligned, free
  * again when the call's work on `stream` is done. Results do not depend on what runs beside: no atomics. */
 #define GG_WINDOW_MAX_STRIDE (1 << 24)

@@ -11,7 +11,7 @@ from test_transformer_ops import DT, att_ref, gen, half_step, normal, qkv, seen,
 WHERE = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
 where = pytest.mark.parametrize('where', WHERE)
 # queries and keys for the three forward kernels: many rows, few rows, few rows with the keys split over workgroups
-SHAPES = [(40, 90), (3, 90), (1, 600)]
+SHAPES = [(34, 70), (3, 70), (1, 600)]
 shapes = pytest.mark.parametrize('n,m', SHAPES)
 
 
@@ -37,3 +37,71 @@ def test_a_value_of_underflowed_probability_counts(where, n, m, fill):
     ref, tol = att_ref(q, k, v, 1.0, seen(1, n, m, (None, 0), 0, None, None, where))[0]
     within(got[..., others], ref[..., others], tol[..., others])
     within(got[:, :, ~sees], ref[:, :, ~sees], tol[:, :, ~sees])
+
+
+def softmax_grads(q, k, v, do, scale, ok):
+    """o, dq, dk, dv in 64 bits by automatic differentiation, masked rows zero"""
+    q, k, v = (t.detach().double().requires_grad_() for t in (q, k, v))
+    grp = q.shape[1] // k.shape[1]
+    x = q @ k.repeat_interleave(grp, 1).mT * scale
+    x = x.masked_fill(~ok[:, None], -math.inf)
+    some = ok.any(-1)[:, None, :, None]
+    p = x.masked_fill(~some, 0.0).softmax(-1) * some
+    o = p @ v.repeat_interleave(grp, 1)
+    return [o.detach(), *torch.autograd.grad(o, (q, k, v), do.double())]
+
+
+@where
+@shapes
+@pytest.mark.parametrize('exponent', [21, 105])
+@pytest.mark.parametrize('sign', [-1, 1])
+def test_far_scores(where, n, m, exponent, sign):
+    """scores of 2^21 and 2^105 on either side, far below and above where a running maximum might start: equal ones share the probability
+    (exactly: the products are powers of two), one half as large in magnitude takes it all or has none, and so do the gradients"""
+    g = gen(21, where)
+    q, k, v, do = (t.clone() for t in qkv(1, 2, 1, n, m, 32, 'bf16', g))
+    q.zero_()
+    k.zero_()
+    q[..., 3] = 2.0 ** (exponent // 2)
+    k[..., 3] = sign * 2.0 ** (exponent - exponent // 2)
+    k[0, 0, 7, 3] *= 0.5                                # the row's largest score below zero, one that does not count above
+    window = (None, 0)
+    ok = seen(1, n, m, window, 0, None, None, where)
+    # numbers of the gradients' own size: dS k and dS q are up to 2^53 here
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = ops.impl.window_attention(*leaves, scale=1.0, window=window)
+    got = [o, *torch.autograd.grad(o, leaves, do)]
+    ref = softmax_grads(q, k, v, do, 1.0, ok)
+    u = half_step(torch.bfloat16)
+    P = (torch.where(ok[:, None], q.double() @ k.double().mT, torch.full((), -1e300, dtype=torch.float64, device=where))).softmax(-1) * ok[:, None]
+    # the row's pass is fp32: 2^-18 covers its sums of up to 600 terms; o's own rounding is kept for D. The results are rounded once.
+    e = 2.0 ** -18
+    size = P * ((do.abs().double() @ v.abs().double().mT) + (do.abs().double() * (P @ v.abs().double())).sum(-1, keepdim=True))
+    tol = [u * ref[0].abs() + e * (P @ v.abs().double()), u * ref[1].abs() + e * (size @ k.abs().double()),
+           u * ref[2].abs() + e * (size.mT @ q.abs().double()).sum(1, keepdim=True),
+           u * ref[3].abs() + e * (P.mT @ do.abs().double()).sum(1, keepdim=True)]
+    for name, a, b, t in zip(('o', 'dq', 'dk', 'dv'), got, ref, tol):
+        within(a, b, t, name)
+    with torch.no_grad():
+        assert torch.equal(ops.impl.window_attention(*leaves, scale=1.0, window=window), o)
+
+
+@where
+@shapes
+def test_scores_of_minus_infinity_alone(where, n, m):
+    """a query whose seen keys all score -inf has 0 / 0 as in any softmax, one that sees no key zeros; a single finite score among them takes all"""
+    g = gen(22, where)
+    q, k, v, do = (t.clone() for t in qkv(3, 2, 1, n, m, 32, 'bf16', g))
+    q[..., 0] = 1.0
+    k[..., 0] = -math.inf
+    mask = torch.ones((3, m), dtype=torch.bool, device=where)
+    mask[1] = False
+    k[2, 0, 0] = 0
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = ops.impl.window_attention(*leaves, scale=0.5, key_mask=mask)
+    assert torch.isnan(o[0]).all() and not o[1].any()
+    within(o[2], v[2, :, :1].expand_as(o[2]), 0.0)
+    dq, dk, dv = torch.autograd.grad(o, leaves, do)
+    assert torch.isnan(dq[0]).all() and torch.isnan(dk[0]).all() and torch.isnan(dv[0]).all()
+    assert not any(t[1].any() for t in (dq, dk, dv))
+    within(dv[2, 0, 0], do[2].double().sum((0, 1)), half_step(torch.bfloat16) * do[2].double().sum((0, 1)).abs() + 2.0 ** -18 * do[2].double().abs().sum((0, 1)))
