@@ -32,7 +32,10 @@
 #define GGW_LOG2E 1.4426950408889634f
 #define GGW_FAR 1048576.0f           // (see above)
 #define GGW_LOW (-3.402823466e38f)   // where the running maximum starts: any finite score is above it, or is it
-#define GGW_TAU 8.0f                 // the running maximum moves when a score exceeds it by 2^8: fewer rescales of the output, P <= 2^8
+// What P is taken relative to ("the running maximum") moves when a score exceeds it by TAU (in log2): fewer rescales of the output. It
+// moves to LEAD below the largest score: the largest P is 2^LEAD .. 2^TAU. IEEE half, whose least number is 2^-24, has 2^15 to spare
+// above one; bf16 has fp32's range.
+template <int T> struct GgwExp { static constexpr float LEAD = T == GG_ELT_F16 ? 7.f : 0.f, TAU = LEAD + 8.f; };
 
 struct GgWinParams {
     const unsigned short *q, *k, *v, *d_o;
@@ -61,14 +64,39 @@ GG_DEVICE f32x16 ggw_mfma(u16x8 a, u16x8 b, f32x16 c) {
     if constexpr (T == GG_ELT_BF16) return gg_mfma_32x32x16_bf16(a, b, c);
     else return gg_mfma_32x32x16_f16(a, b, c);
 }
-// registers 8c .. 8c + 7 of a result, rounded to 16 bits: the B operand of the follow-up contraction (P and dS are rounded to the operands'
-// type for the matrix pipe, as any 16-bit attention does; their sums stay fp32)
+// registers 8c .. 8c + 7 of a result, rounded to 16 bits: the B operand of the follow-up contraction. P and dS are rounded to the operands'
+// type because the matrix pipe takes both operands in one type, and an fp32 product runs at a sixteenth of its rate; their sums stay
+// fp32. Each rounding is half a step of the type relative to the value (32 captions of 78 tokens, bf16: o and gradients are 0.0022 -
+// 0.0025 from 64 bits in the mean, 0.0016 - 0.0017 with P and dS in fp32).
 template <int T>
 GG_DEVICE u16x8 ggw_pack8(const f32x16& v, int c) {
     u16x8 f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = gg_elt<T>(v[8 * c + e]);
     return f;
+}
+// dS in IEEE half. P (dP - D) of small gradients lies below half's least number, so a lane keeps a power of two for its row (dk / dv: its
+// key) that dS is multiplied with before it is rounded, and its sums with it: 2^e, lowered where a larger dS would leave the range,
+// so that the largest so far is 2^8 .. 2^15 (what is rounded to half's least number is 2^-32 of it, or less). bf16 needs none.
+struct GgwScale { int e; };
+GG_DEVICE float ggw_pow2(int e) { return __builtin_bit_cast(float, (unsigned)(127 + e) << 23); }       // -126 <= e <= 127
+template <int N>
+GG_DEVICE void ggw_rescale(GgwScale& s, f32x16& ds, f32x16* sums) {
+    float mx = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fabsf(ds[r]));
+    mx = gg_max_xor32(mx);
+    if (!gg_wave_any(mx >= 32768.f)) return;
+    const bool move = mx >= 32768.f && mx < __builtin_inff();          // (what is infinite is computed again at the end)
+    const int k = move ? (int)(__builtin_bit_cast(unsigned, mx) >> 23) - 127 - 8 : 0;
+    const float f = ggw_pow2(-k);
+    s.e -= k;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ds[r] *= f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sums[i][r] *= f;
 }
 // which of the wave's 32 rows (columns of the transposed results) hold something that is not finite, as bits
 template <int N>
@@ -274,7 +302,7 @@ GG_DEVICE bool ggw_mask(f32x16* st, int blocks, const GgwWave& w, int sinks, int
     return saw;
 }
 // one softmax step over N 32-key blocks of scores: running maximum m (log2 domain), this lane's part of the row's sum l, the probabilities
-// packed as the next product's operands. The maximum moves (and O with it) only when a score exceeds it by 2^GGW_TAU.
+// packed as the next product's operands. The maximum moves (and O with it) only when a score exceeds it by TAU.
 template <int T, int DB, int N>
 GG_DEVICE void ggw_softmax(f32x16* st, u16x8* pf, f32x16* ot, float& m, float& l, float a2) {
     float mx = -__builtin_inff();
@@ -283,8 +311,8 @@ GG_DEVICE void ggw_softmax(f32x16* st, u16x8* pf, f32x16* ot, float& m, float& l
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[jb][r]);
     mx = gg_max_xor32(mx) * a2;
-    if (gg_wave_any(mx > m + GGW_TAU)) {
-        const float mn = fmaxf(m, mx), corr = gg_exp2f(m - mn);
+    if (gg_wave_any(mx > m + GgwExp<T>::TAU)) {
+        const float mn = fmaxf(m, mx - GgwExp<T>::LEAD), corr = gg_exp2f(m - mn);
         l *= corr;
         m = mn;
 #pragma unroll
@@ -699,10 +727,10 @@ GG_DEVICE void ggw_write_dq(const GgWinParams& p, const GgwWave& w, int b, int h
             *(u16x4*)(row + db * 32 + 8 * gq) = o4;
         }
 }
-// dS of one 32-key block from its scores and dP - D, in the scores' place
-GG_DEVICE void ggw_ds(f32x16& st, const f32x16& dp, float a2, float lse, bool masked, const GgwWave& w, int sinks, int j, unsigned long long bits) {
+// dS (times 2^e where neg_lse = e - lse) of one 32-key block from its scores and dP - D, in the scores' place
+GG_DEVICE void ggw_ds(f32x16& st, const f32x16& dp, float a2, float neg_lse, bool masked, const GgwWave& w, int sinks, int j, unsigned long long bits) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) st[r] = gg_exp2f(gg_fmaf(st[r], a2, -lse)) * dp[r];
+    for (int r = 0; r < 16; ++r) st[r] = gg_exp2f(gg_fmaf(st[r], a2, neg_lse)) * dp[r];
     if (masked) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -792,6 +820,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dq_kernel(GgWinParams p) {
         ggw_dma<D>(kb, j0, len, p.kn, ko, sK[buf], wave);
         ggw_dma<D>(vb, j0, len, p.vn, vo, sV[buf], wave);
     };
+    GgwScale sc = {64};
     f32x16 dqt[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -824,12 +853,18 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dq_kernel(GgWinParams p) {
                                  if (s & 1) dp = ggw_mfma<T>(x, gf[s >> 1], dp);
                                  else st = ggw_mfma<T>(x, qf[s >> 1], st);
                              });
-            ggw_ds(st, dp, a2, lse, masked, w, p.sinks, j0 + jb * 32 + 4 * hi, bits >> (jb * 32));
+            ggw_ds(st, dp, a2, T == GG_ELT_F16 ? (float)sc.e - lse : -lse, masked, w, p.sinks, j0 + jb * 32 + 4 * hi, bits >> (jb * 32));
+            if constexpr (T == GG_ELT_F16) ggw_rescale<DB>(sc, st, dqt);
             const u16x8 sf[2] = {ggw_pack8<T>(st, 0), ggw_pack8<T>(st, 1)};
             ggw_pipe<2 * DB>([&](int s) { return ggw_frag_tr<D>(sK[buf], (s % DB) * 32, jb * 32 + 16 * (s / DB), lo); },
                              [&](int s, u16x8 x) { dqt[s % DB] = ggw_mfma<T>(x, sf[s / DB], dqt[s % DB]); });
         }
     }
+    if constexpr (T == GG_ELT_F16)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dqt[db][r] *= ggw_pow2(-sc.e);
     const unsigned bad = ggw_not_finite<DB>(dqt) | ggw_rows32(ggw_far(lse));
     if (__builtin_expect(bad != 0, 0))
         for (int k = 0; k < 32; ++k) {
@@ -952,6 +987,9 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
     const float a2 = p.scale * GGW_LOG2E;
     f32x16 acc[2 * DB];                     // dk, dv
     f32x16 *dkt = acc, *dvt = acc + DB;
+    // half: P for dv is 2^14 P (a constant does: P <= 1), dS = P (dP - D) 2^e
+    constexpr int PE = T == GG_ELT_F16 ? 14 : 0;
+    GgwScale sc = {64};
 
     const unsigned short* qb = p.q + b * p.qb + (long long)kvh * p.g * p.qh;
     const unsigned short* gb = p.d_o + b * p.gb + (long long)kvh * p.g * p.gh;
@@ -1015,6 +1053,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
         const unsigned at = in ? r : rb;
         r_lse = in ? lse[at] : __builtin_inff();
         far |= ggw_far(r_lse);
+        r_lse -= (float)PE;
         r_d = in ? dvec[at] : 0.f;
         r_pos = in ? rt + shift : -2 * GGW_NONE;
         rt += step_t;
@@ -1068,6 +1107,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
                                  if (s & 1) dp = ggw_mfma<T>(x, vf[s >> 1], dp);
                                  else st = ggw_mfma<T>(x, kf[s >> 1], st);
                              });
+            const float ps = T == GG_ELT_F16 ? ggw_pow2(sc.e - PE) : 1.f;
 #pragma unroll
             for (int gq = 0; gq < 4; ++gq) {
                 const int at = ib * 32 + 8 * gq + 4 * hi;
@@ -1076,7 +1116,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
                 for (int e = 0; e < 4; ++e) {
                     const int r = 4 * gq + e;
                     st[r] = gg_exp2f(gg_fmaf(st[r], a2, -ls[e]));
-                    dp[r] = st[r] * (dp[r] - dd[e]);
+                    dp[r] = st[r] * (T == GG_ELT_F16 ? (dp[r] - dd[e]) * ps : dp[r] - dd[e]);
                 }
                 if (!full)
 #pragma unroll
@@ -1087,6 +1127,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
                         dp[r] = see ? dp[r] : 0.f;
                     }
             }
+            if constexpr (T == GG_ELT_F16) ggw_rescale<DB>(sc, dp, dkt);
             const u16x8 pf[2] = {ggw_pack8<T>(st, 0), ggw_pack8<T>(st, 1)}, sf[2] = {ggw_pack8<T>(dp, 0), ggw_pack8<T>(dp, 1)};
             ggw_pipe<4 * DB, D == 128 ? 2 : 4>([&](int s) { return ggw_frag_tr<D>(s & 1 ? sQ[buf] : sG[buf], (s / 2 % DB) * 32, ib * 32 + 16 * (s / (2 * DB)), lo); },
                              [&](int s, u16x8 x) {
@@ -1096,6 +1137,14 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
                              });
         }
     }
+    if constexpr (T == GG_ELT_F16)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                dkt[db][r] *= ggw_pow2(-sc.e);
+                dvt[db][r] *= ggw_pow2(-PE);
+            }
     const unsigned bad = gg_wave_any(far) ? ~0u : ggw_not_finite<2 * DB>(acc);       // (a far row may have reached any key)
     if (__builtin_expect(bad != 0, 0))
         for (int k = 0; k < 32; ++k) {

@@ -105,3 +105,43 @@ def test_scores_of_minus_infinity_alone(where, n, m):
     assert torch.isnan(dq[0]).all() and torch.isnan(dk[0]).all() and torch.isnan(dv[0]).all()
     assert not any(t[1].any() for t in (dq, dk, dv))
     within(dv[2, 0, 0], do[2].double().sum((0, 1)), half_step(torch.bfloat16) * do[2].double().sum((0, 1)).abs() + 2.0 ** -18 * do[2].double().abs().sum((0, 1)))
+
+
+@where
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+@pytest.mark.parametrize('exponent', [0, -13, 9])
+@pytest.mark.parametrize('shape', [(1, 2, 1, 64, 1024, 32, (None, None)), (1, 1, 1, 130, 130, 64, (None, 0)), (1, 2, 2, 40, 300, 128, (200, 0))])
+def test_gradients_of_any_size(where, dtype, exponent, shape):
+    """an incoming gradient of 2^-13 gives 2^-13 times the gradients of one, each rounded once to the result's type: nothing on the way is
+    lost to half's subnormal numbers, or to its range with 2^9"""
+    B, h, hk, n, m, d, window = shape
+    dt = DT[dtype]
+    q, k, v, do = qkv(B, h, hk, n, m, d, dtype, gen(23, where))
+    if dtype == 'fp16' and exponent > 0:
+        v = v * 2.0 ** -4                               # (results that half can hold)
+        q, k = q * 0.5, k * 0.5
+    small = (do * 2.0 ** exponent).to(dt)               # what half keeps of it is the gradient that is meant
+    unit = small.double() * 2.0 ** -exponent
+    ok = seen(B, n, m, window, 0, None, None, where)
+    scale = d ** -0.5
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.impl.window_attention(*leaves, scale=scale, window=window), leaves, small)
+    # the tolerance of a gradient of order one, scaled; half: half a subnormal step of the result besides
+    step = 2.0 ** -25 if dtype == 'fp16' else 0.0
+    for name, got, (ref, tol) in zip(('dq', 'dk', 'dv'), grads, att_ref(q, k, v, scale, ok, unit)[1:]):
+        within(got, ref * 2.0 ** exponent, tol * 2.0 ** exponent + step, name)
+
+
+@where
+def test_half_rounds_gradients_once(where):
+    """half with gradients of 1e-4 and 1e-3: the error of dq and dk, in relative L2, is at most twice that of the exact result rounded to half
+    (P, dP's operands and dS carry relative roundings of their own)"""
+    for size in (1e-4, 1e-3):
+        q, k, v, do = qkv(1, 1, 1, 64, 1024, 32, 'fp16', gen(24, where))
+        do = (do.float() * size).half()
+        ref = softmax_grads(q, k, v, do, 32 ** -0.5, torch.ones(1, 64, 1024, dtype=torch.bool, device=where))[1:3]
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        got = torch.autograd.grad(ops.impl.window_attention(*leaves, scale=32 ** -0.5), leaves, do)[:2]
+        for a, b in zip(got, ref):
+            once = (b.half().double() - b).norm()
+            assert (a.double() - b).norm() <= 2 * once + 2.0 ** -10 * b.norm()
