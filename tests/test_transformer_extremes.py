@@ -145,3 +145,32 @@ def test_half_rounds_gradients_once(where):
         for a, b in zip(got, ref):
             once = (b.half().double() - b).norm()
             assert (a.double() - b).norm() <= 2 * once + 2.0 ** -10 * b.norm()
+
+
+@where
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+def test_row_sums_from_the_unrounded_output(where, dtype):
+    """D = dO.o is taken from o before its rounding. All scores are zero and 64 keys are seen, so P = 2^-6 is exact; o is near 8 and dP - D of order
+    |dO|, and the keys share a mean that only sum_j dS_ij = 0 keeps out of dq: with o rounded in D rows would be twice over the tolerance"""
+    g = gen(25, where)
+    dt = DT[dtype]
+    u, e = half_step(dt), 2.0 ** -24
+    n, m, d = 64, 64, 32
+    q = torch.zeros((1, 2, n, d), dtype=dt, device=where)
+    k = normal((1, 1, m, d), dt, g, shift=64.0)
+    v = normal((1, 1, m, d), dt, g, shift=8.0)
+    do = normal((1, 2, n, d), dt, g)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    dq, = torch.autograd.grad(ops.impl.window_attention(*leaves, scale=1.0), leaves[:1], do)
+    K, V, G = k.double(), v.double(), do.double()
+    o = V.mean(2, keepdim=True).expand(1, 2, n, d)
+    dP, D = G @ V.mT, (G * o).sum(-1, keepdim=True)
+    dS = (dP - D) / m
+    ref = dS @ K
+    # o in two words is off by u^2 and by fp32's sum of 64 terms; the products' sums are fp32; dS is rounded once
+    eD = (G.abs() * o.abs()).sum(-1, keepdim=True) * (u * u + (64 + d + 4) * e)
+    eS = u * dS.abs() + (eD + (d + 4) * e * (G.abs() @ V.abs().mT)) / m + 2.0 ** -20 * dS.abs()
+    within(dq, ref, eS @ K.abs() + 64 * e * (dS.abs() @ K.abs()) + u * ref.abs())
+    rounded = (G * o.to(dt).double()).sum(-1, keepdim=True)
+    lost = (rounded - D).abs() * K.mean(2, keepdim=True).abs()
+    assert (lost > 2 * (eS @ K.abs())).any()            # what the case would show
