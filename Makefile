@@ -31,8 +31,10 @@ build/gg_emu.o: tests/emu/gg_emu.cpp
 
 gigagan_pytorch_amd/libgigagan_amd.so: $(UNITS:%=build/%.o)
 	$(HIPCC) --offload-arch=gfx950 -shared -fPIC $^ -o $@
+	python3 -c 'import __graft_entry__ as g; g._mark(g.HIP_LIB, g.source_id(g.HIP_LIB))'
 tests/emu/libgigagan_amd_emu.so: $(UNITS:%=build/%_emu.o) build/gg_emu.o
 	$(HOSTCXX) -shared -fPIC $^ -o $@
+	python3 -c 'import __graft_entry__ as g; g._mark(g.EMU_LIB, g.source_id(g.EMU_LIB))'
 
 clean:
 	rm -f build/*.o gigagan_pytorch_amd/libgigagan_amd.so tests/emu/libgigagan_amd_emu.so

@@ -44,7 +44,8 @@ _built = False
 
 
 def _ensure_built():
-    """build the native artefacts once per session where there are none (after a change to a source: build again by hand first)."""
+    """build the native artefacts once per session where there are none. After a change to a source build again by hand first: libraries of
+    other sources are named in the header and fail test_build.py."""
     global _built
     if _built or os.environ.get('PYTEST_XDIST_WORKER'):
         return
@@ -52,6 +53,12 @@ def _ensure_built():
     if not (EMU_LIB.exists() and HIP_LIB.exists()):
         import __graft_entry__ as g
         g.build()
+
+
+def pytest_report_header(config):
+    import __graft_entry__ as g
+    return [f'STALE: {lib.relative_to(ROOT)} was built from other sources than these; call __graft_entry__.build()'
+            for lib in (EMU_LIB, HIP_LIB) if g.is_current(lib) is False]
 
 
 @pytest.fixture(autouse=True)
