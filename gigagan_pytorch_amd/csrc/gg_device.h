@@ -177,14 +177,14 @@ GG_DEVICE void gg_bufs_load_lds16(GgBufS r, unsigned voff, unsigned soff, void* 
     const unsigned so = __builtin_amdgcn_readfirstlane(soff);
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds" ::"v"(voff), "s"(r), "s"(m), "s"(so) : "memory");
 }
+// a value the compiler must take as new here (it cannot hoist what is computed from it above this point)
+GG_DEVICE void gg_opaque(unsigned& v) { asm volatile("" : "+v"(v)); }
+// nothing is scheduled across this point: a software pipeline written out in the source keeps its order (left to itself the compiler
+// sinks every LDS read to its use to save registers, and each use then waits for the LDS)
+GG_DEVICE void gg_sched_fence() { __builtin_amdgcn_sched_barrier(0); }
 // hand-over of LDS data between the lanes of ONE wave (a wave-private staging area): the hardware executes a wave's LDS instructions
 // in order, so nothing is emitted - the builtin only pins the compiler's schedule; the emulator, whose lanes are independent fibers,
 // makes it a wave rendezvous
-// nothing is scheduled across this point: a software pipeline written out in the source keeps its order (left to itself the compiler
-// sinks every LDS read to its use to save registers, and each use then waits for the LDS)
-// a value the compiler must take as new here (it cannot hoist what is computed from it above this point)
-GG_DEVICE void gg_opaque(unsigned& v) { asm volatile("" : "+v"(v)); }
-GG_DEVICE void gg_sched_fence() { __builtin_amdgcn_sched_barrier(0); }
 GG_DEVICE void gg_wave_sync() { __builtin_amdgcn_wave_barrier(); }
 // a 16-byte store marked non-temporal (global_store_dwordx4 ... nt): a streamed output row does not displace the operand tiles that the
 // same workgroups keep re-reading from this XCD's L2 (gg_pgemm.h)

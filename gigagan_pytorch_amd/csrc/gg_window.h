@@ -889,9 +889,6 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dq_kernel(GgWinParams p) {
 }
 
 // ---- backward, part 2: dk, dv -----------------------------------------------------------------------------------------
-// workgroup: 4 waves x 32 keys, row tiles of 64 (Q and dO by LDS-DMA, double buffered, each read as rows and transposed). The key tiles that hold sinks are seen by
-// every later row (and where there are few key tiles, every one): their rows are cut into p.sink_chunks chunks, each a workgroup of its own that leaves fp32 sums for
-// gg_win_sink_kernel.  part_o: [B*hk][sink_tiles][chunks][2][128][D].
 // the rows ra .. rb that see some key of the 128-key tile at k0, or their part `chunk` of `chunks` (whole 64-row tiles); none: ra > rb.
 // Compared as tokens before they become rows: keys far in front of every query are a token that, times g, 32 bits do not hold.
 struct GgwRows { int ra, rb; };
@@ -954,6 +951,10 @@ GG_DEVICE void ggw_fix_dkv(const GgWinParams& p, const unsigned short* qb, const
         }
 }
 
+// workgroup: 4 waves x 32 keys, row tiles of 64 (Q and dO by LDS-DMA, double buffered, each read as rows and transposed). The key tiles
+// that hold sinks are seen by every later row: where the chip needs it their rows are cut into p.sink_chunks chunks, each a workgroup of
+// its own that leaves fp32 sums for gg_win_sink_kernel; where there are few key tiles, every tile's are (gg_win_plan).
+// part_o: [B*hk][sink_tiles][chunks][2][128][D].
 template <int T, int D>
 GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
     constexpr int KK = D / 16, DB = D / 32;
@@ -1038,7 +1039,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
     const GgwLane lanes = ggw_lane<D>();
     float r_lse = 0.f, r_d = 0.f;
     int r_pos = 0;
-    bool far = false;
+    unsigned long long far = 0;             // (wave-uniform)
     auto fetch = [&](int i0, int buf) {
         const GgBufS bq = gg_make_bufs(qb + (unsigned long long)(unsigned)ft * p.qn, GGW_SPAN), bg = gg_make_bufs(gb + (unsigned long long)(unsigned)ft * p.gn, GGW_SPAN);
         const bool all = i0 + 63 <= rb;
@@ -1087,7 +1088,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
         ct += step_t;
         ch += step_h;
         if (ch >= p.g) { ch -= p.g; ++ct; }
-        far |= ggw_far(r_lse);          // (not where it is loaded: nothing waits for it there)
+        far |= gg_ballot(ggw_far(r_lse));           // (not where it is loaded: nothing waits for it there)
         if (threadIdx.x < 64) { sLse[buf][threadIdx.x] = r_lse - (float)PE; sD[buf][threadIdx.x] = r_d; sPos[buf][threadIdx.x] = r_pos; }
         gg_wait_vm<0>();
         gg_barrier_lds();
@@ -1152,7 +1153,7 @@ GG_KERNEL GG_LAUNCH_BOUNDS2(256, 2) void gg_win_dkv_kernel(GgWinParams p) {
                 dkt[db][r] *= ggw_pow2(-sc.e);
                 dvt[db][r] *= ggw_pow2(-PE);
             }
-    const unsigned bad = gg_wave_any(far) ? ~0u : ggw_not_finite<2 * DB>(acc);       // (a far row may have reached any key)
+    const unsigned bad = far ? ~0u : ggw_not_finite<2 * DB>(acc);       // (a far row may have reached any key)
     if (__builtin_expect(bad != 0, 0))
         for (int k = 0; k < 32; ++k) {
             const int j = kj0 + k;

@@ -1,5 +1,5 @@
 """Registers, scratch and LDS of every kernel in the product library as hipcc allocates them (cross-compiles without a GPU):
-    python tests/kernel_resource_report.py [--all]
+    python tests/kernel_resource_report.py [--all] [unit ...]        (units: gg_api, gg_transformer; both where none is named)
 prints the kernels that spill to scratch, sit at the 256-VGPR cap or hold more than 64 KB of LDS (--all: every kernel). This is the
 listing that found gg_aconv's spilling 4x4 form and the register headroom for gg_conv3's two-workgroups-per-CU tile in round 6
 (test infrastructure)."""
@@ -11,10 +11,14 @@ from pathlib import Path
 
 ROOT = Path(__file__).resolve().parents[1]
 CSRC = ROOT / 'gigagan_pytorch_amd' / 'csrc'
+units = [a for a in sys.argv[1:] if not a.startswith('-')] or ['gg_api', 'gg_transformer']
 with tempfile.TemporaryDirectory() as tmp:
-    cmd = ['hipcc', '--offload-arch=gfx950', '-O3', '-std=c++17', '-mllvm', '-amdgpu-mfma-vgpr-form', f'-I{ROOT / "include"}', f'-I{CSRC}',
-           '-Rpass-analysis=kernel-resource-usage', '-c', str(CSRC / 'gg_api.hip'), '-o', f'{tmp}/a.o']
-    txt = subprocess.run(cmd, capture_output=True, text=True).stderr
+    txt = ''
+    for unit in units:
+        cmd = ['hipcc', '--offload-arch=gfx950', '-O3', '-std=c++17', '-mllvm', '-amdgpu-mfma-vgpr-form', '-Xclang', '-target-feature', '-Xclang',
+               '-packed-fp32-ops', '-DGG_UNITS', f'-I{ROOT / "include"}', f'-I{CSRC}', '-Rpass-analysis=kernel-resource-usage', '-c',
+               str(CSRC / f'{unit}.hip'), '-o', f'{tmp}/a.o']
+        txt += subprocess.run(cmd, capture_output=True, text=True).stderr
 rows = []
 for blk in re.split(r'remark: Function Name: ', txt)[1:]:
     def field(key):

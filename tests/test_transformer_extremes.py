@@ -53,13 +53,13 @@ def softmax_grads(q, k, v, do, scale, ok):
 
 @where
 @shapes
-@pytest.mark.parametrize('exponent', [21, 105])
+@pytest.mark.parametrize('dtype,exponent', [('bf16', 21), ('bf16', 105), ('fp16', 21)])
 @pytest.mark.parametrize('sign', [-1, 1])
-def test_far_scores(where, n, m, exponent, sign):
+def test_far_scores(where, n, m, dtype, exponent, sign):
     """scores of 2^21 and 2^105 on either side, far below and above where a running maximum might start: equal ones share the probability
     (exactly: the products are powers of two), one half as large in magnitude takes it all or has none, and so do the gradients"""
     g = gen(21, where)
-    q, k, v, do = (t.clone() for t in qkv(1, 2, 1, n, m, 32, 'bf16', g))
+    q, k, v, do = (t.clone() for t in qkv(1, 2, 1, n, m, 32, dtype, g))
     q.zero_()
     k.zero_()
     q[..., 3] = 2.0 ** (exponent // 2)
@@ -72,7 +72,7 @@ def test_far_scores(where, n, m, exponent, sign):
     o = ops.impl.window_attention(*leaves, scale=1.0, window=window)
     got = [o, *torch.autograd.grad(o, leaves, do)]
     ref = softmax_grads(q, k, v, do, 1.0, ok)
-    u = half_step(torch.bfloat16)
+    u = half_step(DT[dtype])
     P = (torch.where(ok[:, None], q.double() @ k.double().mT, torch.full((), -1e300, dtype=torch.float64, device=where))).softmax(-1) * ok[:, None]
     # the row's pass is fp32: 2^-18 covers its sums of up to 600 terms; o's own rounding is kept for D. The results are rounded once.
     e = 2.0 ** -18
