@@ -482,8 +482,10 @@ GG_DEVICE void ggw_fix_rows(const GgWinParams& p, const GgwWave& w, const GgwRan
 }
 
 // workgroup: 4 waves x 32 rows; key tiles of 64 fetched once for all of them by LDS-DMA, double buffered: one barrier a tile, behind
-// which the next tile's transfers start and run under this tile's arithmetic. What bounds it is the LDS: every product takes a kilobyte
-// operand from it (32768 tokens, window 4096, 32 heads on 8 of 128: without those reads 1515 of 2145 us, without the softmax 1751, without the transfers 1875). Measured and
+// which the next tile's transfers start and run under this tile's arithmetic. No unit bounds it alone (32768 tokens, window 4096, 32 heads
+// on 8 of 128: matrix pipe busy 54 % of the time, vector ALU 52 %, two waves a SIMD; without the operand reads from the LDS - a kilobyte
+// a product - 1515 of 2145 us, without the softmax 1751, without the transfers 1875); at 64 features the softmax leads (vector ALU
+// 62 %, matrix pipe 32 %). Measured and
 // not kept: two 32-row blocks a wave for each operand read (half the reads, but one wave a SIMD: 2604 against 2010 in the same run),
 // eight waves a tile in two groups half a tile apart (2334 against 2114), wave priorities (no change).
 // SPLIT: the tiles are dealt out to p.splits workgroups, which leave (m, l, O) for gg_win_join_kernel.

@@ -2044,14 +2044,16 @@ class HipOps:
     def window_attention(self, q, k, v, *, scale, window=(None, None), sinks=0, key_mask=None, lengths=None):
         """attention with a sliding window and a few first keys (sinks) that stay visible.
 
-        q (B, h, n, d), k and v (B, hk, m, d), h a multiple of hk (grouped heads), d 32, 64 or 128, bf16 or fp16, any strides. The queries
+        q (B, h, n, d), k and v (B, hk, m, d), h a multiple of hk (grouped heads, 65504 a key head at most), d 32, 64 or 128, bf16 or
+        fp16, any strides. The queries
         are the LAST n of a sequence: query i of item b sits at position p = lengths[b] - n + i (lengths (B,) int32 or int64 on the
         device, at most m; m without) and sees key j when j < lengths[b], p - left <= j or j < sinks, j <= p + right, and key_mask[b, j]
         ((B, m) bool, optional). window = (left, right), None = no bound; (None, 0) is causal attention; n = 1 is a decoding step on a
         cache. A query that sees no key, and one at a negative position, gets zeros and no gradient. What lies in k and v where no
-        query sees it (stale slots, NaN padding) does not reach the result.
+        query sees it (stale slots, NaN padding) does not reach the result; what a query sees does, with a probability of zero too.
 
-        Returns (B, h, n, d), a view of (B, n, h, d) storage. First-order gradients for q, k and v."""
+        Returns (B, h, n, d), a view of (B, n, h, d) storage. First-order gradients for q, k and v: differentiating them raises, and so do
+        forward-mode derivatives."""
         for name, t in (('q', q), ('k', k), ('v', v)):
             if t.dim() != 4:
                 raise ValueError(f'window_attention: {name} must be (B, heads, tokens, features), got {tuple(t.shape)}')
@@ -2134,7 +2136,8 @@ class HipOps:
     def layer_norm(self, x, weight, bias=None, eps=1e-5):
         """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (..., C): bf16, fp16 or fp32 rows, the result in x's
         type and contiguous; weight and bias (C,) in any floating type, their gradients summed in fp32. 0 < C <= 16384. Rows with one
-        pitch are read where they lie; other layouts are copied first. First-order gradients."""
+        pitch are read where they lie; other layouts are copied first. First-order gradients: differentiating them raises, and so do
+        forward-mode derivatives."""
         C = x.shape[-1] if x.dim() else 0
         if not 0 < C <= K.LAYERNORM_MAX_C:
             raise ValueError(f'layer_norm: last axis of 1 to {K.LAYERNORM_MAX_C} features expected, got shape {tuple(x.shape)}')
@@ -2155,8 +2158,8 @@ class HipOps:
         q (B, h, n, d), optional k (B, hk, n, d) of q's type (fewer heads allowed): bf16, fp16 or fp32, any strides. positions: int32,
         int64 or fp32, (n, axes) for the whole batch or (B, n, axes); `spec` a RotarySpec (sections of feature pairs per axis,
         theta, pairing). Angles are taken in fp64, so far positions keep their precision. Returns the turned q, or (q, k), as (B, heads, n, d)
-        views of (B, n, heads, d) storage - the layout the attention entry points read without a copy. Differentiable any number of times;
-        positions get no gradient."""
+        views of (B, n, heads, d) storage - the layout the attention entry points read without a copy. Differentiable any number of times
+        (forward-mode derivatives raise); positions get no gradient."""
         if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:])):
             raise ValueError(f'rotary: q (B, h, n, d) and k (B, hk, n, d) expected, got {tuple(q.shape)}'
                              + ('' if k is None else f' and {tuple(k.shape)}'))
