@@ -1,7 +1,7 @@
 """Registers, scratch and LDS of every kernel in the product library as hipcc allocates them (cross-compiles without a GPU):
     python tests/kernel_resource_report.py [--all] [unit ...]        (units: gg_api, gg_transformer; both where none is named)
 prints the kernels that spill to scratch, sit at the 256-VGPR cap or hold more than 64 KB of LDS (--all: every kernel). This is the
-listing that found gg_aconv's spilling 4x4 form and the register headroom for gg_conv3's two-workgroups-per-CU tile in round 6
+listing that found gg_aconv's spilling 4x4 form and the register headroom for gg_conv3's two-workgroups-per-CU tile
 (test infrastructure)."""
 import re
 import subprocess
