@@ -355,8 +355,8 @@ GG_DEVICE void ggw_store_o(const GgWinParams& p, long long at, f32x4 x) {
     if (p.o_lo) *(u16x4*)(p.o_lo + at) = lo;
 }
 // A row that saw no key: zeros, and +inf for its log-sum-exp (its P is zero everywhere in the backward). A row that saw keys and has
-// l = 0 saw scores of -inf alone: NaN. Where a row's parts
-// are joined, a row that saw no key has the maximum -inf, any other GGW_LOW or more in some part.
+// l = 0 saw scores of -inf alone: NaN. Where a row's parts are joined, one that saw no key has the maximum -inf in all of them, any other
+// GGW_LOW or more in some.
 GG_DEVICE float ggw_inverse(float l, bool saw) { return l == 0.f ? (saw ? __builtin_nanf("") : 0.f) : 1.f / l; }
 GG_DEVICE bool ggw_far(float m) { return fabsf(m) >= GGW_FAR && fabsf(m) < __builtin_inff(); }
 GG_DEVICE float ggw_lse(float m, float l, bool saw) {

@@ -80,3 +80,29 @@ def test_fused_attention_differentiated_twice(where, null, masked, n, m):
     ref = second(plain, [t.float().requires_grad_() for t in leaves])
     for a, b in zip(got, ref):
         assert rel_err(a, b) < TOL / 2           # one operator: P, dP, dS and the results rounded to bf16, twice
+
+
+@pytest.mark.gpu
+def test_trainer_with_dot_product_attention_on_a_small_map(tmp_path):
+    """the captured training step, its gradient penalty through 8 x 8 maps of dot-product attention, eager and as captured graphs"""
+    from gigagan_pytorch_amd import GigaGAN
+    from gigagan_pytorch_amd.data import SyntheticImages
+    from gigagan_pytorch_amd.gigagan import cycle
+    losses = []
+    for graphs in (False, True):
+        torch.manual_seed(0)
+        gan = GigaGAN(generator=dict(image_size=32, dim_capacity=8, dim_max=64, style_network=dict(dim=64, depth=2), unconditional=True),
+                      discriminator=dict(image_size=32, dim_capacity=8, dim_max=64, attn_resolutions=(8,), attn_heads=2, self_attn_dot_product=True,
+                                         self_attn_rotary=True, unconditional=True),
+                      amp=True, mixed_precision_type='bf16', apply_gradient_penalty_every=2, use_hip_graphs=graphs, device=torch.device('cuda', 0),
+                      model_folder=str(tmp_path / f'm{graphs}'), results_folder=str(tmp_path / f'r{graphs}'))
+        assert any(getattr(m, 'dot_product', False) for m in gan.D.modules())
+        it = cycle(SyntheticImages(4, 32, device=torch.device('cuda', 0)))
+        torch.manual_seed(1)
+        runs = []
+        for _ in range(6):
+            d, g = gan.train_step(it, 4)
+            runs.append([float(v) for v in (*d, *g) if v is not None])
+        assert all(abs(v) < float('inf') for r in runs for v in r)
+        losses.append(runs)
+    assert len(losses[0]) == len(losses[1]) and all(len(a) == len(b) for a, b in zip(*losses))
