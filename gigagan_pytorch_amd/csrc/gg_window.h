@@ -348,8 +348,12 @@ GG_DEVICE void ggw_store_o(const GgWinParams& p, long long at, f32x4 x) {
     u16x4 hi, lo;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        hi[e] = gg_elt<T>(x[e]);
-        lo[e] = gg_elt<T>(x[e] - gg_elt_f<T>(hi[e]));
+        // (what is stored and what is taken off are one conversion: left to itself the compiler rounds the product with 1 / l to half twice,
+        // fused for the store and from fp32 for the difference, and near a tie the two are a unit in the last place apart)
+        unsigned h = gg_elt<T>(x[e]);
+        gg_opaque(h);
+        hi[e] = (unsigned short)h;
+        lo[e] = gg_elt<T>(x[e] - gg_elt_f<T>((unsigned short)h));
     }
     *(u16x4*)(p.o + at) = hi;
     if (p.o_lo) *(u16x4*)(p.o_lo + at) = lo;

@@ -5,17 +5,19 @@ import math
 import pytest
 import torch
 
+from gigagan_pytorch_amd import kernels as K
 from gigagan_pytorch_amd import ops
 from test_transformer_ops import DT, att_ref, gen, half_step, normal, qkv, seen, within
 
 WHERE = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
 where = pytest.mark.parametrize('where', WHERE)
-# queries and keys for the three forward kernels: many rows, few rows, few rows with the keys split over workgroups
+# queries and keys for the forward kernels: many rows, few rows, few rows with the keys split over workgroups; on the GPU many rows with
+# the keys split, and dk / dv in row chunks besides
 SHAPES = [(34, 70), (3, 70), (1, 600)]
-shapes = pytest.mark.parametrize('n,m', SHAPES)
+shapes = pytest.mark.parametrize('where,n,m', [('cpu', *s) for s in SHAPES]
+                                 + [pytest.param('cuda', *s, marks=pytest.mark.gpu) for s in SHAPES + [(40, 2000), (300, 300)]])
 
 
-@where
 @shapes
 @pytest.mark.parametrize('fill', [math.nan, math.inf])
 def test_a_value_of_underflowed_probability_counts(where, n, m, fill):
@@ -51,7 +53,6 @@ def softmax_grads(q, k, v, do, scale, ok):
     return [o.detach(), *torch.autograd.grad(o, (q, k, v), do.double())]
 
 
-@where
 @shapes
 @pytest.mark.parametrize('dtype,exponent', [('bf16', 21), ('bf16', 105), ('fp16', 21)])
 @pytest.mark.parametrize('sign', [-1, 1])
@@ -88,7 +89,6 @@ def test_far_scores(where, n, m, dtype, exponent, sign):
         assert torch.equal(ops.impl.window_attention(*leaves, scale=1.0, window=window), o)
 
 
-@where
 @shapes
 def test_scores_of_minus_infinity_alone(where, n, m):
     """a query whose seen keys all score -inf has 0 / 0 as in any softmax, one that sees no key zeros; a single finite score among them takes all"""
@@ -176,3 +176,23 @@ def test_row_sums_from_the_unrounded_output(where, dtype):
     rounded = (G * o.to(dt).double()).sum(-1, keepdim=True)
     lost = (rounded - D).abs() * K.mean(2, keepdim=True).abs()
     assert (lost > 2 * (eS @ K.abs())).any()            # what the case would show
+
+
+@shapes
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+def test_the_output_in_two_words(n, m, where, dtype):
+    """o and what its rounding took off add up to o as fp32 had it, near a tie of the rounding too: scores of zero make P a constant and o a mean of
+    up to 2000 values"""
+    g = gen(26, where)
+    dt = DT[dtype]
+    q = torch.zeros((1, 2, n, 32), dtype=dt, device=where)
+    k, v = normal((1, 1, m, 32), dt, g), normal((1, 1, m, 32), dt, g)
+    o, o_lo, _ = K.window_fwd(q, k, v, 1.0, -1, 0, 0, None, None, True)
+    seen_keys = torch.arange(m - n + 1, m + 1, device=where, dtype=torch.float64)[:, None]
+    V = v.double()[0, 0]
+    ref = (V.cumsum(0)[m - n:] / seen_keys).expand(1, 2, n, 32)
+    size = (V.abs().cumsum(0)[m - n:] / seen_keys).expand(1, 2, n, 32)
+    # the second word is rounded by u of it, which is u of o at most (half: by 2^-25 at least); sums of fp32 in tiles of 64, 1 / l and the product
+    u = half_step(dt)
+    tol = u * u * ref.abs() + (2.0 ** -25 if dtype == 'fp16' else 0.0) + (64 + m / 64 + 8) * 2.0 ** -24 * size
+    within(o.double() + o_lo.transpose(1, 2).double(), ref, tol)
